@@ -257,6 +257,93 @@ typedef struct mxb200_gemm_desc {
 MXB200_API size_t mxb200_gemm_group_workspace_bytes(const mxb200_gemm_desc* g, int n);
 MXB200_API int mxb200_gemm_group(const mxb200_gemm_desc* g, int n, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- Blocks of 128 values with one fp32 scale (no counterpart in the reference) --------------------------------------------
+ * E4M3 with one fp32 scale for 128 values: 128 columns of a row of an activation, 128 x 128 values of a weight, 128 tokens of a
+ * column for the operands of a weight gradient. A last block may be shorter. The scales that the quantizers make are the
+ * smallest powers of two s >= 2^-126 with max|block| <= 448 s (MXB200_SCALE_REFERENCE's rule); the products take any fp32
+ * scales, e.g. those of a quantized checkpoint. NaN stays NaN and does not count in a maximum, Inf saturates to 448 s.
+ *
+ * Rows may be sorted by expert: expert e of `experts` (<= 1024) has rows [ends[e - 1], ends[e]), ends being int32 on the
+ * device, never read on the host; an end is held to between the previous expert's and the number of rows. Rows behind the last
+ * end are nobody's. ends null (experts = 1): one expert has all rows. Features are multiples of 16, rows may be any number.
+ * All pointers 16-byte aligned (ends, and the scales that a product reads: 4).
+ *
+ * Token blocks: how many blocks of 128 rows the tokens of `experts` experts take at most, each expert's starting a new one; the
+ * operands of a weight gradient have 128 times as many rows. */
+MXB200_API int64_t mxb200_block_token_blocks(int64_t tokens, int experts);
+
+/* x: (rows, cols) bf16 with ld >= cols values between rows (ld % 8 == 0). row_data (rows, cols) e4m3 and row_scale
+ * (ceil(cols / 128), rows): blocks along rows. token_data (128 * token blocks, cols) and token_scale (token blocks, cols): blocks
+ * along each expert's tokens, whose last block is filled up with zeros. Either may be null. With token_data, rows of no expert
+ * are written to neither. */
+MXB200_API int mxb200_block_quantize(const void* x, int64_t rows, int64_t cols, int64_t ld, const int32_t* ends, int experts,
+                                     void* row_data, float* row_scale, void* token_data, float* token_scale, void* stream);
+
+/* w: (experts, rows, cols) contiguous, bf16 (w_bf16 != 0) or fp32, to data of that shape and scale
+ * (experts, ceil(rows / 128), ceil(cols / 128)). */
+MXB200_API int mxb200_block_quantize_weight(const void* w, int w_bf16, int experts, int64_t rows, int64_t cols, void* data,
+                                            float* scale, void* stream);
+
+typedef enum mxb200_block_kind {
+  MXB200_BLOCK_FORWARD = 0,     /* d (tokens, out) bf16 = b (tokens, in), rows . a (experts, out, in)^T, weight */
+  MXB200_BLOCK_INPUT_GRAD = 1,  /* d (tokens, in) bf16 = b (tokens, out), rows . a (experts, out, in), weight */
+  MXB200_BLOCK_WEIGHT_GRAD = 2  /* d (experts, out, in) bf16 or fp32 = a (., out)^T, tokens . b (., in), tokens */
+} mxb200_block_kind;
+
+/* One product per expert over its rows, fp32 accumulation, rounded once. Rows of no expert: zeros; the weight gradient of an
+ * expert without rows: zeros. Needs no workspace. tokens may be 0. */
+typedef struct mxb200_block_gemm_args {
+  const void* a;
+  const float* a_scale;
+  const void* b;
+  const float* b_scale;
+  void* d;
+  const int32_t* ends;
+  int64_t tokens, in_features, out_features;
+  int32_t experts;
+  int32_t kind;     /* mxb200_block_kind */
+  int32_t out_kind; /* mxb200_out_kind; F32 for the weight gradient only */
+} mxb200_block_gemm_args;
+MXB200_API int mxb200_block_gemm(const mxb200_block_gemm_args* args, void* stream);
+
+/* RMS norm behind a residual add, its result also in blocks of 128 along rows. All matrices (rows, cols) contiguous bf16,
+ * cols % 16 == 0 and <= 16384, any number of rows.
+ *   res = bf16(x + r); rstd = 1 / sqrt(mean(res^2) + eps); n = bf16(res * rstd * gain); q, scale as mxb200_block_quantize of n.
+ * Without r, res is x itself and not written (both null). */
+typedef struct mxb200_block_norm_args {
+  const void* x;
+  const void* r;    /* optional, with res */
+  const void* gain; /* optional: (cols) fp32, or bf16 where gain_bf16 != 0 */
+  void* res;
+  void* n;          /* optional */
+  void* q;          /* (rows, cols) e4m3 */
+  float* scale;     /* (ceil(cols / 128), rows) */
+  float* rstd;      /* (rows) */
+  int64_t rows;
+  int32_t cols;
+  int32_t gain_bf16;
+  float eps;
+} mxb200_block_norm_args;
+MXB200_API int mxb200_block_norm_fwd(const mxb200_block_norm_args* args, void* stream);
+
+/* Its backward: with d = dn * gain, hat = res * rstd: dx = bf16(rstd * (d - hat * mean(d * hat)) + dres), the gradient of x and
+ * of r; dgain = sum over rows of dn * hat, in gain's type, in a fixed order. workspace (dgain only): at least
+ * mxb200_block_norm_workspace_bytes, 16-byte aligned, uninitialised, reusable by later calls on the same stream. */
+typedef struct mxb200_block_norm_bwd_args {
+  const void* dn;
+  const void* dres; /* optional: what else reaches res */
+  const void* res;
+  const float* rstd;
+  const void* gain; /* optional */
+  void* dx;
+  void* dgain;      /* optional, with gain */
+  int64_t rows;
+  int32_t cols;
+  int32_t gain_bf16;
+} mxb200_block_norm_bwd_args;
+MXB200_API size_t mxb200_block_norm_workspace_bytes(int64_t rows, int32_t cols);
+MXB200_API int mxb200_block_norm_bwd(const mxb200_block_norm_bwd_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Static message for a status (the reference's seam returns const char* messages, mx_gemm_kernel.h:12). */
 MXB200_API const char* mxb200_strerror(int status);
 

@@ -16,6 +16,7 @@ ERR_SHAPE, ERR_ALIGNMENT, ERR_NULL, ERR_ARGUMENT, ERR_WORKSPACE, ERR_DEVICE, ERR
 SCALE_REFERENCE, SCALE_OCP_FLOOR = 0, 1
 PROLOGUE_NONE, PROLOGUE_RELU_SQUARE = 0, 1
 OUT_BF16, OUT_F32 = 0, 1
+BLOCK_FORWARD, BLOCK_INPUT_GRAD, BLOCK_WEIGHT_GRAD = 0, 1, 2
 STATIC_SCRATCH_BYTES = 32 << 20
 
 # every symbol include/mxb200.h declares
@@ -27,6 +28,8 @@ SYMBOLS = (
     "mxb200_count_valid", "mxb200_reduce_losses", "mxb200_scale_bf16",
     "mxb200_gemm_group_workspace_bytes", "mxb200_gemm_group",
     "mxb200_gemm_splits", "mxb200_gemm_workspace_bytes", "mxb200_gemm_splitk", "mxb200_gemm_splitk_static",
+    "mxb200_block_token_blocks", "mxb200_block_quantize", "mxb200_block_quantize_weight", "mxb200_block_gemm",
+    "mxb200_block_norm_fwd", "mxb200_block_norm_workspace_bytes", "mxb200_block_norm_bwd",
     "mxb200_strerror",
     "mxb200_device_status", "mxb200_selftest_bounded_wait", "mxb200_set_gemm_config", "mxb200_launch_count", "mxb200_version",
 )
@@ -62,6 +65,28 @@ class GemmDesc(ctypes.Structure):
     _fields_ = [("a", ctypes.c_void_p), ("a_scale", ctypes.c_void_p), ("b", ctypes.c_void_p), ("b_scale", ctypes.c_void_p),
                 ("d", ctypes.c_void_p), ("resid", ctypes.c_void_p), ("alpha", ctypes.c_void_p), ("M", ctypes.c_int64),
                 ("N", ctypes.c_int64), ("K", ctypes.c_int64), ("out_kind", ctypes.c_int32), ("accumulate", ctypes.c_int32)]
+
+
+class BlockGemmArgs(ctypes.Structure):
+    """mxb200_block_gemm_args."""
+    _fields_ = [("a", ctypes.c_void_p), ("a_scale", ctypes.c_void_p), ("b", ctypes.c_void_p), ("b_scale", ctypes.c_void_p),
+                ("d", ctypes.c_void_p), ("ends", ctypes.c_void_p), ("tokens", ctypes.c_int64), ("in_features", ctypes.c_int64),
+                ("out_features", ctypes.c_int64), ("experts", ctypes.c_int32), ("kind", ctypes.c_int32),
+                ("out_kind", ctypes.c_int32)]
+
+
+class BlockNormArgs(ctypes.Structure):
+    """mxb200_block_norm_args."""
+    _fields_ = [("x", ctypes.c_void_p), ("r", ctypes.c_void_p), ("gain", ctypes.c_void_p), ("res", ctypes.c_void_p),
+                ("n", ctypes.c_void_p), ("q", ctypes.c_void_p), ("scale", ctypes.c_void_p), ("rstd", ctypes.c_void_p),
+                ("rows", ctypes.c_int64), ("cols", ctypes.c_int32), ("gain_bf16", ctypes.c_int32), ("eps", ctypes.c_float)]
+
+
+class BlockNormBwdArgs(ctypes.Structure):
+    """mxb200_block_norm_bwd_args."""
+    _fields_ = [("dn", ctypes.c_void_p), ("dres", ctypes.c_void_p), ("res", ctypes.c_void_p), ("rstd", ctypes.c_void_p),
+                ("gain", ctypes.c_void_p), ("dx", ctypes.c_void_p), ("dgain", ctypes.c_void_p), ("rows", ctypes.c_int64),
+                ("cols", ctypes.c_int32), ("gain_bf16", ctypes.c_int32)]
 
 
 class Mxb200Error(RuntimeError):
@@ -100,6 +125,15 @@ def _load() -> ctypes.CDLL:
     lib.mxb200_gemm_workspace_bytes.restype = ctypes.c_size_t
     lib.mxb200_gemm_splitk.argtypes = [vp, vp, vp, vp, vp, i32, vp, i64, i64, i64, vp, i32, i32, vp, ctypes.c_size_t, vp]
     lib.mxb200_gemm_splitk_static.argtypes = [vp, vp, vp, vp, vp, i32, vp, i64, i64, i64, vp, i32, i32, vp]
+    lib.mxb200_block_token_blocks.argtypes = [i64, i32]
+    lib.mxb200_block_token_blocks.restype = i64
+    lib.mxb200_block_quantize.argtypes = [vp, i64, i64, i64, vp, i32, vp, vp, vp, vp, vp]
+    lib.mxb200_block_quantize_weight.argtypes = [vp, i32, i32, i64, i64, vp, vp, vp]
+    lib.mxb200_block_gemm.argtypes = [ctypes.POINTER(BlockGemmArgs), vp]
+    lib.mxb200_block_norm_fwd.argtypes = [ctypes.POINTER(BlockNormArgs), vp]
+    lib.mxb200_block_norm_workspace_bytes.argtypes = [i64, ctypes.c_int32]
+    lib.mxb200_block_norm_workspace_bytes.restype = ctypes.c_size_t
+    lib.mxb200_block_norm_bwd.argtypes = [ctypes.POINTER(BlockNormBwdArgs), vp, ctypes.c_size_t, vp]
     lib.mxb200_selftest_bounded_wait.argtypes = [ctypes.c_uint64, vp]
     lib.mxb200_strerror.argtypes = [i32]
     lib.mxb200_strerror.restype = ctypes.c_char_p

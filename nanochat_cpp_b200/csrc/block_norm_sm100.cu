@@ -1,0 +1,423 @@
+// RMS norm behind a residual add, its result in the 128-value block format, and its backward.
+//
+//   res = bf16(x + r),  rstd = 1 / sqrt(mean(res^2) + eps),  n = bf16(res rstd gain),  (q, scale) = rows of n in blocks of 128
+//   d = dn gain,  hat = res rstd,  dx = bf16(rstd (d - hat mean(d hat)) + dres)  (of x and of r),  dgain = sum over rows of dn hat
+//
+// A row lies in the registers of its threads from load to store, so every tensor is read or written once; both kernels are
+// bound by memory. A row of up to 2048 columns belongs to one warp, whose sums are shuffles, a wider one (up to 16384) to 256
+// threads. 16 lanes hold 128 consecutive values, one scale block. Sums, rstd and the gain's gradient are fp32.
+//
+// The gain's gradient: every CTA adds up its rows in a fixed order in registers and writes one row of partial sums; a second
+// kernel adds those rows in order. No atomics: the same bits every time.
+#include <algorithm>
+#include <cstdint>
+
+#include <cuda_bf16.h>
+
+#include "bf16x2_sm100.cuh"
+#include "block_common.cuh"
+#include "internal.h"
+#include "ptx_sm100.cuh"
+
+namespace mxb200 {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWarpCols = 2048, kMaxCols = 16384;
+
+struct ForwardParams {
+  const void* x;
+  const void* r;
+  const void* gain;
+  void* res;
+  void* n;
+  uint8_t* q;
+  float* scale;
+  float* rstd;
+  int64_t rows;
+  int cols;
+  int gain_bf16;
+  float eps;
+};
+
+struct BackwardParams {
+  const void* dn;
+  const void* dres;
+  const void* res;
+  const float* rstd;
+  const void* gain;
+  void* dx;
+  float* partial;  // (gridDim.x, cols); null: no gradient of the gain
+  int64_t rows;
+  int cols;
+  int gain_bf16;
+};
+
+__device__ __forceinline__ void unpack(const uint4& w, float (&f)[8]) {
+  f[0] = lo_f32(w.x), f[1] = hi_f32(w.x), f[2] = lo_f32(w.y), f[3] = hi_f32(w.y);
+  f[4] = lo_f32(w.z), f[5] = hi_f32(w.z), f[6] = lo_f32(w.w), f[7] = hi_f32(w.w);
+}
+
+__device__ __forceinline__ uint4 pack(const float (&f)[8]) {
+  return make_uint4(pack_bf16x2_rn(f[0], f[1]), pack_bf16x2_rn(f[2], f[3]), pack_bf16x2_rn(f[4], f[5]), pack_bf16x2_rn(f[6], f[7]));
+}
+
+__device__ __forceinline__ uint4 load16(const void* p, int64_t at) {
+  return *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p) + at);
+}
+
+__device__ __forceinline__ void store16(void* p, int64_t at, const uint4& w) {
+  *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p) + at) = w;
+}
+
+__device__ __forceinline__ void load_gain(const void* gain, int gain_bf16, int col, float (&g)[8]) {
+  if (gain == nullptr) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      g[k] = 1.f;
+  } else if (gain_bf16) {
+    unpack(load16(gain, col), g);
+  } else {
+    const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(gain) + col);
+    const float4 a = q[0], b = q[1];
+    g[0] = a.x, g[1] = a.y, g[2] = a.z, g[3] = a.w, g[4] = b.x, g[5] = b.y, g[6] = b.z, g[7] = b.w;
+  }
+}
+
+// Sum over the threads of a row: a warp, or all of the block (`parts`: a word per warp). Every thread gets it.
+template <int kPerRow>
+__device__ __forceinline__ float row_sum(float v, float* parts) {
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1)
+    v += __shfl_xor_sync(0xffffffffu, v, d);
+  if constexpr (kPerRow > 32) {
+    __syncthreads();  // the previous row's parts have been read
+    if ((threadIdx.x & 31) == 0)
+      parts[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = 0.f;
+#pragma unroll
+    for (int w = 0; w < kPerRow / 32; ++w)
+      v += parts[w];
+  }
+  return v;
+}
+
+template <int kPerRow, int kVecs>
+__device__ __forceinline__ void norm_forward(const ForwardParams& p) {
+  __shared__ float parts[kThreads / 32];
+  grid_dependency_wait();
+  const int at = threadIdx.x % kPerRow;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads / kPerRow) + threadIdx.x / kPerRow;
+  if (row >= p.rows)
+    return;  // whole warps: a row of 256 threads is the whole block's
+  uint4 v[kVecs];
+#pragma unroll
+  for (int i = 0; i < kVecs; ++i) {
+    const int col = 8 * (i * kPerRow + at);
+    v[i] = col < p.cols ? load16(p.x, row * p.cols + col) : make_uint4(0, 0, 0, 0);
+  }
+  if (p.r != nullptr) {
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) {
+      const int col = 8 * (i * kPerRow + at);
+      if (col < p.cols) {
+        const uint4 r = load16(p.r, row * p.cols + col);
+        v[i] = make_uint4(add_bf16x2(v[i].x, r.x), add_bf16x2(v[i].y, r.y), add_bf16x2(v[i].z, r.z), add_bf16x2(v[i].w, r.w));
+        store16(p.res, row * p.cols + col, v[i]);
+      }
+    }
+  }
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < kVecs; ++i) {
+    float f[8];
+    unpack(v[i], f);
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      sum = fmaf(f[k], f[k], sum);
+  }
+  sum = row_sum<kPerRow>(sum, parts);
+  const float rstd = __frsqrt_rn(sum / static_cast<float>(p.cols) + p.eps);
+  if (at == 0)
+    p.rstd[row] = rstd;
+#pragma unroll
+  for (int i = 0; i < kVecs; ++i) {
+    const int col = 8 * (i * kPerRow + at);
+    const bool in = col < p.cols;
+    float f[8], g[8];
+    if (in)
+      load_gain(p.gain, p.gain_bf16, col, g);
+    unpack(v[i], f);
+    float m = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      f[k] = in ? f[k] * rstd * g[k] : 0.f;
+    const uint4 w = pack(f);
+    if (in && p.n != nullptr)
+      store16(p.n, row * p.cols + col, w);
+    unpack(w, f);  // what is quantized is the bf16 n
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      m = fmaxf(m, fabsf(f[k]));
+#pragma unroll
+    for (int d = 8; d > 0; d >>= 1)
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+    const int e = block_exponent(__float_as_uint(m));
+    const float by = __uint_as_float(mx_multiplier_bits(e));
+    if (in) {
+      *reinterpret_cast<uint2*>(p.q + row * p.cols + col) =
+            make_uint2(e4m3x4_from_f32(f[0] * by, f[1] * by, f[2] * by, f[3] * by),
+                       e4m3x4_from_f32(f[4] * by, f[5] * by, f[6] * by, f[7] * by));
+      if ((at & 15) == 0)
+        p.scale[(col / kBlock) * p.rows + row] = __uint_as_float(static_cast<uint32_t>(e) << 23);
+    }
+  }
+}
+
+template <int kPerRow, int kVecs>
+__device__ __forceinline__ void norm_backward(const BackwardParams& p) {
+  __shared__ float parts[kThreads / 32];
+  __shared__ __align__(16) float gathered[kPerRow == 32 ? kWarpCols : 4];
+  grid_dependency_wait();
+  constexpr int kRows = kThreads / kPerRow;
+  const int at = threadIdx.x % kPerRow;
+  float dgain[kVecs][8];
+#pragma unroll
+  for (int i = 0; i < kVecs; ++i)
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      dgain[i][k] = 0.f;
+  for (int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / kPerRow; row < p.rows;
+       row += static_cast<int64_t>(gridDim.x) * kRows) {
+    uint4 v[kVecs], d[kVecs];
+    const float rstd = p.rstd[row];
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) {
+      const int col = 8 * (i * kPerRow + at);
+      v[i] = col < p.cols ? load16(p.res, row * p.cols + col) : make_uint4(0, 0, 0, 0);
+      d[i] = col < p.cols ? load16(p.dn, row * p.cols + col) : make_uint4(0, 0, 0, 0);
+    }
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) {
+      const int col = 8 * (i * kPerRow + at);
+      float f[8], h[8], g[8];
+      unpack(v[i], h);
+      unpack(d[i], f);
+      if (col < p.cols) {
+        load_gain(p.gain, p.gain_bf16, col, g);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float t = f[k] * (h[k] * rstd);
+          dgain[i][k] += t;
+          sum = fmaf(t, g[k], sum);
+        }
+      }
+    }
+    const float mean = row_sum<kPerRow>(sum, parts) / static_cast<float>(p.cols);
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) {
+      const int col = 8 * (i * kPerRow + at);
+      if (col >= p.cols)
+        continue;
+      float f[8], h[8], g[8], o[8];
+      unpack(v[i], h);
+      unpack(d[i], f);
+      load_gain(p.gain, p.gain_bf16, col, g);
+      if (p.dres != nullptr)
+        unpack(load16(p.dres, row * p.cols + col), o);
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        f[k] = rstd * (f[k] * g[k] - h[k] * rstd * mean) + (p.dres != nullptr ? o[k] : 0.f);
+      store16(p.dx, row * p.cols + col, pack(f));
+    }
+  }
+  if (p.partial == nullptr)
+    return;
+  if constexpr (kPerRow == 32) {
+    // the warps' sums, one warp after the other
+    for (int w = 0; w < kRows; ++w) {
+      if (threadIdx.x / 32 == w) {
+#pragma unroll
+        for (int i = 0; i < kVecs; ++i) {
+          const int col = 8 * (i * 32 + at);
+          if (col < p.cols) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              gathered[col + k] = (w == 0 ? 0.f : gathered[col + k]) + dgain[i][k];
+          }
+        }
+      }
+      __syncthreads();
+    }
+    for (int c = threadIdx.x; c < p.cols; c += kThreads)
+      p.partial[static_cast<int64_t>(blockIdx.x) * p.cols + c] = gathered[c];
+  } else {
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) {
+      const int col = 8 * (i * kPerRow + at);
+      if (col < p.cols) {
+        float4* out = reinterpret_cast<float4*>(p.partial + static_cast<int64_t>(blockIdx.x) * p.cols + col);
+        out[0] = make_float4(dgain[i][0], dgain[i][1], dgain[i][2], dgain[i][3]);
+        out[1] = make_float4(dgain[i][4], dgain[i][5], dgain[i][6], dgain[i][7]);
+      }
+    }
+  }
+}
+
+}  // namespace
+}  // namespace mxb200
+
+// kVecs: 8-value vectors per thread
+#define MXB200_NORM_KERNELS(per_row, vecs)                                                                                            \
+  __global__ void __launch_bounds__(mxb200::kThreads) mxb200_block_norm_##per_row##x##vecs(const __grid_constant__ mxb200::ForwardParams p) { \
+    mxb200::norm_forward<per_row, vecs>(p);                                                                                           \
+  }                                                                                                                                   \
+  __global__ void __launch_bounds__(mxb200::kThreads) mxb200_block_norm_bwd_##per_row##x##vecs(const __grid_constant__ mxb200::BackwardParams p) { \
+    mxb200::norm_backward<per_row, vecs>(p);                                                                                          \
+  }
+MXB200_NORM_KERNELS(32, 2)
+MXB200_NORM_KERNELS(32, 4)
+MXB200_NORM_KERNELS(32, 6)
+MXB200_NORM_KERNELS(32, 8)
+MXB200_NORM_KERNELS(256, 2)
+MXB200_NORM_KERNELS(256, 4)
+MXB200_NORM_KERNELS(256, 8)
+
+// The rows of partial sums, in order: 32 columns and 8 interleaved shares of the rows per block.
+__global__ void __launch_bounds__(256) mxb200_block_norm_sum_gain(const float* partial, int parts, int cols, void* out, int out_bf16) {
+  __shared__ float share[8][32];
+  mxb200::grid_dependency_wait();
+  const int c = blockIdx.x * 32 + (threadIdx.x & 31), g = threadIdx.x >> 5;
+  float sum = 0.f;
+  if (c < cols)
+    for (int i = g; i < parts; i += 8)
+      sum += partial[static_cast<int64_t>(i) * cols + c];
+  share[g][threadIdx.x & 31] = sum;
+  __syncthreads();
+  if (g != 0 || c >= cols)
+    return;
+#pragma unroll
+  for (int i = 1; i < 8; ++i)
+    sum += share[i][threadIdx.x & 31];
+  if (out_bf16)
+    static_cast<__nv_bfloat16*>(out)[c] = __float2bfloat16_rn(sum);
+  else
+    static_cast<float*>(out)[c] = sum;
+}
+
+namespace mxb200 {
+namespace {
+
+constexpr int64_t kMost = int64_t{1} << 30;
+
+struct Variant {
+  void (*forward)(ForwardParams);
+  void (*backward)(BackwardParams);
+  int rows_per_block;
+};
+
+// One warp per row as long as its registers hold it (64 values per lane), then the whole block.
+Variant variant(int cols) {
+  const int vecs = cols / 8;
+  if (cols <= kWarpCols) {
+    if (vecs <= 64)
+      return {mxb200_block_norm_32x2, mxb200_block_norm_bwd_32x2, kThreads / 32};
+    if (vecs <= 128)
+      return {mxb200_block_norm_32x4, mxb200_block_norm_bwd_32x4, kThreads / 32};
+    if (vecs <= 192)
+      return {mxb200_block_norm_32x6, mxb200_block_norm_bwd_32x6, kThreads / 32};
+    return {mxb200_block_norm_32x8, mxb200_block_norm_bwd_32x8, kThreads / 32};
+  }
+  if (vecs <= 512)
+    return {mxb200_block_norm_256x2, mxb200_block_norm_bwd_256x2, 1};
+  if (vecs <= 1024)
+    return {mxb200_block_norm_256x4, mxb200_block_norm_bwd_256x4, 1};
+  return {mxb200_block_norm_256x8, mxb200_block_norm_bwd_256x8, 1};
+}
+
+int check_shape(int64_t rows, int32_t cols) {
+  return rows < 0 || rows > kMost || cols <= 0 || cols > kMaxCols || cols % 16 ? MXB200_ERR_SHAPE : MXB200_OK;
+}
+
+// needed pointers first, then optional ones
+int check_pointers(std::initializer_list<const void*> needed, std::initializer_list<const void*> optional) {
+  for (const void* q : needed)
+    if (q == nullptr)
+      return MXB200_ERR_NULL;
+  for (const auto* list : {&needed, &optional})
+    for (const void* q : *list)
+      if (!aligned16(q))
+        return MXB200_ERR_ALIGNMENT;
+  return MXB200_OK;
+}
+
+// CTAs of the backward: two for each SM, fewer where there are not the rows
+int64_t backward_blocks(int64_t rows, int rows_per_block, int sms) {
+  return std::max<int64_t>(1, std::min<int64_t>((rows + rows_per_block - 1) / rows_per_block, 2 * sms));
+}
+
+}  // namespace
+}  // namespace mxb200
+
+extern "C" int mxb200_block_norm_fwd(const mxb200_block_norm_args* a, void* stream) {
+  using namespace mxb200;
+  if (a == nullptr)
+    return MXB200_ERR_NULL;
+  if (int st = check_shape(a->rows, a->cols); st != MXB200_OK)
+    return st;
+  if (a->rows == 0)
+    return MXB200_OK;
+  DeviceInfo dev;
+  if (int st = current_device(&dev); st != MXB200_OK)
+    return st;
+  if (int st = check_pointers({a->x, a->rstd, a->q, a->scale}, {a->r, a->gain, a->res, a->n}); st != MXB200_OK)
+    return st;
+  if ((a->r == nullptr) != (a->res == nullptr))
+    return MXB200_ERR_ARGUMENT;
+  const Variant v = variant(a->cols);
+  const ForwardParams p{a->x, a->r, a->gain, a->res, a->n, static_cast<uint8_t*>(a->q), a->scale, a->rstd,
+                        a->rows, a->cols, a->gain_bf16, a->eps};
+  return launch_kernel(v.forward, static_cast<unsigned>((a->rows + v.rows_per_block - 1) / v.rows_per_block), kThreads, 0,
+                       static_cast<cudaStream_t>(stream), p);
+}
+
+extern "C" size_t mxb200_block_norm_workspace_bytes(int64_t rows, int32_t cols) {
+  using namespace mxb200;
+  DeviceInfo dev;
+  if (check_shape(rows, cols) != MXB200_OK || current_device(&dev) != MXB200_OK)
+    return 0;
+  return static_cast<size_t>(backward_blocks(rows, variant(cols).rows_per_block, dev.sms)) * cols * sizeof(float);
+}
+
+extern "C" int mxb200_block_norm_bwd(const mxb200_block_norm_bwd_args* a, void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace mxb200;
+  if (a == nullptr)
+    return MXB200_ERR_NULL;
+  if (int st = check_shape(a->rows, a->cols); st != MXB200_OK)
+    return st;
+  DeviceInfo dev;
+  if (int st = current_device(&dev); st != MXB200_OK)
+    return st;
+  const auto s = static_cast<cudaStream_t>(stream);
+  if (a->rows == 0) {
+    if (a->dgain != nullptr && cudaMemsetAsync(a->dgain, 0, a->cols * (a->gain_bf16 ? size_t{2} : size_t{4}), s) != cudaSuccess)
+      return MXB200_ERR_LAUNCH;
+    return MXB200_OK;
+  }
+  if (int st = check_pointers({a->dn, a->res, a->rstd, a->dx}, {a->dres, a->gain, a->dgain, workspace}); st != MXB200_OK)
+    return st;
+  if (a->dgain != nullptr && a->gain == nullptr)
+    return MXB200_ERR_ARGUMENT;
+  if (a->dgain != nullptr && (workspace == nullptr || workspace_bytes < mxb200_block_norm_workspace_bytes(a->rows, a->cols)))
+    return MXB200_ERR_WORKSPACE;
+  const Variant v = variant(a->cols);
+  const int blocks = static_cast<int>(backward_blocks(a->rows, v.rows_per_block, dev.sms));
+  float* partial = a->dgain != nullptr ? static_cast<float*>(workspace) : nullptr;
+  const BackwardParams p{a->dn, a->dres, a->res, a->rstd, a->gain, a->dx, partial, a->rows, a->cols, a->gain_bf16};
+  if (int st = launch_kernel(v.backward, static_cast<unsigned>(blocks), kThreads, 0, s, p); st != MXB200_OK || partial == nullptr)
+    return st;
+  return launch_kernel(mxb200_block_norm_sum_gain, static_cast<unsigned>((a->cols + 31) / 32), 256, 0, s,
+                       static_cast<const float*>(partial), blocks, static_cast<int>(a->cols), a->dgain, static_cast<int>(a->gain_bf16));
+}

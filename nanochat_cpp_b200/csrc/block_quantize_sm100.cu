@@ -1,0 +1,331 @@
+// Quantizers of the 128-value block format: E4M3 with one fp32 power-of-two scale per block.
+//
+//   rows     128 values of a row (activations and gradients on their way into the forward and the input gradient)
+//   tokens   128 rows of a column, blocks starting over at every expert's first row (both operands of a weight gradient)
+//   weight   128 x 128 values
+//
+// Scale = the smallest power of two s >= 2^-126 with max|block| <= 448 s, so x / s is exact and E4M3 rounds once. NaN does not
+// count in the maximum and stays NaN; Inf saturates to 448 s.
+//
+// All three work on 128 x 128 tiles, 256 threads: 16 lanes hold a row's 128 values, 8 each, and a thread 8 rows 16 apart, all
+// loaded before the first is used. A row's maximum is a shuffle over 16 lanes, a column's goes through shared memory. Bound by
+// memory: 2 bytes read and 1 written per value and layout; both layouts of an activation come from one read. Data never leaves
+// transposed, since the matrix product reads either orientation.
+#include <algorithm>
+#include <cstdint>
+
+#include <cuda_bf16.h>
+
+#include "bf16x2_sm100.cuh"
+#include "block_common.cuh"
+#include "internal.h"
+#include "ptx_sm100.cuh"
+
+namespace mxb200 {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kRowsPerThread = 8;
+
+struct QuantizeParams {
+  const void* x;
+  int64_t ld;           // values between rows
+  int64_t x_expert;     // weight: values between experts
+  int64_t rows, cols;
+  const int32_t* ends;  // tokens: rows by expert
+  int experts;
+  uint8_t* row_data;    // rows: (rows, cols); null where they are not wanted
+  float* row_scale;     // (cols / 128, rows)
+  uint8_t* col_data;    // tokens: (token blocks * 128, cols); weight: (experts, rows, cols)
+  float* col_scale;     // tokens: (token blocks, cols); weight: (experts, rows / 128, cols / 128)
+};
+
+struct Values {
+  float v[8];
+};
+
+template <bool kBf16>
+__device__ __forceinline__ Values load_values(const void* x, int64_t at) {
+  Values r;
+  if constexpr (kBf16) {
+    const uint4 w = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(x) + at);
+    r.v[0] = lo_f32(w.x), r.v[1] = hi_f32(w.x), r.v[2] = lo_f32(w.y), r.v[3] = hi_f32(w.y);
+    r.v[4] = lo_f32(w.z), r.v[5] = hi_f32(w.z), r.v[6] = lo_f32(w.w), r.v[7] = hi_f32(w.w);
+  } else {
+    const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(x) + at);
+    const float4 a = q[0], b = q[1];
+    r.v[0] = a.x, r.v[1] = a.y, r.v[2] = a.z, r.v[3] = a.w, r.v[4] = b.x, r.v[5] = b.y, r.v[6] = b.z, r.v[7] = b.w;
+  }
+  return r;
+}
+
+__device__ __forceinline__ float scale_of(int exponent) {
+  return __uint_as_float(static_cast<uint32_t>(exponent) << 23);
+}
+
+__device__ __forceinline__ float multiplier_of(int exponent) {
+  return __uint_as_float(mx_multiplier_bits(exponent));
+}
+
+__device__ __forceinline__ int exponent_of(float amax) {
+  return block_exponent(__float_as_uint(amax));
+}
+
+// 8 rows 16 apart of the tile from `row` on (rows_left of them exist), 8 columns at `at`.
+template <bool kBf16>
+__device__ __forceinline__ void load_tile(const void* x, int64_t at, int64_t ld, int row, int rows_left, bool col_ok, Values (&v)[kRowsPerThread]) {
+#pragma unroll
+  for (int i = 0; i < kRowsPerThread; ++i) {
+    if (col_ok && row + 16 * i < rows_left)
+      v[i] = load_values<kBf16>(x, at + 16 * i * ld);
+    else
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        v[i].v[k] = 0.f;
+  }
+}
+
+// One block of rows at a time, all its column tiles with a stride of gridDim.y.
+template <bool kBf16, bool kRows, bool kTokens>
+__device__ __forceinline__ void quantize_activation(const QuantizeParams& p, int* first_row, int* first_tile, int* tmp, float (*partial)[kBlock]) {
+  grid_dependency_wait();
+  const int lane16 = threadIdx.x & 15, row = threadIdx.x >> 4;
+  int64_t row0 = static_cast<int64_t>(blockIdx.x) * kBlock;
+  int rows_left;
+  if constexpr (kTokens) {
+    scan_experts(p.ends, p.experts, static_cast<int>(p.rows), kBlock, first_row, first_tile, tmp);
+    const int blocks = first_tile[p.experts];
+    if (static_cast<int>(blockIdx.x) >= blocks)
+      return;
+    const int e = expert_of_tile(first_tile, p.experts, blockIdx.x);
+    const int r = first_row[e] + (static_cast<int>(blockIdx.x) - first_tile[e]) * kBlock;
+    row0 = r;
+    rows_left = min(kBlock, first_row[e + 1] - r);
+  } else {
+    rows_left = static_cast<int>(min(static_cast<int64_t>(kBlock), p.rows - row0));
+  }
+  const int tiles = static_cast<int>((p.cols + kBlock - 1) / kBlock);
+  for (int t = blockIdx.y; t < tiles; t += gridDim.y) {
+    const int64_t col = static_cast<int64_t>(t) * kBlock + 8 * lane16;
+    const bool col_ok = col < p.cols;
+    Values v[kRowsPerThread];
+    load_tile<kBf16>(p.x, (row0 + row) * p.ld + col, p.ld, row, rows_left, col_ok, v);
+    if constexpr (kRows) {
+#pragma unroll
+      for (int i = 0; i < kRowsPerThread; ++i) {
+        float m = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          m = fmaxf(m, fabsf(v[i].v[k]));
+#pragma unroll
+        for (int d = 8; d > 0; d >>= 1)
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+        const int e = exponent_of(m);
+        const float f = multiplier_of(e);
+        const int64_t r = row0 + row + 16 * i;
+        if (row + 16 * i < rows_left) {
+          if (col_ok)
+            *reinterpret_cast<uint2*>(p.row_data + r * p.cols + col) =
+                  make_uint2(e4m3x4_from_f32(v[i].v[0] * f, v[i].v[1] * f, v[i].v[2] * f, v[i].v[3] * f),
+                             e4m3x4_from_f32(v[i].v[4] * f, v[i].v[5] * f, v[i].v[6] * f, v[i].v[7] * f));
+          if (lane16 == 0)
+            p.row_scale[static_cast<int64_t>(t) * p.rows + r] = scale_of(e);
+        }
+      }
+    }
+    if constexpr (kTokens) {
+      float m[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        m[k] = 0.f;
+#pragma unroll
+        for (int i = 0; i < kRowsPerThread; ++i)
+          m[k] = fmaxf(m[k], fabsf(v[i].v[k]));
+        m[k] = fmaxf(m[k], __shfl_xor_sync(0xffffffffu, m[k], 16));
+      }
+      __syncthreads();  // the previous tile's maxima have been read
+      if ((threadIdx.x & 16) == 0) {
+        float4* dst = reinterpret_cast<float4*>(&partial[threadIdx.x >> 5][8 * lane16]);
+        dst[0] = make_float4(m[0], m[1], m[2], m[3]);
+        dst[1] = make_float4(m[4], m[5], m[6], m[7]);
+      }
+      __syncthreads();
+      float f[8];
+      int e[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        m[k] = 0.f;
+#pragma unroll
+      for (int w = 0; w < kThreads / 32; ++w) {
+        const float4* src = reinterpret_cast<const float4*>(&partial[w][8 * lane16]);
+        const float4 a = src[0], b = src[1];
+        m[0] = fmaxf(m[0], a.x), m[1] = fmaxf(m[1], a.y), m[2] = fmaxf(m[2], a.z), m[3] = fmaxf(m[3], a.w);
+        m[4] = fmaxf(m[4], b.x), m[5] = fmaxf(m[5], b.y), m[6] = fmaxf(m[6], b.z), m[7] = fmaxf(m[7], b.w);
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        e[k] = exponent_of(m[k]);
+        f[k] = multiplier_of(e[k]);
+      }
+      if (col_ok) {
+        const int64_t out0 = static_cast<int64_t>(blockIdx.x) * kBlock + row;
+#pragma unroll
+        for (int i = 0; i < kRowsPerThread; ++i)  // rows that do not exist are zeros: they count in the product
+          *reinterpret_cast<uint2*>(p.col_data + (out0 + 16 * i) * p.cols + col) =
+                make_uint2(e4m3x4_from_f32(v[i].v[0] * f[0], v[i].v[1] * f[1], v[i].v[2] * f[2], v[i].v[3] * f[3]),
+                           e4m3x4_from_f32(v[i].v[4] * f[4], v[i].v[5] * f[5], v[i].v[6] * f[6], v[i].v[7] * f[7]));
+        if (row == 0) {
+          float4* dst = reinterpret_cast<float4*>(p.col_scale + static_cast<int64_t>(blockIdx.x) * p.cols + col);
+          dst[0] = make_float4(scale_of(e[0]), scale_of(e[1]), scale_of(e[2]), scale_of(e[3]));
+          dst[1] = make_float4(scale_of(e[4]), scale_of(e[5]), scale_of(e[6]), scale_of(e[7]));
+        }
+      }
+    }
+  }
+}
+
+template <bool kBf16>
+__device__ __forceinline__ void quantize_weight(const QuantizeParams& p, float* partial) {
+  grid_dependency_wait();
+  const int lane16 = threadIdx.x & 15, row = threadIdx.x >> 4;
+  const int64_t tiles_n = (p.cols + kBlock - 1) / kBlock, tiles_m = (p.rows + kBlock - 1) / kBlock;
+  const int64_t tile = blockIdx.x;
+  const int64_t e = tile / (tiles_m * tiles_n), tm = tile / tiles_n % tiles_m, tn = tile % tiles_n;
+  const int64_t row0 = tm * kBlock, col = tn * kBlock + 8 * lane16;
+  const int rows_left = static_cast<int>(min(static_cast<int64_t>(kBlock), p.rows - row0));
+  const bool col_ok = col < p.cols;
+  Values v[kRowsPerThread];
+  load_tile<kBf16>(p.x, e * p.x_expert + (row0 + row) * p.ld + col, p.ld, row, rows_left, col_ok, v);
+  float m = 0.f;
+#pragma unroll
+  for (int i = 0; i < kRowsPerThread; ++i)
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      m = fmaxf(m, fabsf(v[i].v[k]));
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1)
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+  if ((threadIdx.x & 31) == 0)
+    partial[threadIdx.x >> 5] = m;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w)
+    m = fmaxf(m, partial[w]);
+  const int ex = exponent_of(m);
+  const float f = multiplier_of(ex);
+#pragma unroll
+  for (int i = 0; i < kRowsPerThread; ++i)
+    if (col_ok && row + 16 * i < rows_left)
+      *reinterpret_cast<uint2*>(p.col_data + (e * p.rows + row0 + row + 16 * i) * p.cols + col) =
+            make_uint2(e4m3x4_from_f32(v[i].v[0] * f, v[i].v[1] * f, v[i].v[2] * f, v[i].v[3] * f),
+                       e4m3x4_from_f32(v[i].v[4] * f, v[i].v[5] * f, v[i].v[6] * f, v[i].v[7] * f));
+  if (threadIdx.x == 0)
+    p.col_scale[tile] = scale_of(ex);
+}
+
+}  // namespace
+}  // namespace mxb200
+
+__global__ void __launch_bounds__(mxb200::kThreads) mxb200_block_quantize_rows(const __grid_constant__ mxb200::QuantizeParams p) {
+  mxb200::quantize_activation<true, true, false>(p, nullptr, nullptr, nullptr, nullptr);
+}
+
+template <bool kRows>
+__device__ __forceinline__ void quantize_tokens(const mxb200::QuantizeParams& p) {
+  __shared__ int first_row[mxb200::kMaxExperts + 1], first_tile[mxb200::kMaxExperts + 1];
+  __shared__ __align__(16) union {
+    int tmp[mxb200::kMaxExperts];
+    float partial[mxb200::kThreads / 32][mxb200::kBlock];
+  } u;
+  mxb200::quantize_activation<true, kRows, true>(p, first_row, first_tile, u.tmp, u.partial);
+}
+
+__global__ void __launch_bounds__(mxb200::kThreads) mxb200_block_quantize_tokens(const __grid_constant__ mxb200::QuantizeParams p) {
+  quantize_tokens<false>(p);
+}
+
+__global__ void __launch_bounds__(mxb200::kThreads) mxb200_block_quantize_both(const __grid_constant__ mxb200::QuantizeParams p) {
+  quantize_tokens<true>(p);
+}
+
+__global__ void __launch_bounds__(mxb200::kThreads) mxb200_block_quantize_weight_bf16(const __grid_constant__ mxb200::QuantizeParams p) {
+  __shared__ float partial[mxb200::kThreads / 32];
+  mxb200::quantize_weight<true>(p, partial);
+}
+
+__global__ void __launch_bounds__(mxb200::kThreads) mxb200_block_quantize_weight_f32(const __grid_constant__ mxb200::QuantizeParams p) {
+  __shared__ float partial[mxb200::kThreads / 32];
+  mxb200::quantize_weight<false>(p, partial);
+}
+
+namespace mxb200 {
+namespace {
+
+constexpr int64_t kMost = int64_t{1} << 30;
+
+int64_t up(int64_t n, int64_t d) {
+  return (n + d - 1) / d;
+}
+
+// Null or misaligned pointers among those that are needed.
+int check_pointers(std::initializer_list<const void*> pointers) {
+  for (const void* q : pointers) {
+    if (q == nullptr)
+      return MXB200_ERR_NULL;
+    if (!aligned16(q))
+      return MXB200_ERR_ALIGNMENT;
+  }
+  return MXB200_OK;
+}
+
+}  // namespace
+}  // namespace mxb200
+
+extern "C" int mxb200_block_quantize(const void* x, int64_t rows, int64_t cols, int64_t ld, const int32_t* ends, int experts,
+                                     void* row_data, float* row_scale, void* token_data, float* token_scale, void* stream) {
+  using namespace mxb200;
+  if (rows < 0 || rows > kMost || cols <= 0 || cols > kMost || cols % 16 || ld < cols || ld % 8 || experts < 1 || experts > kMaxExperts)
+    return MXB200_ERR_SHAPE;
+  if (ends == nullptr && experts != 1)
+    return MXB200_ERR_NULL;
+  if (rows == 0)
+    return MXB200_OK;
+  const bool want_rows = row_data != nullptr, want_tokens = token_data != nullptr;
+  if (!want_rows && !want_tokens)
+    return MXB200_ERR_NULL;
+  DeviceInfo dev;
+  if (int st = current_device(&dev); st != MXB200_OK)
+    return st;
+  if (int st = check_pointers({x}); st != MXB200_OK)
+    return st;
+  if (int st = want_rows ? check_pointers({row_data, row_scale}) : MXB200_OK; st != MXB200_OK)
+    return st;
+  if (int st = want_tokens ? check_pointers({token_data, token_scale}) : MXB200_OK; st != MXB200_OK)
+    return st;
+  QuantizeParams p{x, ld, 0, rows, cols, ends, experts, static_cast<uint8_t*>(row_data), row_scale,
+                   static_cast<uint8_t*>(token_data), token_scale};
+  // enough blocks to fill the machine; beyond that a block goes on to its rows' next columns, with its experts looked up once
+  const int64_t blocks = want_tokens ? mxb200_block_token_blocks(rows, experts) : up(rows, kBlock);
+  const int64_t parts = std::min<int64_t>(up(cols, kBlock), std::max<int64_t>(1, up(8 * dev.sms, blocks)));
+  const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(std::min<int64_t>(parts, 65535)));
+  const auto kernel = !want_tokens ? mxb200_block_quantize_rows : want_rows ? mxb200_block_quantize_both : mxb200_block_quantize_tokens;
+  return launch_kernel(kernel, grid, kThreads, 0, static_cast<cudaStream_t>(stream), p);
+}
+
+extern "C" int mxb200_block_quantize_weight(const void* w, int w_bf16, int experts, int64_t rows, int64_t cols, void* data,
+                                            float* scale, void* stream) {
+  using namespace mxb200;
+  if (rows <= 0 || rows > kMost || cols <= 0 || cols > kMost || rows % 16 || cols % 16 || experts < 1 || experts > kMaxExperts)
+    return MXB200_ERR_SHAPE;
+  const int64_t tiles = experts * up(rows, kBlock) * up(cols, kBlock);
+  if (tiles > kMost)
+    return MXB200_ERR_SHAPE;
+  DeviceInfo dev;
+  if (int st = current_device(&dev); st != MXB200_OK)
+    return st;
+  if (int st = check_pointers({w, data, scale}); st != MXB200_OK)
+    return st;
+  QuantizeParams p{w, cols, rows * cols, rows, cols, nullptr, experts, nullptr, nullptr, static_cast<uint8_t*>(data), scale};
+  return launch_kernel(w_bf16 ? mxb200_block_quantize_weight_bf16 : mxb200_block_quantize_weight_f32, static_cast<unsigned>(tiles),
+                       kThreads, 0, static_cast<cudaStream_t>(stream), p);
+}

@@ -1988,6 +1988,8 @@ extern "C" int mxb200_device_status(uint32_t* word) {
     w = norm;
   if (const uint32_t quant = mxb200::take_quantize_watchdog_word(); w == 0)
     w = quant;
+  if (const uint32_t block = mxb200::take_block_gemm_watchdog_word(); w == 0)
+    w = block;
   if (word != nullptr)
     *word = w;
   return w == 0 ? MXB200_OK : MXB200_ERR_WATCHDOG;

@@ -33,6 +33,8 @@ EncodeTiledFn encode_fn();
 uint32_t take_norm_watchdog_word();
 // The same for the streaming quantizer.
 uint32_t take_quantize_watchdog_word();
+// The same for the product of 128-value blocks.
+uint32_t take_block_gemm_watchdog_word();
 
 inline bool aligned16(const void* p) {
   return (reinterpret_cast<uintptr_t>(p) & 15u) == 0;
@@ -46,13 +48,13 @@ inline int launch_status() {
 // placed while the stream's previous kernel still runs, as that one's leave their SMs, and wait there for its end with
 // their set-up done. That takes 1 to 2 us of launch latency and ramp-up out of every step of a chain of small kernels.
 template <typename... Params>
-int launch_kernel(void (*kernel)(Params...), unsigned grid, unsigned block, size_t smem, cudaStream_t stream,
+int launch_kernel(void (*kernel)(Params...), dim3 grid, unsigned block, size_t smem, cudaStream_t stream,
                   const Params&... params) {
   cudaLaunchAttribute attribute{};
   attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attribute.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t config{};
-  config.gridDim = dim3(grid);
+  config.gridDim = grid;
   config.blockDim = dim3(block);
   config.dynamicSmemBytes = smem;
   config.stream = stream;

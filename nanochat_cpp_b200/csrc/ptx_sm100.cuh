@@ -112,6 +112,16 @@ __device__ __forceinline__ void tma_load_2d(uint32_t pred, void* smem_dst, const
         : "memory");
 }
 
+// The 3-D form: coordinates {x, y, z}.
+__device__ __forceinline__ void tma_load_3d(uint32_t pred, uint32_t smem_dst, const CUtensorMap* map, uint32_t bar_addr,
+                                            int32_t x, int32_t y, int32_t z) {
+  asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+        "@q cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];\n\t}\n"
+        ::"r"(smem_dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar_addr), "r"(x), "r"(y), "r"(z), "r"(pred)
+        : "memory");
+}
+
 // The same load with an L2 eviction-priority hint (a createpolicy value), for data that is read once.
 __device__ __forceinline__ void tma_load_2d_hint(uint32_t pred, void* smem_dst, const CUtensorMap* map, uint64_t* bar,
                                                  int32_t x, int32_t y, uint64_t policy) {
@@ -121,6 +131,16 @@ __device__ __forceinline__ void tma_load_2d_hint(uint32_t pred, void* smem_dst, 
         ::"r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(pred),
           "l"(policy)
         : "memory");
+}
+
+// 4 bytes global -> shared without passing through registers (both addresses 4-byte aligned), and the arrival that such
+// copies of this thread make on an mbarrier once they have all landed (counted among the barrier's expected arrivals).
+__device__ __forceinline__ void cp_async_4(uint32_t smem_dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_dst), "l"(src) : "memory");
+}
+
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar_addr) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar_addr) : "memory");
 }
 
 // Untiled bulk copy global -> shared: both addresses 16-byte aligned, bytes % 16 == 0.
@@ -234,6 +254,30 @@ __device__ __forceinline__ void tcgen05_mma_mxf8(uint32_t pred, uint32_t d_tmem,
         : "memory");
 }
 
+// D[tmem] (+)= A[smem] . B[smem]^T, E4M3 x E4M3 with fp32 accumulation and no scales; one K = 32 step.
+__device__ __forceinline__ void tcgen05_mma_f8(uint32_t pred, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                               uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "setp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n"
+        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(pred)
+        : "memory");
+}
+
+// 16 TMEM lanes (taddr's lane on) x 32 columns as matrix fragments: for 8-column group j, r[4j], r[4j+1] are row lane / 4,
+// columns 8j + 2 (lane % 4) and the next; r[4j+2], r[4j+3] the same columns of row lane / 4 + 8.
+__device__ __forceinline__ void tmem_ld_16x256b_x4(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
+
 // This thread's TMEM lane (its warp's quarter), 32 consecutive 32-bit columns.
 __device__ __forceinline__ void tmem_ld_32x32b_x32(uint32_t taddr, uint32_t (&r)[32]) {
   asm volatile(
@@ -280,6 +324,12 @@ __device__ __forceinline__ uint64_t make_smem_desc(uint32_t smem_addr, uint32_t 
 // uses goes into bits 4-5 (B) and 29-30 (A).
 __host__ __device__ constexpr uint32_t make_idesc_mxf8(uint32_t m, uint32_t n) {
   return (1u << 23) | ((n >> 3) << 17) | ((m >> 4) << 24);
+}
+
+// Instruction descriptor of kind::f8f6f4, E4M3 x E4M3 (format 0) into fp32 (bit 4); a_mn / b_mn: that operand lies with its
+// rows (M or N) contiguous instead of K (bits 15, 16).
+__host__ __device__ constexpr uint32_t make_idesc_f8(uint32_t m, uint32_t n, bool a_mn, bool b_mn) {
+  return (1u << 4) | (static_cast<uint32_t>(a_mn) << 15) | (static_cast<uint32_t>(b_mn) << 16) | ((n >> 3) << 17) | ((m >> 4) << 24);
 }
 
 __device__ __forceinline__ uint32_t idesc_with_sf(uint32_t idesc, uint32_t a_sf_id, uint32_t b_sf_id) {
@@ -333,6 +383,15 @@ __device__ __forceinline__ void tma_load_2d_pair(uint32_t pred, uint32_t smem_ds
         "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %5, 0;\n\t"
         "@q cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];\n\t}\n"
         ::"r"(smem_dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar_cluster_addr), "r"(x), "r"(y), "r"(pred)
+        : "memory");
+}
+
+__device__ __forceinline__ void tma_load_3d_pair(uint32_t pred, uint32_t smem_dst, const CUtensorMap* map,
+                                                 uint32_t bar_cluster_addr, int32_t x, int32_t y, int32_t z) {
+  asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+        "@q cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];\n\t}\n"
+        ::"r"(smem_dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar_cluster_addr), "r"(x), "r"(y), "r"(z), "r"(pred)
         : "memory");
 }
 
@@ -392,6 +451,32 @@ __device__ __forceinline__ void tcgen05_mma_mxf8_pair(uint32_t pred, uint32_t d_
         "@q tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale [%0], %1, %2, %3, [%5], [%6], p;\n\t}\n"
         ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(sfa_tmem), "r"(sfb_tmem), "r"(pred)
         : "memory");
+}
+
+// The unscaled form across a pair.
+__device__ __forceinline__ void tcgen05_mma_f8_pair(uint32_t pred, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                                    uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "setp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n"
+        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(pred)
+        : "memory");
+}
+
+// ---------------------------------------------------------------------------------------------- fragments
+
+// Four 8 x 8 matrices of 16-bit values, one fragment register each, into shared memory: lane l gives the address of row
+// l % 8 of matrix l / 8 (16 bytes, 16-byte aligned). The transposed form stores the matrices' columns as those rows.
+__device__ __forceinline__ void stmatrix_x4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d)
+               : "memory");
+}
+
+__device__ __forceinline__ void stmatrix_x4_trans(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d)
+               : "memory");
 }
 
 }  // namespace mxb200

@@ -16,6 +16,7 @@
 #include <ATen/FuncTorchTLS.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <c10/util/SmallVector.h>
 #include <torch/csrc/Exceptions.h>
@@ -972,6 +973,363 @@ Tensor softcap_cross_entropy(const Tensor& x_in, const Tensor& weight, const Ten
   return none ? losses : reduced_loss(losses, mean ? count_valid(targets) : Tensor(), mean);
 }
 
+// ---------------------------------------------------------------------------------------------------- blocks of 128
+
+// Linears over E4M3 operands with one fp32 scale for 128 values (include/mxb200.h), dense and by expert, and the residual norm
+// in front of them. Everything runs on the input's device, whatever the current one is.
+
+std::optional<Tensor> some(const Tensor& t) {
+  return t.defined() ? std::optional<Tensor>(t) : std::nullopt;
+}
+
+// Contiguous with a 16-byte aligned start.
+Tensor dense(const Tensor& t) {
+  const Tensor c = t.contiguous();
+  return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 == 0 ? c : c.clone();
+}
+
+constexpr int64_t blocks_of(int64_t n) {
+  return (n + 127) / 128;
+}
+
+bool block_features(int64_t n) {
+  return n > 0 && n % 16 == 0;
+}
+
+// E4M3 values and their fp32 scales; `like` in Python's BlockTensor.
+struct Block {
+  Tensor data, scale;
+};
+
+using GivenBlock = std::optional<std::pair<Tensor, Tensor>>;
+
+// Tokens' operands: (rows, cols) values in blocks along rows, and in blocks along each expert's tokens.
+struct Experts {
+  const int32_t* ends = nullptr;
+  int count = 1;
+};
+
+Block empty_row_blocks(int64_t rows, int64_t cols, at::Device device) {
+  return {empty({rows, cols}, kE4M3, device), empty({blocks_of(cols), rows}, at::kFloat, device)};
+}
+
+Block empty_token_blocks(int64_t rows, int64_t cols, const Experts& e, at::Device device) {
+  const int64_t blocks = mxb200_block_token_blocks(rows, e.count);
+  return {empty({128 * blocks, cols}, kE4M3, device), empty({blocks, cols}, at::kFloat, device)};
+}
+
+// x (rows, cols) bf16 with contiguous columns into either layout or both.
+void quantize_blocks(const Tensor& x, const Experts& e, const Block* rows, const Block* tokens) {
+  const int64_t ld = x.size(0) > 1 ? x.stride(0) : x.size(1);
+  check(mxb200_block_quantize(x.data_ptr(), x.size(0), x.size(1), ld, e.ends, e.count,
+                              rows != nullptr ? rows->data.data_ptr() : nullptr,
+                              rows != nullptr ? static_cast<float*>(rows->scale.data_ptr()) : nullptr,
+                              tokens != nullptr ? tokens->data.data_ptr() : nullptr,
+                              tokens != nullptr ? static_cast<float*>(tokens->scale.data_ptr()) : nullptr, stream()),
+        "quantize_block");
+}
+
+// What the quantizer reads in place: aligned rows, contiguous columns.
+Tensor readable_rows(const Tensor& x) {
+  const bool ok = x.stride(1) == 1 && (x.size(0) <= 1 || (x.stride(0) >= x.size(1) && x.stride(0) % 8 == 0)) &&
+                  reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0;
+  return ok ? x : dense(x);
+}
+
+void block_product(int kind, const Block& a, const Block& b, const Tensor& d, const Experts& e, int64_t tokens, int64_t in, int64_t out) {
+  const mxb200_block_gemm_args g{a.data.data_ptr(), static_cast<const float*>(a.scale.data_ptr()), b.data.data_ptr(),
+                                 static_cast<const float*>(b.scale.data_ptr()), d.data_ptr(), e.ends, tokens, in, out, e.count, kind,
+                                 d.scalar_type() == at::kFloat ? MXB200_OUT_F32 : MXB200_OUT_BF16};
+  check(mxb200_block_gemm(&g, stream()), "block_gemm");
+}
+
+Block quantize_weight_blocks(const Tensor& w_in) {
+  const Tensor w = dense(w_in.detach());
+  const int64_t e = w.dim() == 3 ? w.size(0) : 1, n = w.size(-2), k = w.size(-1);
+  std::vector<int64_t> scales{blocks_of(n), blocks_of(k)};
+  if (w.dim() == 3)
+    scales.insert(scales.begin(), e);
+  const Block q{empty(w.sizes(), kE4M3, w.device()), empty(scales, at::kFloat, w.device())};
+  check(mxb200_block_quantize_weight(w.data_ptr(), w.scalar_type() == at::kBFloat16, static_cast<int>(e), n, k, q.data.data_ptr(),
+                                     static_cast<float*>(q.scale.data_ptr()), stream()),
+        "quantize_block_weight");
+  return q;
+}
+
+// A Linear's operands, checked.
+struct BlockLinearCall {
+  Tensor x;        // undefined where only its blocks are given
+  Tensor w;        // undefined where only its blocks are given
+  Block x_rows;    // undefined: to be made
+  Block w_blocks;  // undefined: to be made
+  Tensor ends;     // undefined: dense
+  int64_t tokens = 0, in = 0, out = 0;
+  at::Device device = at::kCPU;
+
+  Experts experts() const {
+    return ends.defined() ? Experts{static_cast<const int32_t*>(ends.data_ptr()), static_cast<int>(ends.numel())} : Experts{};
+  }
+};
+
+[[noreturn]] void fail_in(const char* what, const char* message) {
+  throw std::runtime_error(std::string(what) + ": " + message);
+}
+
+void require_in(bool ok, const char* what, const char* message) {
+  if (!ok)
+    fail_in(what, message);
+}
+
+Block given_block(const std::pair<Tensor, Tensor>& q, at::IntArrayRef data, at::IntArrayRef scale, at::Device device, const char* what) {
+  for (const Tensor* t : {&q.first, &q.second})
+    require_in(t->device() == device, what, "expected quantized operands on the input's device");
+  require_in(q.first.scalar_type() == kE4M3 && q.second.scalar_type() == at::kFloat, what, "expected e4m3 data with fp32 scales");
+  require_in(q.first.sizes() == data && q.second.sizes() == scale, what, "shape mismatch");
+  return {dense(q.first), q.second.contiguous()};
+}
+
+struct BlockLinear : torch::autograd::Function<BlockLinear> {
+  // With `ctx`, what the backward needs is kept: the weight's blocks for the input's gradient; for the weight's, the input in
+  // blocks along tokens where this pass reads it anyway, else the input.
+  static Tensor run(AutogradContext* ctx, BlockLinearCall& c) {
+    const bool grad_w = ctx != nullptr && c.w.defined() && c.w.requires_grad();
+    const bool grad_x = ctx != nullptr && c.x.defined() && c.x.requires_grad();
+    const Experts e = c.experts();
+    Block tokens;
+    if (!c.x_rows.data.defined()) {
+      c.x_rows = empty_row_blocks(c.tokens, c.in, c.device);
+      if (grad_w)
+        tokens = empty_token_blocks(c.tokens, c.in, e, c.device);
+      quantize_blocks(readable_rows(c.x), grad_w ? e : Experts{}, &c.x_rows, grad_w ? &tokens : nullptr);
+    }
+    if (!c.w_blocks.data.defined())
+      c.w_blocks = quantize_weight_blocks(c.w);
+    const Tensor y = empty({c.tokens, c.out}, at::kBFloat16, c.device);
+    block_product(MXB200_BLOCK_FORWARD, c.w_blocks, c.x_rows, y, e, c.tokens, c.in, c.out);
+    if (ctx != nullptr) {
+      const Tensor none;
+      ctx->save_for_backward({grad_x ? c.w_blocks.data : none, grad_x ? c.w_blocks.scale : none, tokens.data, tokens.scale,
+                              grad_w && !tokens.data.defined() ? c.x : none, c.ends});
+      ctx->saved_data["tokens"] = c.tokens;
+      ctx->saved_data["in"] = c.in;
+      ctx->saved_data["out"] = c.out;
+      if (c.w.defined()) {
+        ctx->saved_data["w_sizes"] = c.w.sizes().vec();
+        ctx->saved_data["w_dtype"] = c.w.scalar_type();
+      }
+    }
+    return y;
+  }
+
+  // x and w again, for autograd: those that are there
+  static Tensor forward(AutogradContext* ctx, const std::optional<Tensor>& x, const std::optional<Tensor>& w, BlockLinearCall* c) {
+    return run(ctx, *c);
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    require(!at::GradMode::is_enabled(), "block linear: its backward has no derivative (create_graph)");
+    const auto saved = ctx->get_saved_variables();
+    const int64_t tokens = ctx->saved_data["tokens"].toInt(), in = ctx->saved_data["in"].toInt(), out = ctx->saved_data["out"].toInt();
+    const Tensor go = readable_rows(grads[0]);
+    const auto device = go.device();
+    BlockLinearCall c;
+    c.ends = saved[5];
+    const Experts e = c.experts();
+    const bool grad_x = saved[0].defined(), grad_w = saved[2].defined() || saved[4].defined();
+    Block g_rows, g_tokens;
+    if (grad_x)
+      g_rows = empty_row_blocks(tokens, out, device);
+    if (grad_w)
+      g_tokens = empty_token_blocks(tokens, out, e, device);
+    if (grad_x || grad_w)
+      quantize_blocks(go, grad_w ? e : Experts{}, grad_x ? &g_rows : nullptr, grad_w ? &g_tokens : nullptr);
+    Tensor dx, dw;
+    if (grad_w) {
+      Block x_tokens{saved[2], saved[3]};
+      if (!x_tokens.data.defined()) {
+        x_tokens = empty_token_blocks(tokens, in, e, device);
+        quantize_blocks(readable_rows(saved[4]), e, nullptr, &x_tokens);
+      }
+      // bf16 weights: rounded once in the epilogue, as the cast of an fp32 result would round it
+      dw = empty(ctx->saved_data["w_sizes"].toIntVector(), ctx->saved_data["w_dtype"].toScalarType(), device);
+      block_product(MXB200_BLOCK_WEIGHT_GRAD, g_tokens, x_tokens, dw, e, tokens, in, out);
+    }
+    if (grad_x) {
+      dx = empty({tokens, in}, at::kBFloat16, device);
+      block_product(MXB200_BLOCK_INPUT_GRAD, {saved[0], saved[1]}, g_rows, dx, e, tokens, in, out);
+    }
+    return {dx, dw, Tensor()};
+  }
+};
+
+Tensor block_linear(const std::optional<Tensor>& x, const std::optional<Tensor>& w, const GivenBlock& x_block, const GivenBlock& w_block,
+                    const std::optional<Tensor>& ends, const char* what) {
+  require_in(x.has_value() || x_block.has_value(), what, "expected an input");
+  require_in(w.has_value() || w_block.has_value(), what, "expected a weight");
+  const Tensor& first = x.has_value() ? *x : x_block->first;
+  require_cuda(first, what);
+  const Tensor& weight = w.has_value() ? *w : w_block->first;
+  require_in(first.dim() == 2 && weight.dim() == (ends.has_value() ? 3 : 2) && first.size(1) == weight.size(-1), what, "shape mismatch");
+  BlockLinearCall c;
+  c.device = first.device();
+  c.tokens = first.size(0), c.in = first.size(1), c.out = weight.size(-2);
+  require_in(block_features(c.in) && block_features(c.out), what, "in and out features must be multiples of 16");
+  require_in(weight.device() == c.device, what, "expected the weight on the input's device");
+  std::vector<int64_t> w_scale{blocks_of(c.out), blocks_of(c.in)};
+  if (ends.has_value()) {
+    require_in(ends->device() == c.device && ends->scalar_type() == at::kInt && ends->dim() == 1 && ends->is_contiguous() &&
+                     ends->numel() == weight.size(0) && ends->numel() >= 1 && ends->numel() <= 1024,
+               what, "ends must be int32 on the input's device, one per expert, 1 to 1024 of them");
+    c.ends = *ends;
+    w_scale.insert(w_scale.begin(), weight.size(0));
+  }
+  if (x.has_value()) {
+    require_in(x->scalar_type() == at::kBFloat16, what, "expected a bf16 input");
+    c.x = *x;
+  }
+  if (w.has_value()) {
+    require_in(w->scalar_type() == at::kBFloat16 || w->scalar_type() == at::kFloat, what, "expected a bf16 or fp32 weight");
+    c.w = *w;
+  }
+  if (x_block.has_value())
+    c.x_rows = given_block(*x_block, {c.tokens, c.in}, {blocks_of(c.in), c.tokens}, c.device, what);
+  if (w_block.has_value())
+    c.w_blocks = given_block(*w_block, weight.sizes(), w_scale, c.device, what);
+  const Tensor none;
+  bool grad = false;
+  for (const Tensor* t : {&c.x, &c.w})
+    if (t->defined())
+      grad |= grad_mode({t});
+  require_in(!grad || x.has_value() || !c.w.requires_grad(), what, "the weight's gradient needs the input itself, not its blocks alone");
+  const c10::cuda::CUDAGuard guard(c.device);
+  const py::gil_scoped_release nogil;
+  if (!grad)
+    return BlockLinear::run(nullptr, c);
+  return BlockLinear::apply(some(c.x), some(c.w), &c);
+}
+
+std::pair<Tensor, Tensor> quantize_block(const Tensor& x) {
+  require_cuda(x, "quantize_block");
+  require(x.dim() == 2 && x.scalar_type() == at::kBFloat16 && block_features(x.size(1)),
+          "quantize_block: expected a 2-D bf16 tensor whose columns are a multiple of 16");
+  const c10::cuda::CUDAGuard guard(x.device());
+  const py::gil_scoped_release nogil;
+  const Block q = empty_row_blocks(x.size(0), x.size(1), x.device());
+  quantize_blocks(readable_rows(x), Experts{}, &q, nullptr);
+  return {q.data, q.scale};
+}
+
+std::pair<Tensor, Tensor> quantize_block_weight(const Tensor& w) {
+  require_cuda(w, "quantize_block_weight");
+  require((w.dim() == 2 || (w.dim() == 3 && w.size(0) >= 1 && w.size(0) <= 1024)) && block_features(w.size(-1)) && block_features(w.size(-2)) &&
+                (w.scalar_type() == at::kBFloat16 || w.scalar_type() == at::kFloat),
+          "quantize_block_weight: expected a bf16 or fp32 (out, in) or (experts, out, in) with features a multiple of 16");
+  const c10::cuda::CUDAGuard guard(w.device());
+  const py::gil_scoped_release nogil;
+  const Block q = quantize_weight_blocks(w);
+  return {q.data, q.scale};
+}
+
+// (res, n, q data, q scale, rstd); res is x where there is no r, n undefined where it is not wanted.
+struct ResidualNormBlock : torch::autograd::Function<ResidualNormBlock> {
+  static variable_list run(const Tensor& x, const Tensor& r, const Tensor& gain, double eps, bool with_n) {
+    const auto device = x.device();
+    const int64_t cols = x.size(-1), rows = x.numel() / cols;
+    const Tensor res = r.defined() ? empty(x.sizes(), at::kBFloat16, device) : x;
+    const Tensor n = with_n ? empty(x.sizes(), at::kBFloat16, device) : Tensor();
+    const Block q = empty_row_blocks(rows, cols, device);
+    const Tensor rstd = empty({rows}, at::kFloat, device);
+    mxb200_block_norm_args a{};
+    a.x = x.data_ptr();
+    a.r = r.defined() ? r.data_ptr() : nullptr;
+    a.gain = gain.defined() ? gain.data_ptr() : nullptr;
+    a.res = r.defined() ? res.data_ptr() : nullptr;
+    a.n = with_n ? n.data_ptr() : nullptr;
+    a.q = q.data.data_ptr(), a.scale = static_cast<float*>(q.scale.data_ptr()), a.rstd = static_cast<float*>(rstd.data_ptr());
+    a.rows = rows, a.cols = static_cast<int32_t>(cols);
+    a.gain_bf16 = gain.defined() && gain.scalar_type() == at::kBFloat16;
+    a.eps = static_cast<float>(eps);
+    check(mxb200_block_norm_fwd(&a, stream()), "residual_norm_block");
+    return {res, n, q.data, q.scale, rstd};
+  }
+
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const std::optional<Tensor>& r_in,
+                               const std::optional<Tensor>& gain_in, double eps) {
+    const Tensor r = r_in.value_or(Tensor()), gain = gain_in.value_or(Tensor());
+    variable_list out = run(x, r, gain, eps, true);
+    ctx->save_for_backward({out[0], out[4], gain});
+    ctx->saved_data["want_gain"] = gain.defined() && gain.requires_grad();
+    ctx->mark_non_differentiable({out[2], out[3], out[4]});
+    ctx->set_materialize_grads(false);
+    ctx->saved_data["r"] = r.defined();
+    return out;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    require(!at::GradMode::is_enabled(), "residual_norm_block: its backward has no derivative (create_graph)");
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &res = saved[0], &rstd = saved[1], &gain = saved[2];
+    const bool has_r = ctx->saved_data["r"].toBool(), want_gain = ctx->saved_data["want_gain"].toBool();
+    const Tensor dres = grads[0].defined() ? dense(grads[0]) : Tensor();
+    Tensor dx, dgain;
+    if (!grads[1].defined()) {
+      dx = dres;
+      if (want_gain)
+        dgain = at::zeros_like(gain);
+    } else {
+      const Tensor dn = dense(grads[1]);
+      const int64_t cols = res.size(-1), rows = res.numel() / cols;
+      dx = empty(res.sizes(), at::kBFloat16, res.device());
+      Tensor workspace;
+      if (want_gain) {
+        dgain = empty(gain.sizes(), gain.scalar_type(), res.device());
+        workspace = empty({static_cast<int64_t>(mxb200_block_norm_workspace_bytes(rows, static_cast<int32_t>(cols)))}, at::kByte, res.device());
+      }
+      mxb200_block_norm_bwd_args a{};
+      a.dn = dn.data_ptr();
+      a.dres = dres.defined() ? dres.data_ptr() : nullptr;
+      a.res = res.data_ptr(), a.rstd = static_cast<const float*>(rstd.data_ptr());
+      a.gain = gain.defined() ? gain.data_ptr() : nullptr;
+      a.dx = dx.data_ptr(), a.dgain = want_gain ? dgain.data_ptr() : nullptr;
+      a.rows = rows, a.cols = static_cast<int32_t>(cols);
+      a.gain_bf16 = gain.defined() && gain.scalar_type() == at::kBFloat16;
+      check(mxb200_block_norm_bwd(&a, want_gain ? workspace.data_ptr() : nullptr, want_gain ? workspace.numel() : 0, stream()),
+            "residual_norm_block");
+    }
+    return {dx, has_r ? dx : Tensor(), dgain, Tensor()};
+  }
+};
+
+std::vector<std::optional<Tensor>> residual_norm_block(const Tensor& x_in, const std::optional<Tensor>& r_in, const std::optional<Tensor>& gain_in,
+                                                       double eps, bool with_n) {
+  constexpr const char* what = "residual_norm_block";
+  require_cuda(x_in, what);
+  require_in(x_in.dim() >= 1 && x_in.scalar_type() == at::kBFloat16 && block_features(x_in.size(-1)) && x_in.size(-1) <= 16384, what,
+             "expected bf16 with at most 16384 columns, a multiple of 16");
+  const Tensor r_given = r_in.has_value() ? *r_in : Tensor(), gain_given = gain_in.has_value() ? *gain_in : Tensor();
+  if (r_given.defined())
+    require_in(r_given.device() == x_in.device() && r_given.scalar_type() == at::kBFloat16 && r_given.sizes() == x_in.sizes(), what,
+               "expected r as bf16 of x's shape on its device");
+  if (gain_given.defined())
+    require_in(gain_given.device() == x_in.device() && gain_given.dim() == 1 && gain_given.size(0) == x_in.size(-1) &&
+                     (gain_given.scalar_type() == at::kFloat || gain_given.scalar_type() == at::kBFloat16),
+               what, "expected a bf16 or fp32 gain per column on x's device");
+  require_in(eps >= 0, what, "eps must not be negative");
+  bool grad = false;
+  for (const Tensor* t : {&x_in, &r_given, &gain_given})
+    if (t->defined())
+      grad |= grad_mode({t});
+  require_in(!grad || with_n, what, "n carries the gradients: with_n=False needs torch.no_grad()");
+  const c10::cuda::CUDAGuard guard(x_in.device());
+  const py::gil_scoped_release nogil;
+  const Tensor x = dense(x_in), r = r_given.defined() ? dense(r_given) : Tensor(), gain = gain_given.defined() ? dense(gain_given) : Tensor();
+  const variable_list out = grad ? ResidualNormBlock::apply(x, some(r), some(gain), eps) : ResidualNormBlock::run(x, r, gain, eps, with_n);
+  std::vector<std::optional<Tensor>> result;
+  for (const Tensor& t : out)
+    result.push_back(some(t));
+  return result;
+}
+
 // ---------------------------------------------------------------------------------------------------- other entry points
 
 // Forward of the fused residual step with MX output (residual_norm.cpp:36-96). Returns (res, n, n_mx..., rstd, s).
@@ -1069,4 +1427,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("softcap_cross_entropy", &softcap_cross_entropy);
   m.def("residual_norm_mx", &residual_norm_mx, py::call_guard<py::gil_scoped_release>());
   m.def("quantize_mx_batch_into", &quantize_mx_batch_into);
+  m.def("fp8_block_matmul", [](const std::optional<Tensor>& x, const std::optional<Tensor>& w, const GivenBlock& x_block, const GivenBlock& w_block) {
+    return block_linear(x, w, x_block, w_block, std::nullopt, "fp8_block_matmul");
+  });
+  m.def("fp8_block_experts", [](const std::optional<Tensor>& x, const std::optional<Tensor>& w, const Tensor& ends, const GivenBlock& x_block,
+                                const GivenBlock& w_block) { return block_linear(x, w, x_block, w_block, ends, "fp8_block_experts"); });
+  m.def("quantize_block", &quantize_block);
+  m.def("quantize_block_weight", &quantize_block_weight);
+  m.def("residual_norm_block", &residual_norm_block);
 }

@@ -25,6 +25,7 @@ __all__ = [
     "quantize_mx_relu_square_bwd", "residual_norm_mx", "residual_norm_mx_fits", "quantize_fp8_weight", "mx_qkv_weights", "mx_gemm", "mx_gemm_out",
     "mx_gemm_f32", "mx_gemm_relu_square", "mx_gemm_relu_square_bwd", "mx_grad_direct", "mx_grad_weights", "fp8_matmul", "fp8_qkv", "fp8_relu_square_mlp", "relu_square_mlp_mx", "fp8_eligible",
     "softcap_ce_loss", "softcap_ce_grad_mx", "softcap_cross_entropy",
+    "BlockTensor", "quantize_block", "quantize_block_weight", "fp8_block_matmul", "fp8_block_experts", "residual_norm_block",
     "SCALE_REFERENCE", "SCALE_OCP_FLOOR",
 ]
 
@@ -546,3 +547,74 @@ def softcap_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.
         raise RuntimeError("softcap_cross_entropy: MX needs N, C, chunk_rows and the padded vocab % 128")
     return native.softcap_cross_entropy(x, weight, targets, int(vocab_size), float(softcap), int(chunk_rows),
                                         ("mean", "sum", "none").index(reduction), _weight_source(cache, weight))
+
+
+# ------------------------------------------------------------------------------------------------ blocks of 128 values
+
+@dataclass
+class BlockTensor:
+    """E4M3 data with one fp32 scale for 128 values. An activation (T, C): 128 columns of a row, scale (ceil(C / 128), T). A
+    weight (out, in) or (experts, out, in): 128 x 128 values, scale (ceil(out / 128), ceil(in / 128)), with the experts in
+    front. Value = data * scale; a weight's scales may be any fp32 numbers, such as a quantized checkpoint's."""
+    data: torch.Tensor
+    scale: torch.Tensor
+
+
+def _pair(q: Optional[BlockTensor]):
+    return None if q is None else (q.data, q.scale)
+
+
+def quantize_block(x: torch.Tensor) -> BlockTensor:
+    """A (T, C) bf16 activation in blocks of 128 along its rows, C % 16 == 0, any T. The scale of a block is the smallest power
+    of two s >= 2^-126 with max|block| <= 448 s, so only the rounding to E4M3 loses bits. NaN stays NaN, Inf becomes 448 s."""
+    return BlockTensor(*native.quantize_block(x))
+
+
+def quantize_block_weight(w: torch.Tensor) -> BlockTensor:
+    """A bf16 or fp32 weight (out, in) or (experts, out, in) in blocks of 128 x 128, features % 16 == 0, scales as
+    quantize_block's."""
+    return BlockTensor(*native.quantize_block_weight(w))
+
+
+def _block_weight(w, cache):
+    """(the weight for autograd or None, its blocks or None)"""
+    if isinstance(w, BlockTensor):
+        return None, _pair(w)
+    if cache is None:
+        return w, None
+    q = cache.get(2, [w], lambda: list(native.quantize_block_weight(w)))
+    return w, (q[0], q[1])
+
+
+def fp8_block_matmul(x: Optional[torch.Tensor], w, x_block: Optional[BlockTensor] = None,
+                     cache: Optional[Fp8WeightCache] = None) -> torch.Tensor:
+    """x (T, in) bf16, w (out, in) -> (T, out) bf16: fp8_matmul with blocks of 128 instead of 32, for any T (one token, none) and
+    features % 16 == 0. w: a bf16 or fp32 weight, quantized here or kept by cache, or a BlockTensor (no gradient). x_block: x
+    already quantized (quantize_block, residual_norm_block); x then only carries autograd and may be None where the weight gets
+    no gradient.
+
+    Gradients come through autograd, the weight's in its own type. They use the incoming gradient in blocks along its rows for
+    dx, and gradient and input in blocks of 128 tokens for dw."""
+    w, w_block = _block_weight(w, cache)
+    return native.fp8_block_matmul(x, w, _pair(x_block), w_block)
+
+
+def fp8_block_experts(x: Optional[torch.Tensor], w, ends: torch.Tensor, x_block: Optional[BlockTensor] = None,
+                      cache: Optional[Fp8WeightCache] = None) -> torch.Tensor:
+    """fp8_block_matmul of each expert's rows with its own weight: x (T, in) bf16 sorted by expert, w (experts, out, in), ends
+    (experts) int32 on the device, the running total of the experts' row counts -> (T, out) bf16. Expert e has rows
+    [ends[e - 1], ends[e]), which may be none; rows behind the last end belong to nobody, their outputs and gradients are
+    zeros. ends is never read on the host; an end below the previous one, or above T, counts as that. At most 1024 experts.
+    Token blocks of the weight's gradient start over at every expert."""
+    w, w_block = _block_weight(w, cache)
+    return native.fp8_block_experts(x, w, ends, _pair(x_block), w_block)
+
+
+def residual_norm_block(x: torch.Tensor, r: Optional[torch.Tensor] = None, gain: Optional[torch.Tensor] = None,
+                        eps: float = torch.finfo(torch.float32).eps, with_n: bool = True):
+    """res = x + r (bf16), n = rms_norm(res) * gain, and n in blocks of 128: (res, n, n_block, rstd). x, r: bf16 (..., C), C a
+    multiple of 16 up to 16384; gain: (C) bf16 or fp32. n_block is quantize_block(n.view(-1, C)), bit for bit: hand it to
+    fp8_block_matmul or fp8_block_experts as x_block, with n as x. Without r, res is x. Gradients reach x, r and gain through res
+    and n. with_n=False (no gradients then): n is not written and None."""
+    res, n, data, scale, rstd = native.residual_norm_block(x, r, gain, eps, with_n)
+    return res, n, BlockTensor(data, scale), rstd
