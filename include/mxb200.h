@@ -266,18 +266,20 @@ MXB200_API int mxb200_gemm_group(const mxb200_gemm_desc* g, int n, void* workspa
  * Rows may be sorted by expert: expert e of `experts` (<= 1024) has rows [ends[e - 1], ends[e]), ends being int32 on the
  * device, never read on the host; an end is held to between the previous expert's and the number of rows. Rows behind the last
  * end are nobody's. ends null (experts = 1): one expert has all rows. Features are multiples of 16, rows may be any number.
- * All pointers 16-byte aligned (ends, and the scales that a product reads: 4).
+ * All pointers 16-byte aligned (ends, and the fp32 scales that a product reads: 4).
  *
  * Token blocks: how many blocks of 128 rows the tokens of `experts` experts take at most, each expert's starting a new one; the
  * operands of a weight gradient have 128 times as many rows. */
 MXB200_API int64_t mxb200_block_token_blocks(int64_t tokens, int experts);
 
 /* x: (rows, cols) bf16 with ld >= cols values between rows (ld % 8 == 0). row_data (rows, cols) e4m3 and row_scale
- * (ceil(cols / 128), rows): blocks along rows. token_data (128 * token blocks, cols) and token_scale (token blocks, cols): blocks
- * along each expert's tokens, whose last block is filled up with zeros. Either may be null. With token_data, rows of no expert
- * are written to neither. */
+ * (ceil(cols / 128), rows): blocks along rows. token_data (128 * token blocks, cols) and token_scale (token blocks,
+ * ceil(cols / 128), 128): blocks along each expert's tokens, whose last block is filled up with zeros. Their scales, always
+ * powers of two, are kept as the tensor core takes them: for each 128 columns a tile of 128 words, the word of column c at
+ * 4 (c % 32) + c / 32 within the tile, its four bytes the scale's biased exponent. Either output may be null. With token_data,
+ * rows of no expert are written to neither. */
 MXB200_API int mxb200_block_quantize(const void* x, int64_t rows, int64_t cols, int64_t ld, const int32_t* ends, int experts,
-                                     void* row_data, float* row_scale, void* token_data, float* token_scale, void* stream);
+                                     void* row_data, float* row_scale, void* token_data, uint32_t* token_scale, void* stream);
 
 /* w: (experts, rows, cols) contiguous, bf16 (w_bf16 != 0) or fp32, to data of that shape and scale
  * (experts, ceil(rows / 128), ceil(cols / 128)). */
@@ -294,9 +296,9 @@ typedef enum mxb200_block_kind {
  * expert without rows: zeros. Needs no workspace. tokens may be 0. */
 typedef struct mxb200_block_gemm_args {
   const void* a;
-  const float* a_scale;
+  const void* a_scale; /* fp32; the weight gradient's as mxb200_block_quantize makes token_scale */
   const void* b;
-  const float* b_scale;
+  const void* b_scale;
   void* d;
   const int32_t* ends;
   int64_t tokens, in_features, out_features;

@@ -4,16 +4,23 @@
 //   input grad    dx[t, k] = sum over blocks b of sg[b, t] sw[b, k / 128]  * sum over n in b of gq[t, n] wq[n, k]
 //   weight grad   dw[n, k] = sum over token blocks b of sg[b, n] sx[b, k]  * sum over t in b of gq[t, n] xq[t, k]
 //
-// Rows (tokens) may be sorted by expert; each expert has its own weight, and token blocks never cross experts.
+// Rows (tokens) may be sorted by expert; each expert has its own weight, and token blocks never cross experts. No operand is
+// ever transposed in memory: the input gradient contracts over the weight's rows and the weight gradient over tokens, and both
+// read their operands as they lie, row-contiguous, through the tensor core's MN-major form.
 //
-// The scales are any fp32 numbers, so they cannot ride on the tensor core's own block scales (powers of two): the tensor core
-// makes the plain fp32 product of one block (K = 128: four MMAs) in tensor memory, and the epilogue warps take it from there
-// with one fused multiply-add per value into accumulators in registers, while the next block's MMAs fill another tensor
-// memory buffer. The rows of the tensor core's tile (its lanes) are the weight's, the columns are tokens: few tokens then
-// cost few columns, not a tile of 128 rows, and an expert's last tile is as narrow as its last rows.
+// Forward and input gradient take any fp32 scales, which cannot ride on the tensor core's own block scales (powers of two): the
+// tensor core makes the plain fp32 product of one block (K = 128: four MMAs) in tensor memory, and the epilogue warps take it
+// from there with one fused multiply-add per value into accumulators in registers, while the next block's MMAs fill another
+// tensor memory buffer. Two kernels:
+//   * many tokens: a CTA pair, 256 tokens (the tensor core's rows, tensor memory's lanes) x 256 features. A thread has one
+//     token and 128 features of one weight block, so one scale, the product of the two, serves all its values: 64 packed
+//     multiply-adds per block and nothing else.
+//   * few tokens: one CTA, 128 features (rows) x up to 128 tokens (columns). Few tokens cost few columns, not a tile of 128
+//     rows, and an expert's last tile is as narrow as its last rows. Scales differ by column: fragments (16x256b) give a thread
+//     8 columns of 4 rows each 32, so that a scale read from shared memory serves 4 values.
 //
-// No operand is ever transposed in memory. The input gradient contracts over the weight's rows and the weight gradient over
-// tokens; both read their operands as they lie, row-contiguous, through the tensor core's MN-major form.
+// The weight gradient's scales are this library's own, powers of two, and differ by row and by column: here the tensor core
+// applies them (kind::mxf8f6f4, the four K = 32 steps of a block under the same scale byte) and sums up in tensor memory.
 #include <algorithm>
 #include <cstddef>
 #include <cstdint>
@@ -34,12 +41,17 @@ namespace {
 constexpr uint64_t kWaitLimitNs = 2000000000ull;
 constexpr uint32_t kTmemCols = 512;
 constexpr int kEpilogueWarps = 8;
-constexpr int kThreads = 32 * (2 + kEpilogueWarps);
-constexpr int kStages = 5;
+// Warps 0 to 2 load operands, issue MMAs and load scales, warp 3 idles; 4 to 11 are the epilogue. The epilogue warps of the
+// pair kernel need more registers than an even share (168 of 384 threads): they draw on the first four warps' (setmaxnreg; the
+// sum, 128 x 72 + 256 x 216, is what the block was launched with).
+constexpr int kFirstEpilogueWarp = 4;
+constexpr int kThreads = 32 * (kFirstEpilogueWarp + kEpilogueWarps);
+constexpr int kLaunchRegisters = 168, kFewRegisters = 72, kManyRegisters = 216;
+static_assert(4 * kFewRegisters + kEpilogueWarps * kManyRegisters <= (4 + kEpilogueWarps) * kLaunchRegisters, "registers of the block");
 constexpr int kScaleSlots = 8;
 constexpr uint32_t kABytes = 128 * 128, kBBytes = 128 * 128;
-constexpr uint32_t kBBoxBytes = 32 * 128;  // tokens' rows come 32 at a time, as many as the tile has
-constexpr int kPanel = 8;                  // weight tiles per raster panel
+constexpr uint32_t kBBoxBytes = 32 * 128;  // few tokens' rows come 32 at a time, as many as the tile has
+constexpr int kPanel = 8;                  // feature tiles per raster panel
 
 enum Mode : int { kForward = 0, kInputGrad = 1, kWeightGrad = 2 };
 
@@ -50,77 +62,57 @@ enum WaitSite : uint32_t {
   kSiteAccEmpty = 4,
   kSiteAccFull = 5,
   kSiteScaleFull = 6,
+  kSiteOverlap = 7,
 };
 
-template <int kCtas>
-struct Tile {
-  static constexpr int kM = 128 * kCtas;
-  static constexpr int kN = 128 * kCtas;
-  static constexpr int kPartN = kN / 2;           // columns per epilogue warp: two warps share a tensor memory quarter
-  static constexpr int kChunks = kPartN / 32;
-  static constexpr int kAccBuffers = kTmemCols / kN;
-};
-
-// What the columns' scales and, for the weight gradient, the rows' are to one block.
-struct ScaleSlot {
-  float col[256];
-  float row[128];  // [0] alone holds the weight's scale in the other two modes
-};
-
-constexpr uint32_t kStageRowBytes = 80;  // 32 bf16 and 16 bytes that put 8 rows' 16-byte pieces into different banks
-constexpr uint32_t kOutBytes = 32 * kStageRowBytes;
-
-struct Shared {
-  ScaleSlot scales[kScaleSlots];
-  unsigned char out[kEpilogueWarps][kOutBytes];
+// Barriers and what the roles of a CTA share. kStages: operand stages of kABytes + kBBytes.
+template <int kStages_>
+struct Common {
+  static constexpr int kStages = kStages_;
   uint64_t full[kStages], empty[kStages];
   uint64_t acc_full[4], acc_empty[4];
   uint64_t scale_full[kScaleSlots], scale_empty[kScaleSlots];
+  uint64_t overlap_free;
   uint32_t tmem_base;
   uint32_t abort_flag;
   int first_row[kMaxExperts + 2];
   int first_tile[kMaxExperts + 2];
 };
 
-constexpr size_t kSmemBytes = 1024 + kStages * static_cast<size_t>(kABytes + kBBytes) + sizeof(Shared);
-static_assert(kSmemBytes <= 232448, "shared memory of one CTA");
-static_assert(kStages * kABytes >= kMaxExperts * 4, "the operand stages hold the scan's copy of ends");
-
 struct Params {
-  const float* col_scale;  // (blocks, col_ld)
-  const float* row_scale;  // weight gradient: (blocks, row_ld); else the weight's (experts, ., .)
-  int64_t col_ld, row_ld;
+  const float* token_scale;   // (blocks, token_ld)
+  const float* weight_scale;  // (experts, ., .)
+  int64_t token_ld;
   int64_t w_scale_expert;
-  int w_scale_m, w_scale_b;  // strides of the weight's scale over row tiles of 128 and over blocks
+  int w_scale_f, w_scale_b;   // strides of the weight's scale over feature tiles of 128 and over blocks
   void* d;
   const int32_t* ends;
-  int experts;     // 1 where ends is null
-  int rows;        // tokens
-  int m, n;        // rows of the A operand; columns of the output of a weight gradient
-  int blocks;      // contraction blocks (forward, input grad)
+  int experts;   // 1 where ends is null
+  int rows;      // tokens
+  int features;  // of the output; weight gradient: its rows
+  int n;         // weight gradient: its columns
+  int blocks;    // contraction blocks (forward, input grad)
   int out_bf16;
 };
 
-struct Unit {
-  int expert;
-  int m0, n0;        // first row of A; first token, or first column of dw
-  int cols;          // columns that exist
-  int block0, blocks;
+struct Maps {
+  CUtensorMap a, b;
+  CUtensorMap a_scale, b_scale;  // weight gradient
 };
 
-__device__ __forceinline__ bool wait_bounded(uint32_t bar, uint32_t parity, Shared* s, uint32_t site) {
+__device__ __forceinline__ bool wait_bounded(uint32_t bar, uint32_t parity, uint32_t* abort_flag, uint32_t site) {
   bool ok = true;
   if (!mbar_try_wait(bar, parity)) {
     const uint64_t t0 = global_timer_ns();
     uint32_t spins = 0;
     while (!mbar_try_wait(bar, parity)) {
       if ((++spins & 63u) == 0) {
-        if (*reinterpret_cast<volatile uint32_t*>(&s->abort_flag) != 0) {
+        if (*reinterpret_cast<volatile uint32_t*>(abort_flag) != 0) {
           ok = false;
           break;
         }
         if (global_timer_ns() - t0 > kWaitLimitNs) {
-          *reinterpret_cast<volatile uint32_t*>(&s->abort_flag) = 1;
+          *reinterpret_cast<volatile uint32_t*>(abort_flag) = 1;
           atomicCAS(&g_block_gemm_watchdog_word, 0u, 0x20000000u | (blockIdx.x << 8) | site);
           ok = false;
           break;
@@ -159,319 +151,24 @@ __device__ __forceinline__ float2 both(uint64_t v) {
   return make_float2(__uint_as_float(lo), __uint_as_float(hi));
 }
 
-// The position a walk over units has in (expert, weight tile, token tile): all of a panel's weight tiles for one token tile,
-// then for the next, so that the CTAs at work at one time share operands in L2.
-template <int kMode, int kCtas>
-__device__ __forceinline__ Unit unit_at(const Params& p, const Shared* s, int u) {
-  using T = Tile<kCtas>;
-  const int mt = (p.m + T::kM - 1) / T::kM;
-  Unit x;
-  int nt, v;
-  if constexpr (kMode == kWeightGrad) {
-    nt = (p.n + T::kN - 1) / T::kN;
-    x.expert = u / (mt * nt);
-    v = u - x.expert * mt * nt;
-    x.block0 = s->first_tile[x.expert];
-    x.blocks = s->first_tile[x.expert + 1] - x.block0;
-  } else {
-    const int t = u / mt;  // token tiles before this one, over all experts
-    x.expert = expert_of_tile(s->first_tile, p.experts + (p.ends != nullptr), t);
-    nt = s->first_tile[x.expert + 1] - s->first_tile[x.expert];
-    v = u - s->first_tile[x.expert] * mt;
-    x.block0 = 0;
-    x.blocks = x.expert < p.experts ? p.blocks : 0;  // rows of no expert: zeros
-  }
-  const int panel = v / (kPanel * nt);
-  v -= panel * kPanel * nt;
-  const int width = min(kPanel, mt - panel * kPanel);
-  const int n = v / width;
-  x.m0 = (panel * kPanel + v - n * width) * T::kM;
-  x.n0 = n * T::kN;
-  if constexpr (kMode == kWeightGrad) {
-    x.cols = min(T::kN, p.n - x.n0);
-  } else {
-    x.n0 += s->first_row[x.expert];
-    x.cols = min(T::kN, s->first_row[x.expert + 1] - x.n0);
-  }
-  return x;
-}
-
-// ---------------------------------------------------------------------------------------------------- producer
-
-template <int kMode, int kCtas>
-__device__ __forceinline__ void produce(const Params& p, const CUtensorMap* map_a, const CUtensorMap* map_b, Shared* s,
-                                        uint32_t a0, uint32_t b0, int rank, int first, int step, int units, int lane) {
-  using T = Tile<kCtas>;
-  const uint32_t el = elect_one() ? 1u : 0u;
-  const uint32_t empty0 = smem_u32(&s->empty[0]), full0 = smem_u32(&s->full[0]);
-  const uint32_t full_leader0 = kCtas == 2 ? map_to_cta(full0, 0) : full0;
-  const uint32_t scale_full0 = smem_u32(&s->scale_full[0]), scale_empty0 = smem_u32(&s->scale_empty[0]);
-  uint32_t stage = 0, phase = 0, slot = 0, slot_phase = 0;
-  for (int u = first; u < units; u += step) {
-    const Unit x = unit_at<kMode, kCtas>(p, s, u);
-    const int half = (x.cols + 16 * kCtas - 1) / (16 * kCtas) * 16;  // columns of the tile that this CTA brings
-    const int row_a = x.m0 + rank * 128, col_b = x.n0 + rank * half;
-    const int boxes = kMode == kWeightGrad ? 4 : (half + 31) / 32;
-    const uint32_t bytes = kABytes + boxes * kBBoxBytes;
-    for (int b = 0; b < x.blocks; ++b) {
-      if (!wait_bounded(empty0 + stage * 8, phase ^ 1u, s, kSiteStageEmpty))
-        return;
-      const int k = (x.block0 + b) * kBlock;
-      const uint32_t full = full_leader0 + stage * 8;
-      if (rank == 0)
-        mbar_arrive_expect_tx(el, full0 + stage * 8, bytes * kCtas);
-      const int ax = kMode == kForward ? k : row_a, ay = kMode == kForward ? row_a : k;
-      const int az = kMode == kWeightGrad ? 0 : x.expert;
-      if constexpr (kCtas == 2)
-        tma_load_3d_pair(el, a0 + stage * kABytes, map_a, full, ax, ay, az);
-      else
-        tma_load_3d(el, a0 + stage * kABytes, map_a, full, ax, ay, az);
-      for (int i = 0; i < boxes; ++i) {
-        const int bx = kMode == kWeightGrad ? col_b : k, by = (kMode == kWeightGrad ? k : col_b) + 32 * i;
-        const uint32_t dst = b0 + stage * kBBytes + i * kBBoxBytes;
-        if constexpr (kCtas == 2)
-          tma_load_3d_pair(el, dst, map_b, full, bx, by, 0);
-        else
-          tma_load_3d(el, dst, map_b, full, bx, by, 0);
-      }
-      if (++stage == kStages)
-        stage = 0, phase ^= 1u;
-
-      // the block's scales
-      if (!wait_bounded(scale_empty0 + slot * 8, slot_phase ^ 1u, s, kSiteScaleEmpty))
-        return;
-      const uint32_t dst = smem_u32(&s->scales[slot]);
-      const float* col = p.col_scale + (x.block0 + b) * p.col_ld + x.n0;
-      for (int i = lane; i < x.cols; i += 32)
-        cp_async_4(dst + 4 * i, col + i);
-      const uint32_t row_dst = dst + static_cast<uint32_t>(offsetof(ScaleSlot, row));
-      if constexpr (kMode == kWeightGrad) {
-        const float* row = p.row_scale + (x.block0 + b) * p.row_ld + row_a;
-        for (int i = lane; i < 128; i += 32)
-          if (row_a + i < p.m)
-            cp_async_4(row_dst + 4 * i, row + i);
-      } else if (lane == 0 && row_a < p.m) {
-        cp_async_4(row_dst, p.row_scale + x.expert * p.w_scale_expert + (row_a >> 7) * static_cast<int64_t>(p.w_scale_m) +
-                                  (x.block0 + b) * static_cast<int64_t>(p.w_scale_b));
-      }
-      cp_async_arrive(scale_full0 + slot * 8);
-      if (++slot == kScaleSlots)
-        slot = 0, slot_phase ^= 1u;
-    }
-  }
-}
-
-// ---------------------------------------------------------------------------------------------------- MMA issuer
-
-template <int kMode, int kCtas>
-__device__ __forceinline__ void issue_mmas(const Params& p, Shared* s, uint32_t a0, uint32_t b0, uint32_t tmem_base, int first,
-                                           int step, int units) {
-  using T = Tile<kCtas>;
-  constexpr bool kAMn = kMode != kForward, kBMn = kMode == kWeightGrad;
-  // 128-byte swizzle, groups of 8 rows of 128 bytes 1024 apart. K-major: K = 32 is 32 bytes within a row; MN-major: 32 rows.
-  constexpr uint32_t kAStep = kAMn ? 4096 >> 4 : 32 >> 4, kBStep = kBMn ? 4096 >> 4 : 32 >> 4;
-  const uint32_t el = elect_one() ? 1u : 0u;
-  const uint32_t empty0 = smem_u32(&s->empty[0]), full0 = smem_u32(&s->full[0]);
-  const uint64_t a_desc0 = make_smem_desc(a0, 1024, 1024, 2), b_desc0 = make_smem_desc(b0, 1024, 1024, 2);
-  uint32_t stage = 0, phase = 0, buf = 0, buf_phase = 0;
-  for (int u = first; u < units; u += step) {
-    const Unit x = unit_at<kMode, kCtas>(p, s, u);
-    const uint32_t n = (x.cols + 16 * kCtas - 1) / (16 * kCtas) * (16 * kCtas);
-    const uint32_t idesc = make_idesc_f8(T::kM, n, kAMn, kBMn);
-    for (int b = 0; b < x.blocks; ++b) {
-      if (!wait_bounded(smem_u32(&s->acc_empty[buf]), buf_phase ^ 1u, s, kSiteAccEmpty) ||
-          !wait_bounded(full0 + stage * 8, phase, s, kSiteStageFull))
-        return;
-      tcgen05_fence_after_sync();
-      const uint32_t acc = tmem_base + buf * T::kN;
-      const uint64_t a = a_desc0 + stage * (kABytes >> 4), bd = b_desc0 + stage * (kBBytes >> 4);
-#pragma unroll
-      for (uint32_t k = 0; k < 4; ++k) {
-        if constexpr (kCtas == 2)
-          tcgen05_mma_f8_pair(el, acc, a + k * kAStep, bd + k * kBStep, idesc, k > 0);
-        else
-          tcgen05_mma_f8(el, acc, a + k * kAStep, bd + k * kBStep, idesc, k > 0);
-      }
-      if constexpr (kCtas == 2) {
-        tcgen05_commit_pair(el, empty0 + stage * 8, 3);
-        tcgen05_commit_pair(el, &s->acc_full[buf], 3);
-      } else {
-        tcgen05_commit(el, &s->empty[stage]);
-        tcgen05_commit(el, &s->acc_full[buf]);
-      }
-      if (++stage == kStages)
-        stage = 0, phase ^= 1u;
-      if (++buf == T::kAccBuffers)
-        buf = 0, buf_phase ^= 1u;
-    }
-  }
-}
-
-// ---------------------------------------------------------------------------------------------------- epilogue
-
-// 32 columns of this warp's 32 rows to the output. v[j][i]: 8-column group j, row 8 i + lane / 4, columns 2 (lane % 4), + 1.
-template <int kMode>
-__device__ __forceinline__ void store_chunk(const Params& p, const Unit& x, unsigned char* stage, int lane, int row0, int c0,
-                                            const uint64_t (&v)[4][4]) {
-  const uint32_t st = smem_u32(stage);
-  if (kMode == kWeightGrad && !p.out_bf16) {
-    float* d = static_cast<float*>(p.d) + static_cast<int64_t>(x.expert) * p.m * p.n;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row = row0 + 8 * i + (lane >> 2);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int c = c0 + 8 * j + 2 * (lane & 3);
-        if (row < p.m && c < x.cols)
-          *reinterpret_cast<float2*>(d + static_cast<int64_t>(row) * p.n + x.n0 + c) = both(v[j][i]);
-      }
-    }
-    return;
-  }
-  __syncwarp();  // the previous chunk has been read out
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    uint32_t h[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = both(v[j][i]);
-      h[i] = pack_bf16x2_rn(f.x, f.y);
-    }
-    if constexpr (kMode == kWeightGrad)  // a row of the stage: 32 columns of one row of dw
-      stmatrix_x4(st + lane * kStageRowBytes + j * 16, h[0], h[1], h[2], h[3]);
-    else  // ... 32 features of one token
-      stmatrix_x4_trans(st + (8 * j + (lane & 7)) * kStageRowBytes + (lane >> 3) * 16, h[0], h[1], h[2], h[3]);
-  }
-  __syncwarp();
-  uint16_t* d = static_cast<uint16_t*>(p.d);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = 8 * i + (lane >> 2), piece = lane & 3;
-    const uint4 w = *reinterpret_cast<const uint4*>(stage + r * kStageRowBytes + piece * 16);
-    if constexpr (kMode == kWeightGrad) {
-      const int64_t row = static_cast<int64_t>(x.expert) * p.m + row0 + r;
-      if (row0 + r < p.m && c0 + piece * 8 < x.cols)
-        *reinterpret_cast<uint4*>(d + row * p.n + x.n0 + c0 + piece * 8) = w;
-    } else {
-      if (c0 + r < x.cols && row0 + piece * 8 < p.m)
-        *reinterpret_cast<uint4*>(d + static_cast<int64_t>(x.n0 + c0 + r) * p.m + row0 + piece * 8) = w;
-    }
-  }
-}
-
-template <int kMode, int kCtas>
-__device__ __forceinline__ void accumulate(const Params& p, Shared* s, uint32_t tmem_base, int rank, int first, int step, int units,
-                                           int warp, int lane) {
-  using T = Tile<kCtas>;
-  const int quarter = warp & 3, part = (warp - 2) >> 2;  // a warp may read the tensor memory lanes 32 (warp % 4) on
-  const int part0 = part * T::kPartN;
-  const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
-  const uint32_t acc_empty0 = kCtas == 2 ? map_to_cta(smem_u32(&s->acc_empty[0]), 0) : smem_u32(&s->acc_empty[0]);
-  unsigned char* stage = s->out[warp - 2];
-  uint32_t buf = 0, buf_phase = 0, slot = 0, slot_phase = 0;
-  for (int u = first; u < units; u += step) {
-    const Unit x = unit_at<kMode, kCtas>(p, s, u);
-    uint64_t acc[T::kChunks][4][4];
-#pragma unroll
-    for (int c = 0; c < T::kChunks; ++c)
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          acc[c][j][i] = 0;
-    for (int b = 0; b < x.blocks; ++b) {
-      if (!wait_bounded(smem_u32(&s->scale_full[slot]), slot_phase, s, kSiteScaleFull) ||
-          !wait_bounded(smem_u32(&s->acc_full[buf]), buf_phase, s, kSiteAccFull))
-        return;
-      tcgen05_fence_after_sync();
-      const ScaleSlot& sc = s->scales[slot];
-      uint64_t row_scale[4];
-      if constexpr (kMode == kWeightGrad) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float f = sc.row[quarter * 32 + 8 * i + (lane >> 2)];
-          row_scale[i] = pair_f32(f, f);
-        }
-      } else {
-        row_scale[0] = pair_f32(sc.row[0], sc.row[0]);
-      }
-      const uint32_t t = tmem_base + lane_base + buf * T::kN + part0;
-#pragma unroll
-      for (int c = 0; c < T::kChunks; ++c) {
-        if (part0 + 32 * c >= x.cols)
-          break;
-        uint32_t lo[16], hi[16];
-        tmem_ld_16x256b_x4(t + 32 * c, lo);
-        tmem_ld_16x256b_x4(t + 32 * c + (16u << 16), hi);
-        uint64_t col[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 f = *reinterpret_cast<const float2*>(&sc.col[part0 + 32 * c + 8 * j + 2 * (lane & 3)]);
-          col[j] = pair_f32(f.x, f.y);
-          if constexpr (kMode != kWeightGrad)
-            col[j] = mul_f32x2(col[j], row_scale[0]);
-        }
-        tmem_ld_wait();
-#pragma unroll
-        for (int k = 0; k < 16; ++k)
-          asm volatile("" : "+r"(lo[k]), "+r"(hi[k]));
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint64_t v = i < 2 ? pair_u32(lo[4 * j + 2 * i], lo[4 * j + 2 * i + 1])
-                                     : pair_u32(hi[4 * j + 2 * i - 4], hi[4 * j + 2 * i - 3]);
-            const uint64_t f = kMode == kWeightGrad ? mul_f32x2(col[j], row_scale[i]) : col[j];
-            acc[c][j][i] = fma_f32x2(v, f, acc[c][j][i]);
-          }
-      }
-      tcgen05_fence_before_sync();
-      __syncwarp();
-      if (lane == 0) {
-        if constexpr (kCtas == 2)
-          mbar_arrive_cluster(acc_empty0 + buf * 8);
-        else
-          mbar_arrive(&s->acc_empty[buf]);
-        mbar_arrive(&s->scale_empty[slot]);
-      }
-      if (++buf == T::kAccBuffers)
-        buf = 0, buf_phase ^= 1u;
-      if (++slot == kScaleSlots)
-        slot = 0, slot_phase ^= 1u;
-    }
-    const int row0 = x.m0 + rank * 128 + quarter * 32;
-#pragma unroll
-    for (int c = 0; c < T::kChunks; ++c)
-      if (part0 + 32 * c < x.cols && row0 < p.m)
-        store_chunk<kMode>(p, x, stage, lane, row0, part0 + 32 * c, acc[c]);
-  }
-}
-
-// ---------------------------------------------------------------------------------------------------- kernel
-
-template <int kMode, int kCtas>
-__device__ __forceinline__ void block_gemm_body(const Params& p, const CUtensorMap* map_a, const CUtensorMap* map_b) {
-  using T = Tile<kCtas>;
-  extern __shared__ unsigned char smem_raw[];
-  unsigned char* base = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
-  const uint32_t a0 = smem_u32(base), b0 = a0 + kStages * kABytes;
-  Shared* s = reinterpret_cast<Shared*>(base + kStages * (kABytes + kBBytes));
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = kCtas == 2 ? static_cast<int>(cluster_ctarank()) : 0;
-
+// Barriers, tensor memory and the experts' rows; the operand stages at `base` hold the scan's words meanwhile. All threads.
+template <int kCtas, typename S>
+__device__ __forceinline__ uint32_t set_up(const Params& p, const CUtensorMap* map_a, const CUtensorMap* map_b, S* s, unsigned char* base,
+                                           int warp, int acc_buffers, uint32_t scale_arrivals, int tile_rows, bool rest_is_a_tile) {
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kStages; ++i) {
+    for (int i = 0; i < S::kStages; ++i) {
       mbar_init(&s->full[i], 1);
       mbar_init(&s->empty[i], 1);
     }
-    for (int i = 0; i < T::kAccBuffers; ++i) {
+    for (int i = 0; i < acc_buffers; ++i) {
       mbar_init(&s->acc_full[i], 1);
       mbar_init(&s->acc_empty[i], kEpilogueWarps * kCtas);
     }
     for (int i = 0; i < kScaleSlots; ++i) {
-      mbar_init(&s->scale_full[i], 32);
+      mbar_init(&s->scale_full[i], scale_arrivals);
       mbar_init(&s->scale_empty[i], kEpilogueWarps);
     }
+    mbar_init(&s->overlap_free, 4 * kCtas);
     s->abort_flag = 0;
     fence_mbar_init();
     prefetch_tensormap(map_a);
@@ -488,40 +185,25 @@ __device__ __forceinline__ void block_gemm_body(const Params& p, const CUtensorM
   }
   tcgen05_fence_before_sync();
   grid_dependency_wait();
-  scan_experts(p.ends, p.experts, p.rows, kMode == kWeightGrad ? kBlock : T::kN, s->first_row, s->first_tile,
-               reinterpret_cast<int*>(base));
-  if (kMode != kWeightGrad && p.ends != nullptr) {
+  scan_experts(p.ends, p.experts, p.rows, tile_rows, s->first_row, s->first_tile, reinterpret_cast<int*>(base));
+  if (rest_is_a_tile && p.ends != nullptr && threadIdx.x == 0) {
     // the rows behind the last expert's, as one more expert without a weight
-    if (threadIdx.x == 0) {
-      s->first_row[p.experts + 1] = p.rows;
-      s->first_tile[p.experts + 1] = s->first_tile[p.experts] + (p.rows - s->first_row[p.experts] + T::kN - 1) / T::kN;
-    }
-    __syncthreads();
+    s->first_row[p.experts + 1] = p.rows;
+    s->first_tile[p.experts + 1] = s->first_tile[p.experts] + (p.rows - s->first_row[p.experts] + tile_rows - 1) / tile_rows;
   }
-  // the scan's words lie where operands are loaded to
-  fence_proxy_async_smem();
+  fence_proxy_async_smem();  // operands are loaded over the scan's words
   __syncthreads();
   if constexpr (kCtas == 2) {
     cluster_arrive();  // the peer's barriers exist before anything is credited to them
     cluster_wait();
   }
   tcgen05_fence_after_sync();
-  const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(&s->tmem_base);
+  return *reinterpret_cast<volatile uint32_t*>(&s->tmem_base);
+}
 
-  const int mt = (p.m + T::kM - 1) / T::kM;
-  const int units = kMode == kWeightGrad ? p.experts * mt * ((p.n + T::kN - 1) / T::kN)
-                                         : s->first_tile[p.experts + (p.ends != nullptr)] * mt;
-  const int first = blockIdx.x / kCtas, step = gridDim.x / kCtas;
-  if (warp == 0) {
-    produce<kMode, kCtas>(p, map_a, map_b, s, a0, b0, rank, first, step, units, lane);
-  } else if (warp == 1) {
-    if (rank == 0)
-      issue_mmas<kMode, kCtas>(p, s, a0, b0, tmem_base, first, step, units);
-  } else {
-    accumulate<kMode, kCtas>(p, s, tmem_base, rank, first, step, units, warp, lane);
-  }
+template <int kCtas, typename S>
+__device__ __forceinline__ void tear_down(S* s, uint32_t tmem_base, int warp) {
   __syncwarp();
-
   // on an abort, copies and MMAs in flight get time to land before shared and tensor memory go away
   if (*reinterpret_cast<volatile uint32_t*>(&s->abort_flag) != 0) {
     const uint64_t t0 = global_timer_ns();
@@ -543,21 +225,702 @@ __device__ __forceinline__ void block_gemm_body(const Params& p, const CUtensorM
   }
 }
 
+// Where a walk over the units of forward or input gradient is: token tiles (kTokens rows) x feature tiles (kFeatures). Within an
+// expert all of a panel's feature tiles for one token tile, then for the next, so that what runs at one time shares operands in
+// L2.
+struct Unit {
+  int expert;
+  int row0, rows;  // tokens
+  int f0;          // first feature
+  int blocks;      // 0: rows of no expert, zeros
+};
+
+template <int kTokens, int kFeatures, typename S>
+__device__ __forceinline__ Unit unit_at(const Params& p, const S* s, int u) {
+  const int ft = (p.features + kFeatures - 1) / kFeatures;
+  const int t = u / ft;  // token tiles before this one, over all experts
+  Unit x;
+  x.expert = expert_of_tile(s->first_tile, p.experts + (p.ends != nullptr), t);
+  x.blocks = x.expert < p.experts ? p.blocks : 0;
+  const int tiles = s->first_tile[x.expert + 1] - s->first_tile[x.expert];
+  int v = u - s->first_tile[x.expert] * ft;
+  const int panel = v / (kPanel * tiles);
+  v -= panel * kPanel * tiles;
+  const int width = min(kPanel, ft - panel * kPanel);
+  const int n = v / width;
+  x.f0 = (panel * kPanel + v - n * width) * kFeatures;
+  x.row0 = s->first_row[x.expert] + n * kTokens;
+  x.rows = min(kTokens, s->first_row[x.expert + 1] - x.row0);
+  return x;
+}
+
+template <typename S>
+__device__ __forceinline__ int units_of(const Params& p, const S* s, int features_per_tile) {
+  return s->first_tile[p.experts + (p.ends != nullptr)] * ((p.features + features_per_tile - 1) / features_per_tile);
+}
+
+// Output of a thread's row, 128 bytes at a time, through shared memory: a row per lane goes in, four whole rows (128-byte lines)
+// per store instruction come out. Written straight from the rows' owners, 16 bytes in each of 32 rows per instruction, the
+// stores took longer than the products of up to 20 blocks.
+constexpr uint32_t kLineRowBytes = 144;  // 128 and 16 that put 8 rows' 16-byte pieces into different banks
+struct __align__(16) LineStage {
+  unsigned char bytes[32 * kLineRowBytes];
+};
+
+// piece(q): this lane's 16 bytes q of 8. rows, bytes: what exists of the 32 rows and of the line.
+template <typename Piece>
+__device__ __forceinline__ void store_lines(LineStage* stage, int lane, unsigned char* d, int64_t row_bytes, int rows, int bytes, Piece piece) {
+  __syncwarp();  // the previous lines have been read out
+#pragma unroll
+  for (int q = 0; q < 8; ++q)
+    *reinterpret_cast<uint4*>(stage->bytes + lane * kLineRowBytes + q * 16) = piece(q);
+  __syncwarp();
+  const int at = (lane & 7) * 16;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = 4 * i + (lane >> 3);
+    const uint4 w = *reinterpret_cast<const uint4*>(stage->bytes + r * kLineRowBytes + at);
+    if (r < rows && at < bytes)
+      *reinterpret_cast<uint4*>(d + r * row_bytes + at) = w;
+  }
+}
+
+// ==================================================================================================== few tokens
+//
+// Rows of the tensor core's tile are features (the weight is operand A), columns tokens.
+
+namespace few {
+
+constexpr int kTileF = 128, kTileT = 128;
+constexpr int kPartT = kTileT / 2;  // columns per epilogue warp: two warps share a tensor memory quarter
+constexpr int kChunks = kPartT / 32;
+constexpr int kAccBuffers = kTmemCols / kTileT;
+constexpr uint32_t kStageRowBytes = 80;  // 32 bf16 and 16 bytes that put 8 rows' 16-byte pieces into different banks
+
+struct __align__(16) ScaleSlot {  // tokens' scales are read in pairs
+  float token[kTileT];
+  float weight;
+};
+
+struct Shared : Common<5> {
+  ScaleSlot scales[kScaleSlots];
+  __align__(16) unsigned char out[kEpilogueWarps][32 * kStageRowBytes];
+};
+
+constexpr size_t kSmemBytes = 1024 + Shared::kStages * static_cast<size_t>(kABytes + kBBytes) + sizeof(Shared);
+static_assert(kSmemBytes <= 232448, "shared memory of one CTA");
+static_assert(Shared::kStages * kABytes >= kMaxExperts * 4, "the operand stages hold the scan's copy of ends");
+
+template <int kMode>
+__device__ __forceinline__ void load_operands(const Params& p, const CUtensorMap* map_w, const CUtensorMap* map_t, Shared* s, uint32_t a0,
+                                              uint32_t b0, int units) {
+  const uint32_t el = elect_one() ? 1u : 0u;
+  const uint32_t empty0 = smem_u32(&s->empty[0]), full0 = smem_u32(&s->full[0]);
+  uint32_t stage = 0, phase = 0;
+  for (int u = blockIdx.x; u < units; u += gridDim.x) {
+    const Unit x = unit_at<kTileT, kTileF>(p, s, u);
+    const int boxes = (x.rows + 31) / 32;
+    for (int b = 0; b < x.blocks; ++b) {
+      if (!wait_bounded(empty0 + stage * 8, phase ^ 1u, &s->abort_flag, kSiteStageEmpty))
+        return;
+      const uint32_t full = full0 + stage * 8;
+      mbar_arrive_expect_tx(el, full, kABytes + boxes * kBBoxBytes);
+      tma_load_3d(el, a0 + stage * kABytes, map_w, full, kMode == kForward ? b * kBlock : x.f0, kMode == kForward ? x.f0 : b * kBlock, x.expert);
+      for (int i = 0; i < boxes; ++i)
+        tma_load_3d(el, b0 + stage * kBBytes + i * kBBoxBytes, map_t, full, b * kBlock, x.row0 + 32 * i, 0);
+      if (++stage == Shared::kStages)
+        stage = 0, phase ^= 1u;
+    }
+  }
+}
+
+// A block's scales by 4-byte copies: an expert's tokens start at any row.
+__device__ __forceinline__ void load_scales(const Params& p, Shared* s, int units, int lane) {
+  const uint32_t scale_full0 = smem_u32(&s->scale_full[0]), scale_empty0 = smem_u32(&s->scale_empty[0]);
+  uint32_t slot = 0, slot_phase = 0;
+  for (int u = blockIdx.x; u < units; u += gridDim.x) {
+    const Unit x = unit_at<kTileT, kTileF>(p, s, u);
+    for (int b = 0; b < x.blocks; ++b) {
+      if (!wait_bounded(scale_empty0 + slot * 8, slot_phase ^ 1u, &s->abort_flag, kSiteScaleEmpty))
+        return;
+      const float* token = p.token_scale + b * p.token_ld + x.row0;
+      for (int i = lane; i < x.rows; i += 32)
+        cp_async_4(smem_u32(&s->scales[slot].token[i]), token + i);
+      if (lane == 0)
+        cp_async_4(smem_u32(&s->scales[slot].weight), p.weight_scale + x.expert * p.w_scale_expert +
+                                                            (x.f0 >> 7) * static_cast<int64_t>(p.w_scale_f) + b * static_cast<int64_t>(p.w_scale_b));
+      cp_async_arrive(scale_full0 + slot * 8);
+      if (++slot == kScaleSlots)
+        slot = 0, slot_phase ^= 1u;
+    }
+  }
+}
+
+template <int kMode>
+__device__ __forceinline__ void issue_mmas(const Params& p, Shared* s, uint32_t a0, uint32_t b0, uint32_t tmem_base, int units) {
+  constexpr bool kAMn = kMode == kInputGrad;
+  // 128-byte swizzle, groups of 8 rows of 128 bytes 1024 apart. K-major: K = 32 is 32 bytes within a row; MN-major: 32 rows.
+  constexpr uint32_t kAStep = kAMn ? 4096 >> 4 : 32 >> 4, kBStep = 32 >> 4;
+  const uint32_t el = elect_one() ? 1u : 0u;
+  const uint32_t full0 = smem_u32(&s->full[0]);
+  const uint64_t a_desc0 = make_smem_desc(a0, 1024, 1024, 2), b_desc0 = make_smem_desc(b0, 1024, 1024, 2);
+  uint32_t stage = 0, phase = 0, buf = 0, buf_phase = 0;
+  for (int u = blockIdx.x; u < units; u += gridDim.x) {
+    const Unit x = unit_at<kTileT, kTileF>(p, s, u);
+    const uint32_t idesc = make_idesc_f8(kTileF, (x.rows + 15) / 16 * 16, kAMn, false);
+    for (int b = 0; b < x.blocks; ++b) {
+      if (!wait_bounded(smem_u32(&s->acc_empty[buf]), buf_phase ^ 1u, &s->abort_flag, kSiteAccEmpty) ||
+          !wait_bounded(full0 + stage * 8, phase, &s->abort_flag, kSiteStageFull))
+        return;
+      tcgen05_fence_after_sync();
+      const uint64_t a = a_desc0 + stage * (kABytes >> 4), bd = b_desc0 + stage * (kBBytes >> 4);
+#pragma unroll
+      for (uint32_t k = 0; k < 4; ++k)
+        tcgen05_mma_f8(el, tmem_base + buf * kTileT, a + k * kAStep, bd + k * kBStep, idesc, k > 0);
+      tcgen05_commit(el, &s->empty[stage]);
+      tcgen05_commit(el, &s->acc_full[buf]);
+      if (++stage == Shared::kStages)
+        stage = 0, phase ^= 1u;
+      if (++buf == kAccBuffers)
+        buf = 0, buf_phase ^= 1u;
+    }
+  }
+}
+
+// 32 tokens of this warp's 32 features to the output. v[j][i]: tokens 8 j + 2 (lane % 4), + 1, feature 8 i + lane / 4.
+__device__ __forceinline__ void store_chunk(const Params& p, const Unit& x, unsigned char* stage, int lane, int feature0, int t0,
+                                            const uint64_t (&v)[4][4]) {
+  const uint32_t st = smem_u32(stage);
+  __syncwarp();  // the previous chunk has been read out
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    uint32_t h[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = both(v[j][i]);
+      h[i] = pack_bf16x2_rn(f.x, f.y);
+    }
+    // a row of the stage: 32 features of one token
+    stmatrix_x4_trans(st + (8 * j + (lane & 7)) * kStageRowBytes + (lane >> 3) * 16, h[0], h[1], h[2], h[3]);
+  }
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = 8 * i + (lane >> 2), piece = lane & 3;
+    const uint4 w = *reinterpret_cast<const uint4*>(stage + r * kStageRowBytes + piece * 16);
+    if (t0 + r < x.rows && feature0 + piece * 8 < p.features)
+      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.d) + static_cast<int64_t>(x.row0 + t0 + r) * p.features + feature0 + piece * 8) = w;
+  }
+}
+
+__device__ __forceinline__ void accumulate(const Params& p, Shared* s, uint32_t tmem_base, int units, int warp, int lane) {
+  const int quarter = warp & 3, part0 = ((warp - kFirstEpilogueWarp) >> 2) * kPartT;  // a warp reads tensor memory lanes 32 (warp % 4) on
+  const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
+  unsigned char* stage = s->out[warp - kFirstEpilogueWarp];
+  uint32_t buf = 0, buf_phase = 0, slot = 0, slot_phase = 0;
+  for (int u = blockIdx.x; u < units; u += gridDim.x) {
+    const Unit x = unit_at<kTileT, kTileF>(p, s, u);
+    uint64_t acc[kChunks][4][4];
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          acc[c][j][i] = 0;
+    for (int b = 0; b < x.blocks; ++b) {
+      if (!wait_bounded(smem_u32(&s->scale_full[slot]), slot_phase, &s->abort_flag, kSiteScaleFull) ||
+          !wait_bounded(smem_u32(&s->acc_full[buf]), buf_phase, &s->abort_flag, kSiteAccFull))
+        return;
+      tcgen05_fence_after_sync();
+      const ScaleSlot& sc = s->scales[slot];
+      const uint64_t weight = pair_f32(sc.weight, sc.weight);
+      const uint32_t t = tmem_base + lane_base + buf * kTileT + part0;
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c) {
+        if (part0 + 32 * c >= x.rows)
+          break;
+        uint32_t lo[16], hi[16];
+        tmem_ld_16x256b_x4(t + 32 * c, lo);
+        tmem_ld_16x256b_x4(t + 32 * c + (16u << 16), hi);
+        uint64_t scale[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 f = *reinterpret_cast<const float2*>(&sc.token[part0 + 32 * c + 8 * j + 2 * (lane & 3)]);
+          scale[j] = mul_f32x2(pair_f32(f.x, f.y), weight);
+        }
+        tmem_ld_wait();
+#pragma unroll
+        for (int k = 0; k < 16; ++k)
+          asm volatile("" : "+r"(lo[k]), "+r"(hi[k]));
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint64_t v = i < 2 ? pair_u32(lo[4 * j + 2 * i], lo[4 * j + 2 * i + 1])
+                                     : pair_u32(hi[4 * j + 2 * i - 4], hi[4 * j + 2 * i - 3]);
+            acc[c][j][i] = fma_f32x2(v, scale[j], acc[c][j][i]);
+          }
+      }
+      tcgen05_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&s->acc_empty[buf]);
+        mbar_arrive(&s->scale_empty[slot]);
+      }
+      if (++buf == kAccBuffers)
+        buf = 0, buf_phase ^= 1u;
+      if (++slot == kScaleSlots)
+        slot = 0, slot_phase ^= 1u;
+    }
+    const int feature0 = x.f0 + quarter * 32;
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c)
+      if (part0 + 32 * c < x.rows && feature0 < p.features)
+        store_chunk(p, x, stage, lane, feature0, part0 + 32 * c, acc[c]);
+  }
+}
+
+template <int kMode>
+__device__ __forceinline__ void body(const Params& p, const CUtensorMap* map_w, const CUtensorMap* map_t) {
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* base = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  const uint32_t a0 = smem_u32(base), b0 = a0 + Shared::kStages * kABytes;
+  Shared* s = reinterpret_cast<Shared*>(base + Shared::kStages * (kABytes + kBBytes));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t tmem_base = set_up<1>(p, map_w, map_t, s, base, warp, kAccBuffers, 32, kTileT, true);
+  const int units = units_of(p, s, kTileF);
+  if (warp == 0)
+    load_operands<kMode>(p, map_w, map_t, s, a0, b0, units);
+  else if (warp == 1)
+    issue_mmas<kMode>(p, s, a0, b0, tmem_base, units);
+  else if (warp == 2)
+    load_scales(p, s, units, lane);
+  else if (warp >= kFirstEpilogueWarp)
+    accumulate(p, s, tmem_base, units, warp, lane);
+  tear_down<1>(s, tmem_base, warp);
+}
+
+}  // namespace few
+
+// ==================================================================================================== many tokens
+//
+// Rows of the tensor core's tile are tokens (operand A, 128 per CTA), columns features: each CTA brings its tokens and half of
+// the features' rows of the weight.
+
+namespace many {
+
+constexpr int kTileT = 256, kTileF = 256;
+constexpr int kAccBuffers = kTmemCols / kTileF;
+constexpr int kChunks = 4;  // of 32 features: an epilogue warp has 32 tokens and the 128 features of one weight block
+
+struct __align__(16) ScaleSlot {
+  float token[128];
+  float weight[2];
+};
+
+struct Shared : Common<5> {
+  ScaleSlot scales[kScaleSlots];
+  LineStage out[kEpilogueWarps];
+};
+
+constexpr size_t kSmemBytes = 1024 + Shared::kStages * static_cast<size_t>(kABytes + kBBytes) + sizeof(Shared);
+static_assert(kSmemBytes <= 232448, "shared memory of one CTA");
+
+template <int kMode>
+__device__ __forceinline__ void load_operands(const Params& p, const CUtensorMap* map_t, const CUtensorMap* map_w, Shared* s, uint32_t a0,
+                                              uint32_t b0, int rank, int first, int step, int units) {
+  const uint32_t el = elect_one() ? 1u : 0u, el_leader = rank == 0 ? el : 0u;
+  const uint32_t empty0 = smem_u32(&s->empty[0]), full0 = smem_u32(&s->full[0]);
+  const uint32_t full_leader0 = map_to_cta(full0, 0);
+  uint32_t stage = 0, phase = 0;
+  for (int u = first; u < units; u += step) {
+    const Unit x = unit_at<kTileT, kTileF>(p, s, u);
+    const int row = x.row0 + rank * 128, feature = x.f0 + rank * 128;
+    for (int b = 0; b < x.blocks; ++b) {
+      if (!wait_bounded(empty0 + stage * 8, phase ^ 1u, &s->abort_flag, kSiteStageEmpty))
+        return;
+      mbar_arrive_expect_tx(el_leader, full0 + stage * 8, 2 * (kABytes + kBBytes));
+      const uint32_t full = full_leader0 + stage * 8;
+      const int k = b * kBlock;
+      tma_load_3d_pair(el, a0 + stage * kABytes, map_t, full, k, row, 0);
+      tma_load_3d_pair(el, b0 + stage * kBBytes, map_w, full, kMode == kForward ? k : feature, kMode == kForward ? feature : k, x.expert);
+      if (++stage == Shared::kStages)
+        stage = 0, phase ^= 1u;
+    }
+  }
+}
+
+__device__ __forceinline__ void load_scales(const Params& p, Shared* s, int rank, int first, int step, int units, int lane) {
+  const uint32_t scale_full0 = smem_u32(&s->scale_full[0]), scale_empty0 = smem_u32(&s->scale_empty[0]);
+  uint32_t slot = 0, slot_phase = 0;
+  const int weight_tiles = (p.features + kBlock - 1) / kBlock;
+  for (int u = first; u < units; u += step) {
+    const Unit x = unit_at<kTileT, kTileF>(p, s, u);
+    const int row = rank * 128;
+    for (int b = 0; b < x.blocks; ++b) {
+      if (!wait_bounded(scale_empty0 + slot * 8, slot_phase ^ 1u, &s->abort_flag, kSiteScaleEmpty))
+        return;
+      const float* token = p.token_scale + b * p.token_ld + x.row0 + row;
+#pragma unroll
+      for (int i = lane; i < 128; i += 32)
+        if (row + i < x.rows)
+          cp_async_4(smem_u32(&s->scales[slot].token[i]), token + i);
+      if (lane < 2 && (x.f0 >> 7) + lane < weight_tiles)
+        cp_async_4(smem_u32(&s->scales[slot].weight[lane]),
+                   p.weight_scale + x.expert * p.w_scale_expert + ((x.f0 >> 7) + lane) * static_cast<int64_t>(p.w_scale_f) +
+                         b * static_cast<int64_t>(p.w_scale_b));
+      cp_async_arrive(scale_full0 + slot * 8);
+      if (++slot == kScaleSlots)
+        slot = 0, slot_phase ^= 1u;
+    }
+  }
+}
+
+template <int kMode>
+__device__ __forceinline__ void issue_mmas(const Params& p, Shared* s, uint32_t a0, uint32_t b0, uint32_t tmem_base, int first, int step,
+                                           int units) {
+  constexpr bool kBMn = kMode == kInputGrad;
+  constexpr uint32_t kAStep = 32 >> 4, kBStep = kBMn ? 4096 >> 4 : 32 >> 4;
+  constexpr uint32_t idesc = make_idesc_f8(kTileT, kTileF, false, kBMn);
+  const uint32_t el = elect_one() ? 1u : 0u;
+  const uint32_t full0 = smem_u32(&s->full[0]), empty0 = smem_u32(&s->empty[0]);
+  const uint64_t a_desc0 = make_smem_desc(a0, 1024, 1024, 2), b_desc0 = make_smem_desc(b0, 1024, 1024, 2);
+  uint32_t stage = 0, phase = 0, buf = 0, buf_phase = 0;
+  for (int u = first; u < units; u += step) {
+    const int blocks = unit_at<kTileT, kTileF>(p, s, u).blocks;
+    for (int b = 0; b < blocks; ++b) {
+      if (!wait_bounded(smem_u32(&s->acc_empty[buf]), buf_phase ^ 1u, &s->abort_flag, kSiteAccEmpty) ||
+          !wait_bounded(full0 + stage * 8, phase, &s->abort_flag, kSiteStageFull))
+        return;
+      tcgen05_fence_after_sync();
+      const uint64_t a = a_desc0 + stage * (kABytes >> 4), bd = b_desc0 + stage * (kBBytes >> 4);
+#pragma unroll
+      for (uint32_t k = 0; k < 4; ++k)
+        tcgen05_mma_f8_pair(el, tmem_base + buf * kTileF, a + k * kAStep, bd + k * kBStep, idesc, k > 0);
+      tcgen05_commit_pair(el, empty0 + stage * 8, 3);
+      tcgen05_commit_pair(el, &s->acc_full[buf], 3);
+      if (++stage == Shared::kStages)
+        stage = 0, phase ^= 1u;
+      if (++buf == kAccBuffers)
+        buf = 0, buf_phase ^= 1u;
+    }
+  }
+}
+
+__device__ __forceinline__ void accumulate(const Params& p, Shared* s, uint32_t tmem_base, int rank, int first, int step, int units, int warp,
+                                           int lane) {
+  const int quarter = warp & 3, part = (warp - kFirstEpilogueWarp) >> 2;
+  const uint32_t t0 = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + part * 128;
+  const uint32_t acc_empty0 = map_to_cta(smem_u32(&s->acc_empty[0]), 0);
+  uint32_t buf = 0, buf_phase = 0, slot = 0, slot_phase = 0;
+  for (int u = first; u < units; u += step) {
+    const Unit x = unit_at<kTileT, kTileF>(p, s, u);
+    uint64_t acc[kChunks][16];
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        acc[c][j] = 0;
+    for (int b = 0; b < x.blocks; ++b) {
+      if (!wait_bounded(smem_u32(&s->scale_full[slot]), slot_phase, &s->abort_flag, kSiteScaleFull))
+        return;
+      const float f = s->scales[slot].token[quarter * 32 + lane] * s->scales[slot].weight[part];
+      const uint64_t scale = pair_f32(f, f);
+      if (!wait_bounded(smem_u32(&s->acc_full[buf]), buf_phase, &s->abort_flag, kSiteAccFull))
+        return;
+      tcgen05_fence_after_sync();
+      const uint32_t t = t0 + buf * kTileF;
+      uint32_t v[2][32];
+      tmem_ld_32x32b_x32(t, v[0]);
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c) {
+        tmem_ld_wait(v[c & 1]);
+        if (c + 1 < kChunks)
+          tmem_ld_32x32b_x32(t + 32 * (c + 1), v[(c + 1) & 1]);
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          acc[c][j] = fma_f32x2(pair_u32(v[c & 1][2 * j], v[c & 1][2 * j + 1]), scale, acc[c][j]);
+      }
+      tcgen05_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive_cluster(acc_empty0 + buf * 8);
+        mbar_arrive(&s->scale_empty[slot]);
+      }
+      if (++buf == kAccBuffers)
+        buf = 0, buf_phase ^= 1u;
+      if (++slot == kScaleSlots)
+        slot = 0, slot_phase ^= 1u;
+    }
+    const int row = rank * 128 + quarter * 32, feature = x.f0 + part * 128;
+    unsigned char* d = static_cast<unsigned char*>(p.d) + (static_cast<int64_t>(x.row0 + row) * p.features + feature) * 2;
+#pragma unroll
+    for (int c = 0; c < kChunks; c += 2)
+      store_lines(&s->out[warp - kFirstEpilogueWarp], lane, d + 64 * c, static_cast<int64_t>(p.features) * 2, x.rows - row,
+                  (p.features - feature - 32 * c) * 2, [&](int q) {
+                    uint32_t h[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                      const float2 o = both(acc[c + (q >> 2)][4 * (q & 3) + j]);
+                      h[j] = pack_bf16x2_rn(o.x, o.y);
+                    }
+                    return make_uint4(h[0], h[1], h[2], h[3]);
+                  });
+  }
+}
+
+template <int kMode>
+__device__ __forceinline__ void body(const Params& p, const CUtensorMap* map_t, const CUtensorMap* map_w) {
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* base = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  const uint32_t a0 = smem_u32(base), b0 = a0 + Shared::kStages * kABytes;
+  Shared* s = reinterpret_cast<Shared*>(base + Shared::kStages * (kABytes + kBBytes));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = static_cast<int>(cluster_ctarank());
+  const uint32_t tmem_base = set_up<2>(p, map_t, map_w, s, base, warp, kAccBuffers, 32, kTileT, true);
+  const int units = units_of(p, s, kTileF), first = blockIdx.x / 2, step = gridDim.x / 2;
+  if (warp < kFirstEpilogueWarp) {
+    set_max_registers_down<kFewRegisters>();
+    if (warp == 0)
+      load_operands<kMode>(p, map_t, map_w, s, a0, b0, rank, first, step, units);
+    else if (warp == 1 && rank == 0)
+      issue_mmas<kMode>(p, s, a0, b0, tmem_base, first, step, units);
+    else if (warp == 2)
+      load_scales(p, s, rank, first, step, units, lane);
+  } else {
+    set_max_registers_up<kManyRegisters>();
+    accumulate(p, s, tmem_base, rank, first, step, units, warp, lane);
+  }
+  tear_down<2>(s, tmem_base, warp);
+}
+
+}  // namespace many
+
+// ==================================================================================================== weight gradient
+//
+// A CTA pair, 256 x 256 of one expert's dw: operand A gradients (128 of their columns per CTA), B inputs, both MN-major, with
+// scale tiles (512 bytes: a word for each of 128 columns, the E8M0 byte four times, in the order of the copy to tensor
+// memory) through shared into tensor memory. Two
+// accumulator buffers share 32 columns, so that the scales find room beside them: [0, 256), [224, 480), scales at [480, 492);
+// the epilogue drains the shared columns first.
+
+namespace wgrad {
+
+constexpr int kTile = 256;
+constexpr uint32_t kScaleTile = 512, kScaleBytes = 3 * kScaleTile;
+constexpr uint32_t kAcc1 = 224;  // the second accumulator buffer; the first is at 0
+constexpr uint32_t kScaleA = 480, kScaleB = 484;
+
+struct Shared : Common<5> {
+  LineStage out[kEpilogueWarps];
+};
+
+constexpr size_t kStageBytes = kABytes + kBBytes + kScaleBytes;
+constexpr size_t kSmemBytes = 1024 + Shared::kStages * kStageBytes + sizeof(Shared);
+static_assert(kSmemBytes <= 232448, "shared memory of one CTA");
+
+struct Unit {
+  int expert, m0, n0, block0, blocks;
+};
+
+__device__ __forceinline__ Unit unit_at(const Params& p, const Shared* s, int u) {
+  const int mt = (p.features + kTile - 1) / kTile, nt = (p.n + kTile - 1) / kTile;
+  Unit x;
+  x.expert = u / (mt * nt);
+  int v = u - x.expert * mt * nt;
+  const int panel = v / (kPanel * nt);
+  v -= panel * kPanel * nt;
+  const int width = min(kPanel, mt - panel * kPanel);
+  x.n0 = v / width * kTile;
+  x.m0 = (panel * kPanel + v % width) * kTile;
+  x.block0 = s->first_tile[x.expert];
+  x.blocks = s->first_tile[x.expert + 1] - x.block0;
+  return x;
+}
+
+__device__ __forceinline__ void load_operands(const Params& p, const Maps& maps, Shared* s, uint32_t a0, int rank, int first, int step, int units) {
+  const uint32_t el = elect_one() ? 1u : 0u, el_leader = rank == 0 ? el : 0u;
+  const uint32_t empty0 = smem_u32(&s->empty[0]), full0 = smem_u32(&s->full[0]);
+  const uint32_t full_leader0 = map_to_cta(full0, 0);
+  const uint32_t b0 = a0 + Shared::kStages * kABytes, sf0 = b0 + Shared::kStages * kBBytes;
+  uint32_t stage = 0, phase = 0;
+  for (int u = first; u < units; u += step) {
+    const Unit x = unit_at(p, s, u);
+    for (int b = 0; b < x.blocks; ++b) {
+      if (!wait_bounded(empty0 + stage * 8, phase ^ 1u, &s->abort_flag, kSiteStageEmpty))
+        return;
+      mbar_arrive_expect_tx(el_leader, full0 + stage * 8, 2 * kStageBytes);
+      const uint32_t full = full_leader0 + stage * 8, sf = sf0 + stage * kScaleBytes;
+      const int block = x.block0 + b;
+      tma_load_3d_pair(el, a0 + stage * kABytes, &maps.a, full, x.m0 + rank * 128, block * kBlock, 0);
+      tma_load_3d_pair(el, b0 + stage * kBBytes, &maps.b, full, x.n0 + rank * 128, block * kBlock, 0);
+      tma_load_3d_pair(el, sf, &maps.a_scale, full, 0, (x.m0 >> 7) + rank, block);
+      tma_load_3d_pair(el, sf + kScaleTile, &maps.b_scale, full, 0, x.n0 >> 7, block);
+      if (++stage == Shared::kStages)
+        stage = 0, phase ^= 1u;
+    }
+  }
+}
+
+__device__ __forceinline__ void issue_mmas(const Params& p, Shared* s, uint32_t a0, uint32_t tmem_base, int first, int step, int units) {
+  constexpr uint32_t idesc = make_idesc_mxf8(kTile, kTile) | kIdescAMn | kIdescBMn;
+  const uint32_t el = elect_one() ? 1u : 0u;
+  const uint32_t full0 = smem_u32(&s->full[0]), empty0 = smem_u32(&s->empty[0]);
+  const uint32_t b0 = a0 + Shared::kStages * kABytes, sf0 = b0 + Shared::kStages * kBBytes;
+  const uint64_t a_desc0 = make_smem_desc(a0, 1024, 1024, 2), b_desc0 = make_smem_desc(b0, 1024, 1024, 2);
+  const uint64_t sf_desc0 = make_smem_desc(sf0, 0, 128, 0);
+  const uint32_t sfa = tmem_base + kScaleA, sfb = tmem_base + kScaleB;
+  uint32_t stage = 0, phase = 0, local = 0;
+  for (int u = first; u < units; u += step) {
+    const int blocks = unit_at(p, s, u).blocks;
+    if (blocks == 0)
+      continue;
+    const uint32_t buf = local & 1u;
+    if (!wait_bounded(smem_u32(&s->acc_empty[buf]), ((local >> 1) & 1u) ^ 1u, &s->abort_flag, kSiteAccEmpty) ||
+        (local > 0 && !wait_bounded(smem_u32(&s->overlap_free), (local - 1) & 1u, &s->abort_flag, kSiteOverlap)))
+      return;
+    ++local;
+    for (int b = 0; b < blocks; ++b) {
+      if (!wait_bounded(full0 + stage * 8, phase, &s->abort_flag, kSiteStageFull))
+        return;
+      tcgen05_fence_after_sync();
+      const uint64_t sf = sf_desc0 + stage * (kScaleBytes >> 4);
+      tcgen05_cp_32x128b_warpx4_pair(el, sfa, sf);
+      tcgen05_cp_32x128b_warpx4_pair(el, sfb, sf + (kScaleTile >> 4));
+      tcgen05_cp_32x128b_warpx4_pair(el, sfb + 4, sf + 2 * (kScaleTile >> 4));
+      const uint64_t a = a_desc0 + stage * (kABytes >> 4), bd = b_desc0 + stage * (kBBytes >> 4);
+#pragma unroll
+      for (uint32_t k = 0; k < 4; ++k)  // K = 32: 32 rows of 128 bytes
+        tcgen05_mma_mxf8_pair(el, tmem_base + buf * kAcc1, a + k * (4096 >> 4), bd + k * (4096 >> 4), idesc, sfa, sfb, b > 0 || k > 0);
+      tcgen05_commit_pair(el, empty0 + stage * 8, 3);
+      if (++stage == Shared::kStages)
+        stage = 0, phase ^= 1u;
+    }
+    tcgen05_commit_pair(el, &s->acc_full[buf], 3);
+  }
+}
+
+__device__ __forceinline__ void store(const Params& p, Shared* s, uint32_t tmem_base, int rank, int first, int step, int units, int warp, int lane) {
+  const int quarter = warp & 3, part = (warp - kFirstEpilogueWarp) >> 2;
+  const uint32_t t0 = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
+  const uint32_t acc_empty0 = map_to_cta(smem_u32(&s->acc_empty[0]), 0), overlap_free = map_to_cta(smem_u32(&s->overlap_free), 0);
+  uint32_t local = 0;
+  for (int u = first; u < units; u += step) {
+    const Unit x = unit_at(p, s, u);
+    const uint32_t buf = local & 1u;
+    if (x.blocks > 0) {
+      if (!wait_bounded(smem_u32(&s->acc_full[buf]), (local >> 1) & 1u, &s->abort_flag, kSiteAccFull))
+        return;
+      tcgen05_fence_after_sync();
+      ++local;
+    }
+    const int row = x.m0 + rank * 128 + quarter * 32;
+    const int64_t at = (static_cast<int64_t>(x.expert) * p.features + row) * p.n + x.n0;
+    const int value = p.out_bf16 ? 2 : 4;
+    unsigned char* d = static_cast<unsigned char*>(p.d) + at * value;
+    LineStage* stage = &s->out[warp - kFirstEpilogueWarp];
+    uint32_t half[16];  // bf16: the first 32 columns of a line
+#pragma unroll 1
+    for (int i = 0; i < 4; ++i) {
+      // the columns that the buffers share, [224, 256), first: the last chunk of part 1 in buffer 0, the first of part 0 in 1.
+      // A line of bf16 is two chunks: 3, 2, then 1, 0; or 0, 1, then 2, 3.
+      const int c = (buf == 0 ? 3 - i : i) + 4 * part;
+      uint32_t v[32];
+      if (x.blocks > 0) {
+        tmem_ld_32x32b_x32(t0 + buf * kAcc1 + 32 * c, v);
+        tmem_ld_wait(v);
+        if (i == 0 && part == static_cast<int>(1 - buf)) {
+          tcgen05_fence_before_sync();
+          __syncwarp();
+          if (lane == 0)
+            mbar_arrive_cluster(overlap_free);
+        }
+        if (i == 3) {
+          tcgen05_fence_before_sync();
+          __syncwarp();
+          if (lane == 0)
+            mbar_arrive_cluster(acc_empty0 + buf * 8);
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < 32; ++k)
+          v[k] = 0;
+      }
+      if (!p.out_bf16) {
+        store_lines(stage, lane, d + 128 * c, static_cast<int64_t>(p.n) * 4, p.features - row, (p.n - x.n0 - 32 * c) * 4,
+                    [&](int q) { return make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]); });
+        continue;
+      }
+      uint32_t h[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        h[j] = pack_bf16x2_rn(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
+      if ((i & 1) == 0) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          half[j] = h[j];
+      } else {
+        const bool swapped = buf == 0;
+        store_lines(stage, lane, d + 64 * (c & ~1), static_cast<int64_t>(p.n) * 2, p.features - row, (p.n - x.n0 - 32 * (c & ~1)) * 2,
+                    [&](int q) {
+                      const int k = 4 * (q & 3);
+                      const bool from_half = (q < 4) != swapped;
+                      return make_uint4(from_half ? half[k] : h[k], from_half ? half[k + 1] : h[k + 1],
+                                        from_half ? half[k + 2] : h[k + 2], from_half ? half[k + 3] : h[k + 3]);
+                    });
+      }
+    }
+  }
+}
+
+__device__ __forceinline__ void body(const Params& p, const Maps& maps) {
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* base = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  const uint32_t a0 = smem_u32(base);
+  Shared* s = reinterpret_cast<Shared*>(base + Shared::kStages * kStageBytes);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = static_cast<int>(cluster_ctarank());
+  const uint32_t tmem_base = set_up<2>(p, &maps.a, &maps.b, s, base, warp, 2, 1, kBlock, false);
+  const int units = p.experts * ((p.features + kTile - 1) / kTile) * ((p.n + kTile - 1) / kTile);
+  const int first = blockIdx.x / 2, step = gridDim.x / 2;
+  if (warp == 0)
+    load_operands(p, maps, s, a0, rank, first, step, units);
+  else if (warp == 1 && rank == 0)
+    issue_mmas(p, s, a0, tmem_base, first, step, units);
+  else if (warp >= kFirstEpilogueWarp)
+    store(p, s, tmem_base, rank, first, step, units, warp, lane);
+  tear_down<2>(s, tmem_base, warp);
+}
+
+}  // namespace wgrad
+
 struct Launch {
-  CUtensorMap a, b;
+  Maps maps;
   Params p;
 };
 
 }  // namespace
 }  // namespace mxb200
 
-#define MXB200_BLOCK_KERNEL(name, mode)                                                                                     \
-  __global__ void __launch_bounds__(mxb200::kThreads, 1) name(const __grid_constant__ mxb200::Launch args) {                \
-    mxb200::block_gemm_body<mode, 1>(args.p, &args.a, &args.b);                                                             \
-  }
-MXB200_BLOCK_KERNEL(mxb200_block_gemm_forward_128x128, mxb200::kForward)
-MXB200_BLOCK_KERNEL(mxb200_block_gemm_input_grad_128x128, mxb200::kInputGrad)
-MXB200_BLOCK_KERNEL(mxb200_block_gemm_weight_grad_128x128, mxb200::kWeightGrad)
+__global__ void __launch_bounds__(mxb200::kThreads, 1) mxb200_block_gemm_forward_few(const __grid_constant__ mxb200::Launch args) {
+  mxb200::few::body<mxb200::kForward>(args.p, &args.maps.a, &args.maps.b);
+}
+__global__ void __launch_bounds__(mxb200::kThreads, 1) mxb200_block_gemm_input_grad_few(const __grid_constant__ mxb200::Launch args) {
+  mxb200::few::body<mxb200::kInputGrad>(args.p, &args.maps.a, &args.maps.b);
+}
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(mxb200::kThreads, 1)
+      mxb200_block_gemm_forward_many(const __grid_constant__ mxb200::Launch args) {
+  mxb200::many::body<mxb200::kForward>(args.p, &args.maps.a, &args.maps.b);
+}
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(mxb200::kThreads, 1)
+      mxb200_block_gemm_input_grad_many(const __grid_constant__ mxb200::Launch args) {
+  mxb200::many::body<mxb200::kInputGrad>(args.p, &args.maps.a, &args.maps.b);
+}
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(mxb200::kThreads, 1)
+      mxb200_block_gemm_weight_grad(const __grid_constant__ mxb200::Launch args) {
+  mxb200::wgrad::body(args.p, args.maps);
+}
 
 namespace mxb200 {
 namespace {
@@ -581,7 +944,80 @@ int64_t up(int64_t n, int64_t d) {
   return (n + d - 1) / d;
 }
 
+// Scale tiles of (tokens, columns): 128 words for each block of tokens and each 128 columns, `tiles` of a block's at a time.
+int make_scale_map(CUtensorMap* map, const void* base, int64_t columns, int64_t tokens, int tiles) {
+  EncodeTiledFn fn = encode_fn();
+  if (fn == nullptr)
+    return MXB200_ERR_DRIVER;
+  const cuuint64_t n = static_cast<cuuint64_t>(up(columns, kBlock));
+  const cuuint64_t dims[3] = {kBlock, n, static_cast<cuuint64_t>(tokens / kBlock)};
+  const cuuint64_t strides[2] = {kBlock * 4, n * kBlock * 4};
+  const cuuint32_t box[3] = {kBlock, static_cast<cuuint32_t>(tiles), 1};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, const_cast<void*>(base), dims, strides, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? MXB200_OK : MXB200_ERR_DRIVER;
+}
+
 using Kernel = void (*)(Launch);
+
+struct Variant {
+  Kernel kernel;
+  size_t smem;
+  int ctas;             // per unit
+  int tokens, features; // of a unit
+};
+
+constexpr int kFew = 0, kMany = 1;
+
+const Variant& variant(int kind, int many) {
+  static const Variant variants[5] = {
+        {mxb200_block_gemm_forward_few, few::kSmemBytes, 1, few::kTileT, few::kTileF},
+        {mxb200_block_gemm_forward_many, many::kSmemBytes, 2, many::kTileT, many::kTileF},
+        {mxb200_block_gemm_input_grad_few, few::kSmemBytes, 1, few::kTileT, few::kTileF},
+        {mxb200_block_gemm_input_grad_many, many::kSmemBytes, 2, many::kTileT, many::kTileF},
+        {mxb200_block_gemm_weight_grad, wgrad::kSmemBytes, 2, 0, wgrad::kTile}};
+  return variants[kind == MXB200_BLOCK_WEIGHT_GRAD ? 4 : 2 * kind + many];
+}
+
+// Which of the two kernels a product of `blocks` contraction blocks to `features` features takes: the one that is expected to be
+// done first. Both take about 0.45 us for a block of their tile when all SMs are at work, a unit's output costs as much as 3 or 4
+// blocks, and a pair's tile is twice the work per SM of the other's. 16384 x 6144 -> 1536: few tokens 235 us, many 134; 2500 x
+// 1280 -> 3840: 27 and 20; 1111 x 1040 -> 2000: 7.6 and 8.8; 8192 rows over 32 experts, 1536 -> 2048: 59 and 42; 1000 rows over
+// 64: 39 and 54. How the rows spread over experts is not known here: every expert is taken to have some, with half a tile left
+// over.
+bool many_tokens(int64_t tokens, int experts, int features, int blocks, int sms) {
+  const auto time = [&](const Variant& v, double out_blocks, double start) {
+    const int64_t used = std::min<int64_t>(experts, tokens);
+    const int64_t tiles = experts == 1 ? up(tokens, v.tokens) : std::max(used, tokens / v.tokens + used / 2);
+    return start + static_cast<double>(up(tiles * up(features, v.features), sms / v.ctas)) * (blocks + out_blocks) * 0.45;
+  };
+  return time(variant(MXB200_BLOCK_FORWARD, kMany), 4, 4.5) < time(variant(MXB200_BLOCK_FORWARD, kFew), 3, 4);
+}
+
+int set_smem_once(const Variant& v, int device) {
+  static std::mutex mu;
+  static const void* configured[64][5] = {};
+  std::lock_guard<std::mutex> lock(mu);
+  const void* const kernel = reinterpret_cast<const void*>(v.kernel);
+  for (int i = 0; i < 5 && device < 64; ++i) {
+    if (configured[device][i] == kernel)
+      return MXB200_OK;
+    if (configured[device][i] == nullptr)
+      break;
+  }
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(v.smem)) != cudaSuccess) {
+    cudaGetLastError();
+    return MXB200_ERR_LAUNCH;
+  }
+  for (int i = 0; i < 5 && device < 64; ++i)
+    if (configured[device][i] == nullptr) {
+      configured[device][i] = kernel;
+      break;
+    }
+  return MXB200_OK;
+}
 
 int block_gemm(const mxb200_block_gemm_args& g, cudaStream_t stream) {
   if (g.kind < MXB200_BLOCK_FORWARD || g.kind > MXB200_BLOCK_WEIGHT_GRAD ||
@@ -607,65 +1043,50 @@ int block_gemm(const mxb200_block_gemm_args& g, cudaStream_t stream) {
   }
   if (g.a == nullptr || g.a_scale == nullptr || g.b == nullptr || g.b_scale == nullptr || g.d == nullptr)
     return MXB200_ERR_NULL;
-  if (!aligned16(g.a) || !aligned16(g.b) || !aligned16(g.d) ||
-      ((reinterpret_cast<uintptr_t>(g.a_scale) | reinterpret_cast<uintptr_t>(g.b_scale) | reinterpret_cast<uintptr_t>(g.ends)) & 3) != 0)
+  const auto bits = [](const void* q) { return reinterpret_cast<uintptr_t>(q); };
+  if (!aligned16(g.a) || !aligned16(g.b) || !aligned16(g.d) || (bits(g.ends) & 3) != 0 ||
+      ((bits(g.a_scale) | bits(g.b_scale)) & (wgrad ? 15 : 3)) != 0)
     return MXB200_ERR_ALIGNMENT;
   const int64_t in = g.in_features, out = g.out_features;
-  const int64_t capacity = mxb200_block_token_blocks(g.tokens, g.experts) * kBlock;
-  Launch l;
+  Launch l{};
   Params& p = l.p;
-  p.col_scale = g.b_scale, p.row_scale = g.a_scale;
   p.d = g.d, p.ends = g.ends, p.experts = g.experts, p.rows = static_cast<int>(g.tokens);
   p.out_bf16 = g.out_kind == MXB200_OUT_BF16;
-  p.w_scale_expert = up(out, kBlock) * up(in, kBlock);
-  p.row_ld = 0, p.blocks = 0, p.n = 0;
+  const int from = static_cast<int>(g.kind == MXB200_BLOCK_FORWARD ? in : out), to = static_cast<int>(g.kind == MXB200_BLOCK_FORWARD ? out : in);
+  const bool many = !wgrad && many_tokens(g.tokens, g.experts, to, static_cast<int>(up(from, kBlock)), dev.sms);
+  const Variant& v = variant(g.kind, many ? kMany : kFew);
+  int64_t units;
   int st;
-  switch (g.kind) {
-    case MXB200_BLOCK_FORWARD:
-      p.m = static_cast<int>(out), p.blocks = static_cast<int>(up(in, kBlock)), p.col_ld = g.tokens;
-      p.w_scale_m = static_cast<int>(up(in, kBlock)), p.w_scale_b = 1;
-      st = make_map(&l.a, g.a, in, out, g.experts, 128);
-      st = st != MXB200_OK ? st : make_map(&l.b, g.b, in, g.tokens, 1, 32);
-      break;
-    case MXB200_BLOCK_INPUT_GRAD:
-      p.m = static_cast<int>(in), p.blocks = static_cast<int>(up(out, kBlock)), p.col_ld = g.tokens;
-      p.w_scale_m = 1, p.w_scale_b = static_cast<int>(up(in, kBlock));
-      st = make_map(&l.a, g.a, in, out, g.experts, 128);
-      st = st != MXB200_OK ? st : make_map(&l.b, g.b, out, g.tokens, 1, 32);
-      break;
-    default:
-      p.m = static_cast<int>(out), p.n = static_cast<int>(in), p.col_ld = in, p.row_ld = out;
-      p.w_scale_m = p.w_scale_b = 0;
-      st = make_map(&l.a, g.a, out, capacity, 1, 128);
-      st = st != MXB200_OK ? st : make_map(&l.b, g.b, in, capacity, 1, 32);
+  if (wgrad) {
+    const int64_t capacity = mxb200_block_token_blocks(g.tokens, g.experts) * kBlock;
+    p.features = static_cast<int>(out), p.n = static_cast<int>(in);
+    units = g.experts * up(out, v.features) * up(in, v.features);
+    st = make_map(&l.maps.a, g.a, out, capacity, 1, 128);
+    st = st != MXB200_OK ? st : make_map(&l.maps.b, g.b, in, capacity, 1, 128);
+    st = st != MXB200_OK ? st : make_scale_map(&l.maps.a_scale, g.a_scale, out, capacity, 1);
+    st = st != MXB200_OK ? st : make_scale_map(&l.maps.b_scale, g.b_scale, in, capacity, 2);
+  } else {
+    const bool forward = g.kind == MXB200_BLOCK_FORWARD;
+    p.weight_scale = static_cast<const float*>(g.a_scale), p.token_scale = static_cast<const float*>(g.b_scale);
+    p.token_ld = g.tokens, p.features = to, p.blocks = static_cast<int>(up(from, kBlock));
+    p.w_scale_expert = up(out, kBlock) * up(in, kBlock);
+    p.w_scale_f = forward ? static_cast<int>(up(in, kBlock)) : 1, p.w_scale_b = forward ? 1 : static_cast<int>(up(in, kBlock));
+    // token tiles are known on the device only; this many at most
+    const int64_t token_tiles = g.ends == nullptr ? up(g.tokens, v.tokens)
+                                                  : (g.tokens + (v.tokens - 1) * std::min<int64_t>(g.experts + 1, g.tokens)) / v.tokens;
+    units = token_tiles * up(to, v.features);
+    CUtensorMap *weight = many ? &l.maps.b : &l.maps.a, *token = many ? &l.maps.a : &l.maps.b;
+    st = make_map(weight, g.a, in, out, g.experts, 128);
+    st = st != MXB200_OK ? st : make_map(token, g.b, from, g.tokens, 1, many ? 128 : 32);
   }
   if (st != MXB200_OK)
     return st;
-  const int ctas = 1;
-  const int64_t tile = 128 * ctas;
-  // token tiles are known on the device only; this many at most
-  const int64_t token_tiles = g.ends == nullptr ? up(g.tokens, tile) : (g.tokens + (tile - 1) * std::min<int64_t>(g.experts + 1, g.tokens)) / tile;
-  const int64_t units = up(p.m, tile) * (wgrad ? g.experts * up(p.n, tile) : token_tiles);
   if (units > kMost)
     return MXB200_ERR_SHAPE;
-  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(units, dev.sms / ctas)) * ctas;
-  static const Kernel kernels[3] = {mxb200_block_gemm_forward_128x128, mxb200_block_gemm_input_grad_128x128,
-                                    mxb200_block_gemm_weight_grad_128x128};
-  const Kernel kernel = kernels[g.kind];
-  {
-    static std::mutex mu;
-    static bool configured[3][64] = {};
-    std::lock_guard<std::mutex> lock(mu);
-    if (dev.device >= 64 || !configured[g.kind][dev.device]) {
-      if (cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes) != cudaSuccess) {
-        cudaGetLastError();
-        return MXB200_ERR_LAUNCH;
-      }
-      if (dev.device < 64)
-        configured[g.kind][dev.device] = true;
-    }
-  }
-  return launch_kernel(kernel, grid, kThreads, kSmemBytes, stream, l);
+  if (st = set_smem_once(v, dev.device); st != MXB200_OK)
+    return st;
+  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(units, dev.sms / v.ctas)) * v.ctas;
+  return launch_kernel(v.kernel, grid, kThreads, v.smem, stream, l);
 }
 
 }  // namespace

@@ -37,7 +37,8 @@ struct QuantizeParams {
   uint8_t* row_data;    // rows: (rows, cols); null where they are not wanted
   float* row_scale;     // (cols / 128, rows)
   uint8_t* col_data;    // tokens: (token blocks * 128, cols); weight: (experts, rows, cols)
-  float* col_scale;     // tokens: (token blocks, cols); weight: (experts, rows / 128, cols / 128)
+  float* col_scale;     // weight: (experts, rows / 128, cols / 128)
+  uint32_t* col_scale_words;  // tokens: (token blocks, cols / 128, 128)
 };
 
 struct Values {
@@ -174,12 +175,14 @@ __device__ __forceinline__ void quantize_activation(const QuantizeParams& p, int
           *reinterpret_cast<uint2*>(p.col_data + (out0 + 16 * i) * p.cols + col) =
                 make_uint2(e4m3x4_from_f32(v[i].v[0] * f[0], v[i].v[1] * f[1], v[i].v[2] * f[2], v[i].v[3] * f[3]),
                            e4m3x4_from_f32(v[i].v[4] * f[4], v[i].v[5] * f[5], v[i].v[6] * f[6], v[i].v[7] * f[7]));
-        if (row == 0) {
-          float4* dst = reinterpret_cast<float4*>(p.col_scale + static_cast<int64_t>(blockIdx.x) * p.cols + col);
-          dst[0] = make_float4(scale_of(e[0]), scale_of(e[1]), scale_of(e[2]), scale_of(e[3]));
-          dst[1] = make_float4(scale_of(e[4]), scale_of(e[5]), scale_of(e[6]), scale_of(e[7]));
-        }
       }
+      // a tile of 128 columns' scale bytes, each four times, in the order that the copy to tensor memory takes
+      const int c = 8 * lane16 + row;
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (row == k)
+          p.col_scale_words[(static_cast<int64_t>(blockIdx.x) * tiles + t) * kBlock + (c & 31) * 4 + (c >> 5)] =
+                static_cast<uint32_t>(e[k]) * 0x01010101u;
     }
   }
 }
@@ -282,7 +285,7 @@ int check_pointers(std::initializer_list<const void*> pointers) {
 }  // namespace mxb200
 
 extern "C" int mxb200_block_quantize(const void* x, int64_t rows, int64_t cols, int64_t ld, const int32_t* ends, int experts,
-                                     void* row_data, float* row_scale, void* token_data, float* token_scale, void* stream) {
+                                     void* row_data, float* row_scale, void* token_data, uint32_t* token_scale, void* stream) {
   using namespace mxb200;
   if (rows < 0 || rows > kMost || cols <= 0 || cols > kMost || cols % 16 || ld < cols || ld % 8 || experts < 1 || experts > kMaxExperts)
     return MXB200_ERR_SHAPE;
@@ -303,7 +306,7 @@ extern "C" int mxb200_block_quantize(const void* x, int64_t rows, int64_t cols, 
   if (int st = want_tokens ? check_pointers({token_data, token_scale}) : MXB200_OK; st != MXB200_OK)
     return st;
   QuantizeParams p{x, ld, 0, rows, cols, ends, experts, static_cast<uint8_t*>(row_data), row_scale,
-                   static_cast<uint8_t*>(token_data), token_scale};
+                   static_cast<uint8_t*>(token_data), nullptr, token_scale};
   // enough blocks to fill the machine; beyond that a block goes on to its rows' next columns, with its experts looked up once
   const int64_t blocks = want_tokens ? mxb200_block_token_blocks(rows, experts) : up(rows, kBlock);
   const int64_t parts = std::min<int64_t>(up(cols, kBlock), std::max<int64_t>(1, up(8 * dev.sms, blocks)));
@@ -325,7 +328,7 @@ extern "C" int mxb200_block_quantize_weight(const void* w, int w_bf16, int exper
     return st;
   if (int st = check_pointers({w, data, scale}); st != MXB200_OK)
     return st;
-  QuantizeParams p{w, cols, rows * cols, rows, cols, nullptr, experts, nullptr, nullptr, static_cast<uint8_t*>(data), scale};
+  QuantizeParams p{w, cols, rows * cols, rows, cols, nullptr, experts, nullptr, nullptr, static_cast<uint8_t*>(data), scale, nullptr};
   return launch_kernel(w_bf16 ? mxb200_block_quantize_weight_bf16 : mxb200_block_quantize_weight_f32, static_cast<unsigned>(tiles),
                        kThreads, 0, static_cast<cudaStream_t>(stream), p);
 }

@@ -43,6 +43,18 @@ __device__ __forceinline__ void grid_dependency_wait() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
+// The registers of each thread of a warpgroup (four consecutive warps from a multiple of four, all of which execute it): given
+// back, or drawn from what the block's other warpgroups gave back (waits for it). Multiples of 8.
+template <int kRegisters>
+__device__ __forceinline__ void set_max_registers_down() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegisters));
+}
+
+template <int kRegisters>
+__device__ __forceinline__ void set_max_registers_up() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegisters));
+}
+
 // ---------------------------------------------------------------------------------------------- mbarrier
 
 __device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
@@ -331,6 +343,9 @@ __host__ __device__ constexpr uint32_t make_idesc_mxf8(uint32_t m, uint32_t n) {
 __host__ __device__ constexpr uint32_t make_idesc_f8(uint32_t m, uint32_t n, bool a_mn, bool b_mn) {
   return (1u << 4) | (static_cast<uint32_t>(a_mn) << 15) | (static_cast<uint32_t>(b_mn) << 16) | ((n >> 3) << 17) | ((m >> 4) << 24);
 }
+
+// The MN-major bits of either descriptor.
+constexpr uint32_t kIdescAMn = 1u << 15, kIdescBMn = 1u << 16;
 
 __device__ __forceinline__ uint32_t idesc_with_sf(uint32_t idesc, uint32_t a_sf_id, uint32_t b_sf_id) {
   return idesc | (b_sf_id << 4) | (a_sf_id << 29);

@@ -1015,7 +1015,7 @@ Block empty_row_blocks(int64_t rows, int64_t cols, at::Device device) {
 
 Block empty_token_blocks(int64_t rows, int64_t cols, const Experts& e, at::Device device) {
   const int64_t blocks = mxb200_block_token_blocks(rows, e.count);
-  return {empty({128 * blocks, cols}, kE4M3, device), empty({blocks, cols}, at::kFloat, device)};
+  return {empty({128 * blocks, cols}, kE4M3, device), empty({blocks, blocks_of(cols), 128}, at::kInt, device)};
 }
 
 // x (rows, cols) bf16 with contiguous columns into either layout or both.
@@ -1025,7 +1025,7 @@ void quantize_blocks(const Tensor& x, const Experts& e, const Block* rows, const
                               rows != nullptr ? rows->data.data_ptr() : nullptr,
                               rows != nullptr ? static_cast<float*>(rows->scale.data_ptr()) : nullptr,
                               tokens != nullptr ? tokens->data.data_ptr() : nullptr,
-                              tokens != nullptr ? static_cast<float*>(tokens->scale.data_ptr()) : nullptr, stream()),
+                              tokens != nullptr ? static_cast<uint32_t*>(tokens->scale.data_ptr()) : nullptr, stream()),
         "quantize_block");
 }
 
@@ -1037,8 +1037,7 @@ Tensor readable_rows(const Tensor& x) {
 }
 
 void block_product(int kind, const Block& a, const Block& b, const Tensor& d, const Experts& e, int64_t tokens, int64_t in, int64_t out) {
-  const mxb200_block_gemm_args g{a.data.data_ptr(), static_cast<const float*>(a.scale.data_ptr()), b.data.data_ptr(),
-                                 static_cast<const float*>(b.scale.data_ptr()), d.data_ptr(), e.ends, tokens, in, out, e.count, kind,
+  const mxb200_block_gemm_args g{a.data.data_ptr(), a.scale.data_ptr(), b.data.data_ptr(), b.scale.data_ptr(), d.data_ptr(), e.ends, tokens, in, out, e.count, kind,
                                  d.scalar_type() == at::kFloat ? MXB200_OUT_F32 : MXB200_OUT_BF16};
   check(mxb200_block_gemm(&g, stream()), "block_gemm");
 }
