@@ -292,6 +292,8 @@ typedef enum mxb200_block_kind {
   MXB200_BLOCK_WEIGHT_GRAD = 2  /* d (experts, out, in) bf16 or fp32 = a (., out)^T, tokens . b (., in), tokens */
 } mxb200_block_kind;
 
+#define MXB200_BLOCK_FEW_TOKENS 32
+
 /* One product per expert over its rows, fp32 accumulation, rounded once. Rows of no expert: zeros; the weight gradient of an
  * expert without rows: zeros. Needs no workspace. tokens may be 0. */
 typedef struct mxb200_block_gemm_args {
@@ -305,6 +307,9 @@ typedef struct mxb200_block_gemm_args {
   int32_t experts;
   int32_t kind;     /* mxb200_block_kind */
   int32_t out_kind; /* mxb200_out_kind; F32 for the weight gradient only */
+  int64_t b_ld;     /* 0: b is quantized. Else (FORWARD of up to MXB200_BLOCK_FEW_TOKENS tokens) b is bf16, b_ld values between
+                       rows (b_ld % 8 == 0), and quantized on its way, with the bits that mxb200_block_quantize and this
+                       product of its output give; b_scale is not read. A launch costs more than every CTA's repeating that. */
 } mxb200_block_gemm_args;
 MXB200_API int mxb200_block_gemm(const mxb200_block_gemm_args* args, void* stream);
 

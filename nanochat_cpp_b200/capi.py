@@ -72,7 +72,7 @@ class BlockGemmArgs(ctypes.Structure):
     _fields_ = [("a", ctypes.c_void_p), ("a_scale", ctypes.c_void_p), ("b", ctypes.c_void_p), ("b_scale", ctypes.c_void_p),
                 ("d", ctypes.c_void_p), ("ends", ctypes.c_void_p), ("tokens", ctypes.c_int64), ("in_features", ctypes.c_int64),
                 ("out_features", ctypes.c_int64), ("experts", ctypes.c_int32), ("kind", ctypes.c_int32),
-                ("out_kind", ctypes.c_int32)]
+                ("out_kind", ctypes.c_int32), ("b_ld", ctypes.c_int64)]
 
 
 class BlockNormArgs(ctypes.Structure):

@@ -63,6 +63,8 @@ enum WaitSite : uint32_t {
   kSiteAccFull = 5,
   kSiteScaleFull = 6,
   kSiteOverlap = 7,
+  kSitePartialEmpty = 8,
+  kSitePartialFull = 9,
 };
 
 // Barriers and what the roles of a CTA share. kStages: operand stages of kABytes + kBBytes.
@@ -93,6 +95,9 @@ struct Params {
   int n;         // weight gradient: its columns
   int blocks;    // contraction blocks (forward, input grad)
   int out_bf16;
+  int splits;    // few tokens: CTAs of a cluster that share a unit's blocks
+  const void* input;    // few tokens, quantized on the way: bf16 rows token_ld values apart, of `input_cols` values
+  int input_cols;
 };
 
 struct Maps {
@@ -100,12 +105,16 @@ struct Maps {
   CUtensorMap a_scale, b_scale;  // weight gradient
 };
 
+// A warp's wait for a barrier phase, given up after kWaitLimitNs; its lanes agree on the outcome. kCluster: what other CTAs of
+// the cluster wrote before they arrived is visible.
+template <bool kCluster = false>
 __device__ __forceinline__ bool wait_bounded(uint32_t bar, uint32_t parity, uint32_t* abort_flag, uint32_t site) {
+  const auto done = [&] { return kCluster ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity); };
   bool ok = true;
-  if (!mbar_try_wait(bar, parity)) {
+  if (!done()) {
     const uint64_t t0 = global_timer_ns();
     uint32_t spins = 0;
-    while (!mbar_try_wait(bar, parity)) {
+    while (!done()) {
       if ((++spins & 63u) == 0) {
         if (*reinterpret_cast<volatile uint32_t*>(abort_flag) != 0) {
           ok = false;
@@ -151,22 +160,32 @@ __device__ __forceinline__ float2 both(uint64_t v) {
   return make_float2(__uint_as_float(lo), __uint_as_float(hi));
 }
 
+struct SetUp {
+  uint32_t full_arrivals, empty_arrivals;  // of an operand stage
+  uint32_t acc_empty_arrivals;
+  int acc_buffers;
+  uint32_t scale_arrivals;
+  int tile_rows;       // of the tiles that experts' rows are cut into
+  bool rest_is_a_tile; // the rows behind the last expert's, as one more expert without a weight
+};
+
 // Barriers, tensor memory and the experts' rows; the operand stages at `base` hold the scan's words meanwhile. All threads.
+// kCtas: that share tensor memory operations. cluster: the CTAs of a cluster signal one another.
 template <int kCtas, typename S>
 __device__ __forceinline__ uint32_t set_up(const Params& p, const CUtensorMap* map_a, const CUtensorMap* map_b, S* s, unsigned char* base,
-                                           int warp, int acc_buffers, uint32_t scale_arrivals, int tile_rows, bool rest_is_a_tile) {
+                                           int warp, const SetUp& set, bool cluster) {
   if (threadIdx.x == 0) {
     for (int i = 0; i < S::kStages; ++i) {
-      mbar_init(&s->full[i], 1);
-      mbar_init(&s->empty[i], 1);
+      mbar_init(&s->full[i], set.full_arrivals);
+      mbar_init(&s->empty[i], set.empty_arrivals);
     }
-    for (int i = 0; i < acc_buffers; ++i) {
+    for (int i = 0; i < set.acc_buffers; ++i) {
       mbar_init(&s->acc_full[i], 1);
-      mbar_init(&s->acc_empty[i], kEpilogueWarps * kCtas);
+      mbar_init(&s->acc_empty[i], set.acc_empty_arrivals);
     }
     for (int i = 0; i < kScaleSlots; ++i) {
-      mbar_init(&s->scale_full[i], scale_arrivals);
-      mbar_init(&s->scale_empty[i], kEpilogueWarps);
+      mbar_init(&s->scale_full[i], set.scale_arrivals);
+      mbar_init(&s->scale_empty[i], set.acc_empty_arrivals / kCtas);
     }
     mbar_init(&s->overlap_free, 4 * kCtas);
     s->abort_flag = 0;
@@ -185,16 +204,15 @@ __device__ __forceinline__ uint32_t set_up(const Params& p, const CUtensorMap* m
   }
   tcgen05_fence_before_sync();
   grid_dependency_wait();
-  scan_experts(p.ends, p.experts, p.rows, tile_rows, s->first_row, s->first_tile, reinterpret_cast<int*>(base));
-  if (rest_is_a_tile && p.ends != nullptr && threadIdx.x == 0) {
-    // the rows behind the last expert's, as one more expert without a weight
+  scan_experts(p.ends, p.experts, p.rows, set.tile_rows, s->first_row, s->first_tile, reinterpret_cast<int*>(base));
+  if (set.rest_is_a_tile && p.ends != nullptr && threadIdx.x == 0) {
     s->first_row[p.experts + 1] = p.rows;
-    s->first_tile[p.experts + 1] = s->first_tile[p.experts] + (p.rows - s->first_row[p.experts] + tile_rows - 1) / tile_rows;
+    s->first_tile[p.experts + 1] = s->first_tile[p.experts] + (p.rows - s->first_row[p.experts] + set.tile_rows - 1) / set.tile_rows;
   }
   fence_proxy_async_smem();  // operands are loaded over the scan's words
   __syncthreads();
-  if constexpr (kCtas == 2) {
-    cluster_arrive();  // the peer's barriers exist before anything is credited to them
+  if (cluster) {
+    cluster_arrive();  // the others' barriers exist before anything is credited to them
     cluster_wait();
   }
   tcgen05_fence_after_sync();
@@ -202,7 +220,7 @@ __device__ __forceinline__ uint32_t set_up(const Params& p, const CUtensorMap* m
 }
 
 template <int kCtas, typename S>
-__device__ __forceinline__ void tear_down(S* s, uint32_t tmem_base, int warp) {
+__device__ __forceinline__ void tear_down(S* s, uint32_t tmem_base, int warp, bool cluster) {
   __syncwarp();
   // on an abort, copies and MMAs in flight get time to land before shared and tensor memory go away
   if (*reinterpret_cast<volatile uint32_t*>(&s->abort_flag) != 0) {
@@ -212,8 +230,8 @@ __device__ __forceinline__ void tear_down(S* s, uint32_t tmem_base, int warp) {
   }
   tcgen05_fence_before_sync();
   __syncthreads();
-  if constexpr (kCtas == 2) {
-    cluster_arrive();  // neither CTA leaves while the other can still read its shared memory or signal its barriers
+  if (cluster) {
+    cluster_arrive();  // no CTA leaves while another can still read its shared memory or signal its barriers
     cluster_wait();
   }
   if (warp == 1) {
@@ -287,68 +305,101 @@ __device__ __forceinline__ void store_lines(LineStage* stage, int lane, unsigned
 
 // ==================================================================================================== few tokens
 //
-// Rows of the tensor core's tile are features (the weight is operand A), columns tokens.
+// Rows of the tensor core's tile are features (the weight is operand A), columns tokens. Where the output has fewer tiles than
+// the machine SMs, a cluster of up to 8 CTAs shares one: each contracts a share of the blocks, leaves its fp32 tile in shared
+// memory, and adds up every n-th token of all of them, always in the cluster's order.
+//
+// kQuantize: the input comes in bf16 and is quantized on its way into shared memory, by the four warps that would accumulate
+// the second half of the columns: up to 32 tokens per tile. That spares a launch, and for a token or two the work is nothing
+// although every CTA repeats it.
 
 namespace few {
 
-constexpr int kTileF = 128, kTileT = 128;
-constexpr int kPartT = kTileT / 2;  // columns per epilogue warp: two warps share a tensor memory quarter
-constexpr int kChunks = kPartT / 32;
-constexpr int kAccBuffers = kTmemCols / kTileT;
+constexpr int kTileF = 128;
 constexpr uint32_t kStageRowBytes = 80;  // 32 bf16 and 16 bytes that put 8 rows' 16-byte pieces into different banks
+constexpr int kPartialRow = 132;         // floats of a token's 128 features: fragments' rows fall into different banks
 
-struct __align__(16) ScaleSlot {  // tokens' scales are read in pairs
-  float token[kTileT];
-  float weight;
+// kTile: tokens of a unit, 128, or 32 where no more are expected: more stages of the weight, which is what such a product reads,
+// fit beside so few tokens.
+template <int kTile, bool kQuantize_>
+struct Config {
+  static constexpr bool kQuantize = kQuantize_;
+  static constexpr int kTileT = kTile;
+  static constexpr int kWarps = kTile == 32 ? 4 : 8;  // that accumulate
+  static constexpr int kParts = kWarps / 4;           // columns are shared by the warps of a tensor memory quarter
+  static constexpr int kPartT = kTile / kParts;
+  static constexpr int kChunks = kPartT / 32;
+  static constexpr int kAccBuffers = 4;
+
+  struct __align__(16) ScaleSlot {  // tokens' scales are read in pairs
+    float token[kTileT];
+    float weight;
+  };
+
+  struct Shared : Common<kTile == 32 ? 8 : 5> {
+    uint64_t partial_full, partial_empty;
+    ScaleSlot scales[kScaleSlots];
+    union {
+      __align__(16) unsigned char out[kWarps][32 * kStageRowBytes];
+      __align__(16) float partial[kPartT][kPartialRow];
+    };
+  };
+  static constexpr uint32_t kStageBBytes = kTileT * kBlock;
+  static constexpr size_t kSmemBytes = 1024 + Shared::kStages * static_cast<size_t>(kABytes + kStageBBytes) + sizeof(Shared);
+  static_assert(kSmemBytes <= 232448, "shared memory of one CTA");
+  static_assert(Shared::kStages * kABytes >= kMaxExperts * 4, "the operand stages hold the scan's copy of ends");
 };
 
-struct Shared : Common<5> {
-  ScaleSlot scales[kScaleSlots];
-  __align__(16) unsigned char out[kEpilogueWarps][32 * kStageRowBytes];
+// Which CTA of which cluster this is, and its share of a unit's blocks.
+struct Place {
+  int rank, splits, cluster, clusters;
+  __device__ Place(int n) : rank(static_cast<int>(cluster_ctarank())), splits(n), cluster(blockIdx.x / n), clusters(gridDim.x / n) {}
+  __device__ int begin(int blocks) const { return blocks * rank / splits; }
+  __device__ int end(int blocks) const { return blocks * (rank + 1) / splits; }
 };
 
-constexpr size_t kSmemBytes = 1024 + Shared::kStages * static_cast<size_t>(kABytes + kBBytes) + sizeof(Shared);
-static_assert(kSmemBytes <= 232448, "shared memory of one CTA");
-static_assert(Shared::kStages * kABytes >= kMaxExperts * 4, "the operand stages hold the scan's copy of ends");
-
-template <int kMode>
-__device__ __forceinline__ void load_operands(const Params& p, const CUtensorMap* map_w, const CUtensorMap* map_t, Shared* s, uint32_t a0,
-                                              uint32_t b0, int units) {
+template <int kMode, typename C>
+__device__ __forceinline__ void load_operands(const Params& p, const CUtensorMap* map_w, const CUtensorMap* map_t, typename C::Shared* s,
+                                              uint32_t a0, uint32_t b0, const Place& at, int units) {
   const uint32_t el = elect_one() ? 1u : 0u;
   const uint32_t empty0 = smem_u32(&s->empty[0]), full0 = smem_u32(&s->full[0]);
   uint32_t stage = 0, phase = 0;
-  for (int u = blockIdx.x; u < units; u += gridDim.x) {
-    const Unit x = unit_at<kTileT, kTileF>(p, s, u);
-    const int boxes = (x.rows + 31) / 32;
-    for (int b = 0; b < x.blocks; ++b) {
+  for (int u = at.cluster; u < units; u += at.clusters) {
+    const Unit x = unit_at<C::kTileT, kTileF>(p, s, u);
+    const int boxes = C::kQuantize ? 0 : (x.rows + 31) / 32;
+    for (int b = at.begin(x.blocks); b < at.end(x.blocks); ++b) {
       if (!wait_bounded(empty0 + stage * 8, phase ^ 1u, &s->abort_flag, kSiteStageEmpty))
         return;
       const uint32_t full = full0 + stage * 8;
       mbar_arrive_expect_tx(el, full, kABytes + boxes * kBBoxBytes);
       tma_load_3d(el, a0 + stage * kABytes, map_w, full, kMode == kForward ? b * kBlock : x.f0, kMode == kForward ? x.f0 : b * kBlock, x.expert);
       for (int i = 0; i < boxes; ++i)
-        tma_load_3d(el, b0 + stage * kBBytes + i * kBBoxBytes, map_t, full, b * kBlock, x.row0 + 32 * i, 0);
-      if (++stage == Shared::kStages)
+        tma_load_3d(el, b0 + stage * C::kStageBBytes + i * kBBoxBytes, map_t, full, b * kBlock, x.row0 + 32 * i, 0);
+      if (++stage == C::Shared::kStages)
         stage = 0, phase ^= 1u;
     }
   }
 }
 
+__device__ __forceinline__ const float* weight_scale(const Params& p, const Unit& x, int b) {
+  return p.weight_scale + x.expert * p.w_scale_expert + (x.f0 >> 7) * static_cast<int64_t>(p.w_scale_f) + b * static_cast<int64_t>(p.w_scale_b);
+}
+
 // A block's scales by 4-byte copies: an expert's tokens start at any row.
-__device__ __forceinline__ void load_scales(const Params& p, Shared* s, int units, int lane) {
+template <typename C>
+__device__ __forceinline__ void load_scales(const Params& p, typename C::Shared* s, const Place& at, int units, int lane) {
   const uint32_t scale_full0 = smem_u32(&s->scale_full[0]), scale_empty0 = smem_u32(&s->scale_empty[0]);
   uint32_t slot = 0, slot_phase = 0;
-  for (int u = blockIdx.x; u < units; u += gridDim.x) {
-    const Unit x = unit_at<kTileT, kTileF>(p, s, u);
-    for (int b = 0; b < x.blocks; ++b) {
+  for (int u = at.cluster; u < units; u += at.clusters) {
+    const Unit x = unit_at<C::kTileT, kTileF>(p, s, u);
+    for (int b = at.begin(x.blocks); b < at.end(x.blocks); ++b) {
       if (!wait_bounded(scale_empty0 + slot * 8, slot_phase ^ 1u, &s->abort_flag, kSiteScaleEmpty))
         return;
       const float* token = p.token_scale + b * p.token_ld + x.row0;
       for (int i = lane; i < x.rows; i += 32)
         cp_async_4(smem_u32(&s->scales[slot].token[i]), token + i);
       if (lane == 0)
-        cp_async_4(smem_u32(&s->scales[slot].weight), p.weight_scale + x.expert * p.w_scale_expert +
-                                                            (x.f0 >> 7) * static_cast<int64_t>(p.w_scale_f) + b * static_cast<int64_t>(p.w_scale_b));
+        cp_async_4(smem_u32(&s->scales[slot].weight), weight_scale(p, x, b));
       cp_async_arrive(scale_full0 + slot * 8);
       if (++slot == kScaleSlots)
         slot = 0, slot_phase ^= 1u;
@@ -356,8 +407,85 @@ __device__ __forceinline__ void load_scales(const Params& p, Shared* s, int unit
   }
 }
 
-template <int kMode>
-__device__ __forceinline__ void issue_mmas(const Params& p, Shared* s, uint32_t a0, uint32_t b0, uint32_t tmem_base, int units) {
+// The input's blocks from bf16 into shared memory as a TMA load would leave them (128-byte swizzle), and their scales: 16 lanes
+// per token, 8 tokens at a time, a block ahead in registers. The values are block_quantize_sm100.cu's.
+template <typename C>
+__device__ __forceinline__ void quantize(const Params& p, typename C::Shared* s, unsigned char* b_stages, const Place& at, int units, int warp,
+                                         int lane) {
+  static_assert(C::kTileT == 32, "four tokens per thread");
+  const uint32_t full0 = smem_u32(&s->full[0]), empty0 = smem_u32(&s->empty[0]);
+  const uint32_t scale_full0 = smem_u32(&s->scale_full[0]), scale_empty0 = smem_u32(&s->scale_empty[0]);
+  const int lane16 = lane & 15, token0 = 2 * (warp & 3) + (lane >> 4);
+  const int in = p.input_cols;
+  const uint16_t* input = static_cast<const uint16_t*>(p.input);
+  uint4 ahead[4];
+  float weight_ahead = 0.f;
+  const auto fetch = [&](const Unit& x, int b) {
+    const int col = b * kBlock + 8 * lane16;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int t = token0 + 8 * i;
+      ahead[i] = t < x.rows && col < in ? *reinterpret_cast<const uint4*>(input + (x.row0 + t) * p.token_ld + col) : make_uint4(0, 0, 0, 0);
+    }
+    weight_ahead = *weight_scale(p, x, b);
+  };
+  uint32_t stage = 0, phase = 0, slot = 0, slot_phase = 0;
+  for (int u = at.cluster; u < units; u += at.clusters) {
+    const Unit x = unit_at<C::kTileT, kTileF>(p, s, u);
+    const int end = at.end(x.blocks);
+    int b = at.begin(x.blocks);
+    if (b < end)
+      fetch(x, b);
+    for (; b < end; ++b) {
+      uint4 now[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        now[i] = ahead[i];
+      const float weight = weight_ahead;
+      if (b + 1 < end)
+        fetch(x, b + 1);
+      if (!wait_bounded(empty0 + stage * 8, phase ^ 1u, &s->abort_flag, kSiteStageEmpty) ||
+          !wait_bounded(scale_empty0 + slot * 8, slot_phase ^ 1u, &s->abort_flag, kSiteScaleEmpty))
+        return;
+      unsigned char* to = b_stages + stage * C::kStageBBytes;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (8 * i >= x.rows)
+          break;
+        const int t = token0 + 8 * i;
+        const uint32_t w[4] = {now[i].x, now[i].y, now[i].z, now[i].w};
+        uint32_t m = max_abs_skip_nan_bf16x2(max_abs_skip_nan_bf16x2(max_abs_skip_nan_bf16x2(max_abs_skip_nan_bf16x2(0u, w[0]), w[1]), w[2]), w[3]);
+        m &= 0x7fff7fffu;
+        m = max(m & 0xffffu, m >> 16);
+#pragma unroll
+        for (int d = 8; d > 0; d >>= 1)
+          m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
+        const int e = block_exponent(m << 16);
+        const uint16_t by = static_cast<uint16_t>(mx_multiplier_bits(e) >> 16);
+        *reinterpret_cast<uint2*>(to + t * kBlock + (((lane16 >> 1) ^ (t & 7)) << 4) + (lane16 & 1) * 8) =
+              make_uint2(e4m3x4_scaled_fma(w[0], w[1], by, by), e4m3x4_scaled_fma(w[2], w[3], by, by));
+        if (lane16 == 0)
+          s->scales[slot].token[t] = __uint_as_float(static_cast<uint32_t>(e) << 23);
+      }
+      if (threadIdx.x == 32 * (kFirstEpilogueWarp + C::kWarps))
+        s->scales[slot].weight = weight;
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive_addr(full0 + stage * 8);
+        mbar_arrive_addr(scale_full0 + slot * 8);
+      }
+      if (++stage == C::Shared::kStages)
+        stage = 0, phase ^= 1u;
+      if (++slot == kScaleSlots)
+        slot = 0, slot_phase ^= 1u;
+    }
+  }
+}
+
+template <int kMode, typename C>
+__device__ __forceinline__ void issue_mmas(const Params& p, typename C::Shared* s, uint32_t a0, uint32_t b0, uint32_t tmem_base, const Place& at,
+                                           int units) {
   constexpr bool kAMn = kMode == kInputGrad;
   // 128-byte swizzle, groups of 8 rows of 128 bytes 1024 apart. K-major: K = 32 is 32 bytes within a row; MN-major: 32 rows.
   constexpr uint32_t kAStep = kAMn ? 4096 >> 4 : 32 >> 4, kBStep = 32 >> 4;
@@ -365,23 +493,23 @@ __device__ __forceinline__ void issue_mmas(const Params& p, Shared* s, uint32_t 
   const uint32_t full0 = smem_u32(&s->full[0]);
   const uint64_t a_desc0 = make_smem_desc(a0, 1024, 1024, 2), b_desc0 = make_smem_desc(b0, 1024, 1024, 2);
   uint32_t stage = 0, phase = 0, buf = 0, buf_phase = 0;
-  for (int u = blockIdx.x; u < units; u += gridDim.x) {
-    const Unit x = unit_at<kTileT, kTileF>(p, s, u);
+  for (int u = at.cluster; u < units; u += at.clusters) {
+    const Unit x = unit_at<C::kTileT, kTileF>(p, s, u);
     const uint32_t idesc = make_idesc_f8(kTileF, (x.rows + 15) / 16 * 16, kAMn, false);
-    for (int b = 0; b < x.blocks; ++b) {
+    for (int b = at.begin(x.blocks); b < at.end(x.blocks); ++b) {
       if (!wait_bounded(smem_u32(&s->acc_empty[buf]), buf_phase ^ 1u, &s->abort_flag, kSiteAccEmpty) ||
           !wait_bounded(full0 + stage * 8, phase, &s->abort_flag, kSiteStageFull))
         return;
       tcgen05_fence_after_sync();
-      const uint64_t a = a_desc0 + stage * (kABytes >> 4), bd = b_desc0 + stage * (kBBytes >> 4);
+      const uint64_t a = a_desc0 + stage * (kABytes >> 4), bd = b_desc0 + stage * (C::kStageBBytes >> 4);
 #pragma unroll
       for (uint32_t k = 0; k < 4; ++k)
-        tcgen05_mma_f8(el, tmem_base + buf * kTileT, a + k * kAStep, bd + k * kBStep, idesc, k > 0);
+        tcgen05_mma_f8(el, tmem_base + buf * C::kTileT, a + k * kAStep, bd + k * kBStep, idesc, k > 0);
       tcgen05_commit(el, &s->empty[stage]);
       tcgen05_commit(el, &s->acc_full[buf]);
-      if (++stage == Shared::kStages)
+      if (++stage == C::Shared::kStages)
         stage = 0, phase ^= 1u;
-      if (++buf == kAccBuffers)
+      if (++buf == C::kAccBuffers)
         buf = 0, buf_phase ^= 1u;
     }
   }
@@ -413,31 +541,33 @@ __device__ __forceinline__ void store_chunk(const Params& p, const Unit& x, unsi
   }
 }
 
-__device__ __forceinline__ void accumulate(const Params& p, Shared* s, uint32_t tmem_base, int units, int warp, int lane) {
-  const int quarter = warp & 3, part0 = ((warp - kFirstEpilogueWarp) >> 2) * kPartT;  // a warp reads tensor memory lanes 32 (warp % 4) on
+template <typename C>
+__device__ __forceinline__ void accumulate(const Params& p, typename C::Shared* s, uint32_t tmem_base, const Place& at, int units, int warp,
+                                           int lane) {
+  const int quarter = warp & 3, part = (warp - kFirstEpilogueWarp) >> 2, part0 = part * C::kPartT;  // tensor memory lanes 32 (warp % 4) on
   const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
   unsigned char* stage = s->out[warp - kFirstEpilogueWarp];
-  uint32_t buf = 0, buf_phase = 0, slot = 0, slot_phase = 0;
-  for (int u = blockIdx.x; u < units; u += gridDim.x) {
-    const Unit x = unit_at<kTileT, kTileF>(p, s, u);
-    uint64_t acc[kChunks][4][4];
+  uint32_t buf = 0, buf_phase = 0, slot = 0, slot_phase = 0, partial_phase = 0;
+  for (int u = at.cluster; u < units; u += at.clusters) {
+    const Unit x = unit_at<C::kTileT, kTileF>(p, s, u);
+    uint64_t acc[C::kChunks][4][4];
 #pragma unroll
-    for (int c = 0; c < kChunks; ++c)
+    for (int c = 0; c < C::kChunks; ++c)
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           acc[c][j][i] = 0;
-    for (int b = 0; b < x.blocks; ++b) {
+    for (int b = at.begin(x.blocks); b < at.end(x.blocks); ++b) {
       if (!wait_bounded(smem_u32(&s->scale_full[slot]), slot_phase, &s->abort_flag, kSiteScaleFull) ||
           !wait_bounded(smem_u32(&s->acc_full[buf]), buf_phase, &s->abort_flag, kSiteAccFull))
         return;
       tcgen05_fence_after_sync();
-      const ScaleSlot& sc = s->scales[slot];
+      const auto& sc = s->scales[slot];
       const uint64_t weight = pair_f32(sc.weight, sc.weight);
-      const uint32_t t = tmem_base + lane_base + buf * kTileT + part0;
+      const uint32_t t = tmem_base + lane_base + buf * C::kTileT + part0;
 #pragma unroll
-      for (int c = 0; c < kChunks; ++c) {
+      for (int c = 0; c < C::kChunks; ++c) {
         if (part0 + 32 * c >= x.rows)
           break;
         uint32_t lo[16], hi[16];
@@ -468,38 +598,102 @@ __device__ __forceinline__ void accumulate(const Params& p, Shared* s, uint32_t 
         mbar_arrive(&s->acc_empty[buf]);
         mbar_arrive(&s->scale_empty[slot]);
       }
-      if (++buf == kAccBuffers)
+      if (++buf == C::kAccBuffers)
         buf = 0, buf_phase ^= 1u;
       if (++slot == kScaleSlots)
         slot = 0, slot_phase ^= 1u;
     }
-    const int feature0 = x.f0 + quarter * 32;
+    if (at.splits == 1) {
+      const int feature0 = x.f0 + quarter * 32;
 #pragma unroll
-    for (int c = 0; c < kChunks; ++c)
-      if (part0 + 32 * c < x.rows && feature0 < p.features)
-        store_chunk(p, x, stage, lane, feature0, part0 + 32 * c, acc[c]);
+      for (int c = 0; c < C::kChunks; ++c)
+        if (part0 + 32 * c < x.rows && feature0 < p.features)
+          store_chunk(p, x, stage, lane, feature0, part0 + 32 * c, acc[c]);
+      continue;
+    }
+    for (int h = 0; h < C::kParts; ++h) {
+      const int first = h * C::kPartT, rows = min(C::kPartT, x.rows - first);
+      if (rows <= 0)
+        break;
+      // this CTA's share of these columns into its shared memory, once the cluster has read the last ones ...
+      if (!wait_bounded<true>(smem_u32(&s->partial_empty), partial_phase ^ 1u, &s->abort_flag, kSitePartialEmpty))
+        return;
+      if (h == part) {
+#pragma unroll
+        for (int c = 0; c < C::kChunks; ++c) {
+          if (32 * c >= rows)
+            break;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float2 f = both(acc[c][j][i]);
+              float* to = &s->partial[32 * c + 8 * j + 2 * (lane & 3)][quarter * 32 + 8 * i + (lane >> 2)];
+              to[0] = f.x, to[kPartialRow] = f.y;
+            }
+        }
+      }
+      __syncwarp();
+      if (lane < at.splits)
+        mbar_arrive_release_cluster(map_to_cta(smem_u32(&s->partial_full), lane));
+      // ... and the sum of every splits-th token from all of them
+      if (!wait_bounded<true>(smem_u32(&s->partial_full), partial_phase, &s->abort_flag, kSitePartialFull))
+        return;
+      for (int t = at.rank + at.splits * (warp - kFirstEpilogueWarp); t < rows; t += at.splits * C::kWarps) {
+        const uint32_t from = smem_u32(&s->partial[t][4 * lane]);
+        float4 sum = load_cluster(map_to_cta(from, 0));
+        for (int r = 1; r < at.splits; ++r) {
+          const float4 f = load_cluster(map_to_cta(from, r));
+          sum.x += f.x, sum.y += f.y, sum.z += f.z, sum.w += f.w;
+        }
+        if (x.f0 + 4 * lane < p.features)
+          *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.d) + static_cast<int64_t>(x.row0 + first + t) * p.features + x.f0 + 4 * lane) =
+                make_uint2(pack_bf16x2_rn(sum.x, sum.y), pack_bf16x2_rn(sum.z, sum.w));
+      }
+      __syncwarp();
+      if (lane < at.splits)
+        mbar_arrive_release_cluster(map_to_cta(smem_u32(&s->partial_empty), lane));
+      partial_phase ^= 1u;
+    }
   }
 }
 
-template <int kMode>
+template <int kMode, typename C>
 __device__ __forceinline__ void body(const Params& p, const CUtensorMap* map_w, const CUtensorMap* map_t) {
   extern __shared__ unsigned char smem_raw[];
   unsigned char* base = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
-  const uint32_t a0 = smem_u32(base), b0 = a0 + Shared::kStages * kABytes;
-  Shared* s = reinterpret_cast<Shared*>(base + Shared::kStages * (kABytes + kBBytes));
+  unsigned char* b_stages = base + C::Shared::kStages * kABytes;
+  const uint32_t a0 = smem_u32(base), b0 = smem_u32(b_stages);
+  auto* s = reinterpret_cast<typename C::Shared*>(b_stages + C::Shared::kStages * C::kStageBBytes);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t tmem_base = set_up<1>(p, map_w, map_t, s, base, warp, kAccBuffers, 32, kTileT, true);
+  const Place at(p.splits);
+  if (threadIdx.x == 0) {
+    mbar_init(&s->partial_full, C::kWarps * p.splits);
+    mbar_init(&s->partial_empty, C::kWarps * p.splits);
+  }
+  SetUp set{1, 1, C::kWarps, C::kAccBuffers, C::kQuantize ? 4u : 32u, C::kTileT, true};
+  if (C::kQuantize)
+    set.full_arrivals = 5;  // the weight's load and four warps
+  const uint32_t tmem_base = set_up<1>(p, map_w, map_t, s, base, warp, set, p.splits > 1);
   const int units = units_of(p, s, kTileF);
   if (warp == 0)
-    load_operands<kMode>(p, map_w, map_t, s, a0, b0, units);
+    load_operands<kMode, C>(p, map_w, map_t, s, a0, b0, at, units);
   else if (warp == 1)
-    issue_mmas<kMode>(p, s, a0, b0, tmem_base, units);
-  else if (warp == 2)
-    load_scales(p, s, units, lane);
-  else if (warp >= kFirstEpilogueWarp)
-    accumulate(p, s, tmem_base, units, warp, lane);
-  tear_down<1>(s, tmem_base, warp);
+    issue_mmas<kMode, C>(p, s, a0, b0, tmem_base, at, units);
+  else if (warp >= kFirstEpilogueWarp && warp < kFirstEpilogueWarp + C::kWarps)
+    accumulate<C>(p, s, tmem_base, at, units, warp, lane);
+  else if constexpr (C::kQuantize) {
+    if (warp >= kFirstEpilogueWarp)
+      quantize<C>(p, s, b_stages, at, units, warp, lane);
+  } else if (warp == 2) {
+    load_scales<C>(p, s, at, units, lane);
+  }
+  tear_down<1>(s, tmem_base, warp, p.splits > 1);
 }
+
+using Tile128 = Config<128, false>;
+using Tile32 = Config<32, false>;
+using Quantizing = Config<MXB200_BLOCK_FEW_TOKENS, true>;
 
 }  // namespace few
 
@@ -678,7 +872,8 @@ __device__ __forceinline__ void body(const Params& p, const CUtensorMap* map_t, 
   Shared* s = reinterpret_cast<Shared*>(base + Shared::kStages * (kABytes + kBBytes));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = static_cast<int>(cluster_ctarank());
-  const uint32_t tmem_base = set_up<2>(p, map_t, map_w, s, base, warp, kAccBuffers, 32, kTileT, true);
+  const SetUp set{1, 1, 2 * kEpilogueWarps, kAccBuffers, 32, kTileT, true};
+  const uint32_t tmem_base = set_up<2>(p, map_t, map_w, s, base, warp, set, true);
   const int units = units_of(p, s, kTileF), first = blockIdx.x / 2, step = gridDim.x / 2;
   if (warp < kFirstEpilogueWarp) {
     set_max_registers_down<kFewRegisters>();
@@ -692,7 +887,7 @@ __device__ __forceinline__ void body(const Params& p, const CUtensorMap* map_t, 
     set_max_registers_up<kManyRegisters>();
     accumulate(p, s, tmem_base, rank, first, step, units, warp, lane);
   }
-  tear_down<2>(s, tmem_base, warp);
+  tear_down<2>(s, tmem_base, warp, true);
 }
 
 }  // namespace many
@@ -881,7 +1076,8 @@ __device__ __forceinline__ void body(const Params& p, const Maps& maps) {
   Shared* s = reinterpret_cast<Shared*>(base + Shared::kStages * kStageBytes);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = static_cast<int>(cluster_ctarank());
-  const uint32_t tmem_base = set_up<2>(p, &maps.a, &maps.b, s, base, warp, 2, 1, kBlock, false);
+  const SetUp set{1, 1, 2 * kEpilogueWarps, 2, 1, kBlock, false};
+  const uint32_t tmem_base = set_up<2>(p, &maps.a, &maps.b, s, base, warp, set, true);
   const int units = p.experts * ((p.features + kTile - 1) / kTile) * ((p.n + kTile - 1) / kTile);
   const int first = blockIdx.x / 2, step = gridDim.x / 2;
   if (warp == 0)
@@ -890,7 +1086,7 @@ __device__ __forceinline__ void body(const Params& p, const Maps& maps) {
     issue_mmas(p, s, a0, tmem_base, first, step, units);
   else if (warp >= kFirstEpilogueWarp)
     store(p, s, tmem_base, rank, first, step, units, warp, lane);
-  tear_down<2>(s, tmem_base, warp);
+  tear_down<2>(s, tmem_base, warp, true);
 }
 
 }  // namespace wgrad
@@ -904,10 +1100,16 @@ struct Launch {
 }  // namespace mxb200
 
 __global__ void __launch_bounds__(mxb200::kThreads, 1) mxb200_block_gemm_forward_few(const __grid_constant__ mxb200::Launch args) {
-  mxb200::few::body<mxb200::kForward>(args.p, &args.maps.a, &args.maps.b);
+  mxb200::few::body<mxb200::kForward, mxb200::few::Tile128>(args.p, &args.maps.a, &args.maps.b);
+}
+__global__ void __launch_bounds__(mxb200::kThreads, 1) mxb200_block_gemm_forward_32(const __grid_constant__ mxb200::Launch args) {
+  mxb200::few::body<mxb200::kForward, mxb200::few::Tile32>(args.p, &args.maps.a, &args.maps.b);
+}
+__global__ void __launch_bounds__(mxb200::kThreads, 1) mxb200_block_gemm_quantize_few(const __grid_constant__ mxb200::Launch args) {
+  mxb200::few::body<mxb200::kForward, mxb200::few::Quantizing>(args.p, &args.maps.a, &args.maps.b);
 }
 __global__ void __launch_bounds__(mxb200::kThreads, 1) mxb200_block_gemm_input_grad_few(const __grid_constant__ mxb200::Launch args) {
-  mxb200::few::body<mxb200::kInputGrad>(args.p, &args.maps.a, &args.maps.b);
+  mxb200::few::body<mxb200::kInputGrad, mxb200::few::Tile128>(args.p, &args.maps.a, &args.maps.b);
 }
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(mxb200::kThreads, 1)
       mxb200_block_gemm_forward_many(const __grid_constant__ mxb200::Launch args) {
@@ -969,54 +1171,88 @@ struct Variant {
   int tokens, features; // of a unit
 };
 
-constexpr int kFew = 0, kMany = 1;
+enum VariantId : int { kForwardFew, kForward32, kForwardMany, kForwardQuantizing, kInputGradFew, kInputGradMany, kWeightGradPair, kVariants };
 
-const Variant& variant(int kind, int many) {
-  static const Variant variants[5] = {
-        {mxb200_block_gemm_forward_few, few::kSmemBytes, 1, few::kTileT, few::kTileF},
+const Variant& variant(VariantId id) {
+  static const Variant variants[kVariants] = {
+        {mxb200_block_gemm_forward_few, few::Tile128::kSmemBytes, 1, few::Tile128::kTileT, few::kTileF},
+        {mxb200_block_gemm_forward_32, few::Tile32::kSmemBytes, 1, few::Tile32::kTileT, few::kTileF},
         {mxb200_block_gemm_forward_many, many::kSmemBytes, 2, many::kTileT, many::kTileF},
-        {mxb200_block_gemm_input_grad_few, few::kSmemBytes, 1, few::kTileT, few::kTileF},
+        {mxb200_block_gemm_quantize_few, few::Quantizing::kSmemBytes, 1, few::Quantizing::kTileT, few::kTileF},
+        {mxb200_block_gemm_input_grad_few, few::Tile128::kSmemBytes, 1, few::Tile128::kTileT, few::kTileF},
         {mxb200_block_gemm_input_grad_many, many::kSmemBytes, 2, many::kTileT, many::kTileF},
         {mxb200_block_gemm_weight_grad, wgrad::kSmemBytes, 2, 0, wgrad::kTile}};
-  return variants[kind == MXB200_BLOCK_WEIGHT_GRAD ? 4 : 2 * kind + many];
+  return variants[id];
+}
+
+// Token tiles that are expected: how the rows spread over experts is not known here, so every expert is taken to have some, with
+// half a tile left over.
+int64_t expected_tiles(int64_t tokens, int experts, int tile) {
+  const int64_t used = std::min<int64_t>(experts, tokens);
+  return experts == 1 ? up(tokens, tile) : std::max(used, tokens / tile + used / 2);
 }
 
 // Which of the two kernels a product of `blocks` contraction blocks to `features` features takes: the one that is expected to be
 // done first. Both take about 0.45 us for a block of their tile when all SMs are at work, a unit's output costs as much as 3 or 4
 // blocks, and a pair's tile is twice the work per SM of the other's. 16384 x 6144 -> 1536: few tokens 235 us, many 134; 2500 x
 // 1280 -> 3840: 27 and 20; 1111 x 1040 -> 2000: 7.6 and 8.8; 8192 rows over 32 experts, 1536 -> 2048: 59 and 42; 1000 rows over
-// 64: 39 and 54. How the rows spread over experts is not known here: every expert is taken to have some, with half a tile left
-// over.
+// 64: 39 and 54.
 bool many_tokens(int64_t tokens, int experts, int features, int blocks, int sms) {
   const auto time = [&](const Variant& v, double out_blocks, double start) {
-    const int64_t used = std::min<int64_t>(experts, tokens);
-    const int64_t tiles = experts == 1 ? up(tokens, v.tokens) : std::max(used, tokens / v.tokens + used / 2);
-    return start + static_cast<double>(up(tiles * up(features, v.features), sms / v.ctas)) * (blocks + out_blocks) * 0.45;
+    return start + static_cast<double>(up(expected_tiles(tokens, experts, v.tokens) * up(features, v.features), sms / v.ctas)) * (blocks + out_blocks) * 0.45;
   };
-  return time(variant(MXB200_BLOCK_FORWARD, kMany), 4, 4.5) < time(variant(MXB200_BLOCK_FORWARD, kFew), 3, 4);
+  return time(variant(kForwardMany), 4, 4.5) < time(variant(kForwardFew), 3, 4);
 }
 
-int set_smem_once(const Variant& v, int device) {
+constexpr int kMostSplits = 8;
+
+// What the current device does with a kernel, looked up once: its shared memory, and how many clusters of 1 to 8 of its CTAs
+// find room at a time (a cluster stays within one of the GPU's groups of SMs: 15 clusters of 8, 33 of 4, 45 of 3).
+struct Configured {
+  bool done = false;
+  int clusters[kMostSplits + 1] = {};
+};
+
+int configure(VariantId id, const DeviceInfo& dev, Configured* out) {
   static std::mutex mu;
-  static const void* configured[64][5] = {};
+  static Configured known[64][kVariants];
   std::lock_guard<std::mutex> lock(mu);
-  const void* const kernel = reinterpret_cast<const void*>(v.kernel);
-  for (int i = 0; i < 5 && device < 64; ++i) {
-    if (configured[device][i] == kernel)
-      return MXB200_OK;
-    if (configured[device][i] == nullptr)
-      break;
-  }
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(v.smem)) != cudaSuccess) {
-    cudaGetLastError();
-    return MXB200_ERR_LAUNCH;
-  }
-  for (int i = 0; i < 5 && device < 64; ++i)
-    if (configured[device][i] == nullptr) {
-      configured[device][i] = kernel;
-      break;
+  Configured local;
+  Configured& c = dev.device < 64 ? known[dev.device][id] : local;
+  if (!c.done) {
+    const Variant& v = variant(id);
+    const void* const kernel = reinterpret_cast<const void*>(v.kernel);
+    bool ok = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(v.smem)) == cudaSuccess;
+    for (int n = 2; ok && v.ctas == 1 && n <= kMostSplits; ++n) {
+      cudaLaunchAttribute attribute{};
+      attribute.id = cudaLaunchAttributeClusterDimension;
+      attribute.val.clusterDim.x = n, attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+      cudaLaunchConfig_t config{};
+      config.gridDim = dim3(n), config.blockDim = dim3(kThreads), config.dynamicSmemBytes = v.smem;
+      config.attrs = &attribute, config.numAttrs = 1;
+      ok = cudaOccupancyMaxActiveClusters(&c.clusters[n], kernel, &config) == cudaSuccess;
     }
+    if (!ok) {
+      cudaGetLastError();
+      return MXB200_ERR_LAUNCH;
+    }
+    c.clusters[1] = dev.sms / v.ctas;
+    c.done = true;
+  }
+  *out = c;
   return MXB200_OK;
+}
+
+// CTAs that share a unit's blocks: what is expected to take least, among those of which all units' clusters find room at once. A
+// block takes a CTA about 0.3 us, the exchange 2 us and 0.02 for each of the tile's tokens: one token of 6144 -> 1536 takes 16 us
+// in one CTA per unit and 6.9 in eight, 128 tokens of 1536 -> 6144 8.4 in one and 10.8 in two.
+int share_blocks(int64_t units, int blocks, int tile_tokens, const Configured& c) {
+  int best = 1;
+  double least = 0.3 * blocks;
+  for (int n = 2; n <= std::min(kMostSplits, blocks) && units <= c.clusters[n]; ++n)
+    if (const double t = 0.3 * static_cast<double>(up(blocks, n)) + 2 + 0.02 * tile_tokens; t < least)
+      best = n, least = t;
+  return best;
 }
 
 int block_gemm(const mxb200_block_gemm_args& g, cudaStream_t stream) {
@@ -1026,6 +1262,10 @@ int block_gemm(const mxb200_block_gemm_args& g, cudaStream_t stream) {
   constexpr int64_t kMost = int64_t{1} << 30;
   if (g.tokens < 0 || g.tokens > kMost || g.in_features <= 0 || g.in_features > kMost || g.out_features <= 0 ||
       g.out_features > kMost || g.in_features % 16 || g.out_features % 16 || g.experts < 1 || g.experts > kMaxExperts)
+    return MXB200_ERR_SHAPE;
+  if (g.b_ld != 0 && g.kind != MXB200_BLOCK_FORWARD)
+    return MXB200_ERR_ARGUMENT;
+  if (g.b_ld != 0 && (g.b_ld < g.in_features || g.b_ld % 8 || g.tokens > MXB200_BLOCK_FEW_TOKENS))
     return MXB200_ERR_SHAPE;
   if (g.ends == nullptr && g.experts != 1)
     return MXB200_ERR_NULL;
@@ -1041,52 +1281,67 @@ int block_gemm(const mxb200_block_gemm_args& g, cudaStream_t stream) {
     const size_t bytes = static_cast<size_t>(g.experts) * g.out_features * g.in_features * (g.out_kind == MXB200_OUT_F32 ? 4 : 2);
     return cudaMemsetAsync(g.d, 0, bytes, stream) == cudaSuccess ? MXB200_OK : MXB200_ERR_LAUNCH;
   }
-  if (g.a == nullptr || g.a_scale == nullptr || g.b == nullptr || g.b_scale == nullptr || g.d == nullptr)
+  const bool quantize = g.b_ld != 0;
+  if (g.a == nullptr || g.a_scale == nullptr || g.b == nullptr || (g.b_scale == nullptr && !quantize) || g.d == nullptr)
     return MXB200_ERR_NULL;
   const auto bits = [](const void* q) { return reinterpret_cast<uintptr_t>(q); };
   if (!aligned16(g.a) || !aligned16(g.b) || !aligned16(g.d) || (bits(g.ends) & 3) != 0 ||
       ((bits(g.a_scale) | bits(g.b_scale)) & (wgrad ? 15 : 3)) != 0)
     return MXB200_ERR_ALIGNMENT;
   const int64_t in = g.in_features, out = g.out_features;
+  const bool forward = g.kind == MXB200_BLOCK_FORWARD;
+  const int from = static_cast<int>(forward ? in : out), to = static_cast<int>(forward ? out : in);
+  const int blocks = static_cast<int>(up(from, kBlock));
   Launch l{};
   Params& p = l.p;
   p.d = g.d, p.ends = g.ends, p.experts = g.experts, p.rows = static_cast<int>(g.tokens);
   p.out_bf16 = g.out_kind == MXB200_OUT_BF16;
-  const int from = static_cast<int>(g.kind == MXB200_BLOCK_FORWARD ? in : out), to = static_cast<int>(g.kind == MXB200_BLOCK_FORWARD ? out : in);
-  const bool many = !wgrad && many_tokens(g.tokens, g.experts, to, static_cast<int>(up(from, kBlock)), dev.sms);
-  const Variant& v = variant(g.kind, many ? kMany : kFew);
+  p.splits = 1;
+  VariantId id = kWeightGradPair;
+  Configured configured;
   int64_t units;
   int st;
   if (wgrad) {
+    if (st = configure(id, dev, &configured); st != MXB200_OK)
+      return st;
     const int64_t capacity = mxb200_block_token_blocks(g.tokens, g.experts) * kBlock;
     p.features = static_cast<int>(out), p.n = static_cast<int>(in);
-    units = g.experts * up(out, v.features) * up(in, v.features);
+    units = g.experts * up(out, wgrad::kTile) * up(in, wgrad::kTile);
     st = make_map(&l.maps.a, g.a, out, capacity, 1, 128);
     st = st != MXB200_OK ? st : make_map(&l.maps.b, g.b, in, capacity, 1, 128);
     st = st != MXB200_OK ? st : make_scale_map(&l.maps.a_scale, g.a_scale, out, capacity, 1);
     st = st != MXB200_OK ? st : make_scale_map(&l.maps.b_scale, g.b_scale, in, capacity, 2);
   } else {
-    const bool forward = g.kind == MXB200_BLOCK_FORWARD;
+    const bool many = !quantize && many_tokens(g.tokens, g.experts, to, blocks, dev.sms);
+    // at most half a small tile per expert expected, so that few experts need a second one
+    const bool small = g.tokens <= few::Tile32::kTileT || g.tokens <= int64_t{few::Tile32::kTileT} / 2 * g.experts;
+    id = quantize ? kForwardQuantizing : many ? (forward ? kForwardMany : kInputGradMany) : !forward ? kInputGradFew : small ? kForward32 : kForwardFew;
+    const Variant& v = variant(id);
     p.weight_scale = static_cast<const float*>(g.a_scale), p.token_scale = static_cast<const float*>(g.b_scale);
-    p.token_ld = g.tokens, p.features = to, p.blocks = static_cast<int>(up(from, kBlock));
+    p.token_ld = quantize ? g.b_ld : g.tokens, p.features = to, p.blocks = blocks;
+    p.input = g.b, p.input_cols = from;
     p.w_scale_expert = up(out, kBlock) * up(in, kBlock);
     p.w_scale_f = forward ? static_cast<int>(up(in, kBlock)) : 1, p.w_scale_b = forward ? 1 : static_cast<int>(up(in, kBlock));
     // token tiles are known on the device only; this many at most
     const int64_t token_tiles = g.ends == nullptr ? up(g.tokens, v.tokens)
                                                   : (g.tokens + (v.tokens - 1) * std::min<int64_t>(g.experts + 1, g.tokens)) / v.tokens;
     units = token_tiles * up(to, v.features);
+    if (st = configure(id, dev, &configured); st != MXB200_OK)
+      return st;
+    if (!many)
+      p.splits = share_blocks(expected_tiles(g.tokens, g.experts, v.tokens) * up(to, v.features), blocks,
+                              static_cast<int>(std::min<int64_t>(v.tokens, up(g.tokens, g.experts))), configured);
     CUtensorMap *weight = many ? &l.maps.b : &l.maps.a, *token = many ? &l.maps.a : &l.maps.b;
     st = make_map(weight, g.a, in, out, g.experts, 128);
-    st = st != MXB200_OK ? st : make_map(token, g.b, from, g.tokens, 1, many ? 128 : 32);
+    st = st != MXB200_OK || quantize ? st : make_map(token, g.b, from, g.tokens, 1, many ? 128 : 32);
   }
   if (st != MXB200_OK)
     return st;
   if (units > kMost)
     return MXB200_ERR_SHAPE;
-  if (st = set_smem_once(v, dev.device); st != MXB200_OK)
-    return st;
-  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(units, dev.sms / v.ctas)) * v.ctas;
-  return launch_kernel(v.kernel, grid, kThreads, v.smem, stream, l);
+  const Variant& v = variant(id);
+  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(units, configured.clusters[p.splits])) * std::max(v.ctas, p.splits);
+  return launch_kernel_clusters(p.splits > 1 ? p.splits : 0, v.kernel, grid, kThreads, v.smem, stream, l);
 }
 
 }  // namespace

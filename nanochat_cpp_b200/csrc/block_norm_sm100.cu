@@ -4,8 +4,9 @@
 //   d = dn gain,  hat = res rstd,  dx = bf16(rstd (d - hat mean(d hat)) + dres)  (of x and of r),  dgain = sum over rows of dn hat
 //
 // A row lies in the registers of its threads from load to store, so every tensor is read or written once; both kernels are
-// bound by memory. A row of up to 2048 columns belongs to one warp, whose sums are shuffles, a wider one (up to 16384) to 256
-// threads. 16 lanes hold 128 consecutive values, one scale block. Sums, rstd and the gain's gradient are fp32.
+// bound by memory. Forward: a row of up to 2048 columns belongs to one warp, whose sums are shuffles, a wider one (up to 16384)
+// to 256 threads; 16 lanes hold 128 consecutive values, one scale block. Backward: a block's threads own columns and go through
+// its rows, several at a time. Sums, rstd and the gain's gradient are fp32.
 //
 // The gain's gradient: every CTA adds up its rows in a fixed order in registers and writes one row of partial sums; a second
 // kernel adds those rows in order. No atomics: the same bits every time.
@@ -175,93 +176,94 @@ __device__ __forceinline__ void norm_forward(const ForwardParams& p) {
   }
 }
 
-template <int kPerRow, int kVecs>
+// A block's threads own columns (8 kVecs each) and go through its rows kRows at a time, so that the gain's sums of a thread are
+// few and its loads many. One barrier per step: the rows' sums of one step are gathered while the other half of `parts` may still
+// be read.
+template <int kVecs, int kRows>
 __device__ __forceinline__ void norm_backward(const BackwardParams& p) {
-  __shared__ float parts[kThreads / 32];
-  __shared__ __align__(16) float gathered[kPerRow == 32 ? kWarpCols : 4];
+  __shared__ float parts[2][kRows][kThreads / 32];
   grid_dependency_wait();
-  constexpr int kRows = kThreads / kPerRow;
-  const int at = threadIdx.x % kPerRow;
-  float dgain[kVecs][8];
+  const int threads = blockDim.x, warps = threads / 32, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  float gain[kVecs][8], dgain[kVecs][8];
 #pragma unroll
-  for (int i = 0; i < kVecs; ++i)
+  for (int i = 0; i < kVecs; ++i) {
+    const int col = 8 * (i * threads + threadIdx.x);
 #pragma unroll
     for (int k = 0; k < 8; ++k)
-      dgain[i][k] = 0.f;
-  for (int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / kPerRow; row < p.rows;
-       row += static_cast<int64_t>(gridDim.x) * kRows) {
-    uint4 v[kVecs], d[kVecs];
-    const float rstd = p.rstd[row];
+      gain[i][k] = 1.f, dgain[i][k] = 0.f;
+    if (col < p.cols)
+      load_gain(p.gain, p.gain_bf16, col, gain[i]);
+  }
+  int half = 0;
+  for (int64_t row = static_cast<int64_t>(blockIdx.x) * kRows; row < p.rows; row += static_cast<int64_t>(gridDim.x) * kRows, half ^= 1) {
+    uint4 v[kRows][kVecs], d[kRows][kVecs], o[kRows][kVecs];
+    float rstd[kRows], sum[kRows];
 #pragma unroll
-    for (int i = 0; i < kVecs; ++i) {
-      const int col = 8 * (i * kPerRow + at);
-      v[i] = col < p.cols ? load16(p.res, row * p.cols + col) : make_uint4(0, 0, 0, 0);
-      d[i] = col < p.cols ? load16(p.dn, row * p.cols + col) : make_uint4(0, 0, 0, 0);
-    }
-    float sum = 0.f;
+    for (int r = 0; r < kRows; ++r) {
+      const bool there = row + r < p.rows;
+      rstd[r] = there ? p.rstd[row + r] : 0.f;
 #pragma unroll
-    for (int i = 0; i < kVecs; ++i) {
-      const int col = 8 * (i * kPerRow + at);
-      float f[8], h[8], g[8];
-      unpack(v[i], h);
-      unpack(d[i], f);
-      if (col < p.cols) {
-        load_gain(p.gain, p.gain_bf16, col, g);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const float t = f[k] * (h[k] * rstd);
-          dgain[i][k] += t;
-          sum = fmaf(t, g[k], sum);
-        }
+      for (int i = 0; i < kVecs; ++i) {
+        const int col = 8 * (i * threads + threadIdx.x);
+        const int64_t at = (row + r) * p.cols + col;
+        const bool in = there && col < p.cols;
+        v[r][i] = in ? load16(p.res, at) : make_uint4(0, 0, 0, 0);
+        d[r][i] = in ? load16(p.dn, at) : make_uint4(0, 0, 0, 0);
+        o[r][i] = in && p.dres != nullptr ? load16(p.dres, at) : make_uint4(0, 0, 0, 0);
       }
     }
-    const float mean = row_sum<kPerRow>(sum, parts) / static_cast<float>(p.cols);
 #pragma unroll
-    for (int i = 0; i < kVecs; ++i) {
-      const int col = 8 * (i * kPerRow + at);
-      if (col >= p.cols)
-        continue;
-      float f[8], h[8], g[8], o[8];
-      unpack(v[i], h);
-      unpack(d[i], f);
-      load_gain(p.gain, p.gain_bf16, col, g);
-      if (p.dres != nullptr)
-        unpack(load16(p.dres, row * p.cols + col), o);
+    for (int r = 0; r < kRows; ++r) {
+      sum[r] = 0.f;
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
-        f[k] = rstd * (f[k] * g[k] - h[k] * rstd * mean) + (p.dres != nullptr ? o[k] : 0.f);
-      store16(p.dx, row * p.cols + col, pack(f));
+      for (int i = 0; i < kVecs; ++i) {
+        float f[8], h[8];
+        unpack(v[r][i], h);
+        unpack(d[r][i], f);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float t = f[k] * (h[k] * rstd[r]);
+          dgain[i][k] += t;
+          sum[r] = fmaf(t, gain[i][k], sum[r]);
+        }
+      }
+#pragma unroll
+      for (int s = 16; s > 0; s >>= 1)
+        sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], s);
+      if (lane == 0)
+        parts[half][r][warp] = sum[r];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      float mean = 0.f;
+      for (int w = 0; w < warps; ++w)
+        mean += parts[half][r][w];
+      mean /= static_cast<float>(p.cols);
+#pragma unroll
+      for (int i = 0; i < kVecs; ++i) {
+        const int col = 8 * (i * threads + threadIdx.x);
+        float f[8], h[8], e[8];
+        unpack(v[r][i], h);
+        unpack(d[r][i], f);
+        unpack(o[r][i], e);
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          f[k] = rstd[r] * (f[k] * gain[i][k] - h[k] * rstd[r] * mean) + e[k];
+        if (row + r < p.rows && col < p.cols)
+          store16(p.dx, (row + r) * p.cols + col, pack(f));
+      }
     }
   }
   if (p.partial == nullptr)
     return;
-  if constexpr (kPerRow == 32) {
-    // the warps' sums, one warp after the other
-    for (int w = 0; w < kRows; ++w) {
-      if (threadIdx.x / 32 == w) {
 #pragma unroll
-        for (int i = 0; i < kVecs; ++i) {
-          const int col = 8 * (i * 32 + at);
-          if (col < p.cols) {
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-              gathered[col + k] = (w == 0 ? 0.f : gathered[col + k]) + dgain[i][k];
-          }
-        }
-      }
-      __syncthreads();
-    }
-    for (int c = threadIdx.x; c < p.cols; c += kThreads)
-      p.partial[static_cast<int64_t>(blockIdx.x) * p.cols + c] = gathered[c];
-  } else {
-#pragma unroll
-    for (int i = 0; i < kVecs; ++i) {
-      const int col = 8 * (i * kPerRow + at);
-      if (col < p.cols) {
-        float4* out = reinterpret_cast<float4*>(p.partial + static_cast<int64_t>(blockIdx.x) * p.cols + col);
-        out[0] = make_float4(dgain[i][0], dgain[i][1], dgain[i][2], dgain[i][3]);
-        out[1] = make_float4(dgain[i][4], dgain[i][5], dgain[i][6], dgain[i][7]);
-      }
+  for (int i = 0; i < kVecs; ++i) {
+    const int col = 8 * (i * threads + threadIdx.x);
+    if (col < p.cols) {
+      float4* out = reinterpret_cast<float4*>(p.partial + static_cast<int64_t>(blockIdx.x) * p.cols + col);
+      out[0] = make_float4(dgain[i][0], dgain[i][1], dgain[i][2], dgain[i][3]);
+      out[1] = make_float4(dgain[i][4], dgain[i][5], dgain[i][6], dgain[i][7]);
     }
   }
 }
@@ -270,20 +272,25 @@ __device__ __forceinline__ void norm_backward(const BackwardParams& p) {
 }  // namespace mxb200
 
 // kVecs: 8-value vectors per thread
-#define MXB200_NORM_KERNELS(per_row, vecs)                                                                                            \
+#define MXB200_NORM_KERNEL(per_row, vecs)                                                                                             \
   __global__ void __launch_bounds__(mxb200::kThreads) mxb200_block_norm_##per_row##x##vecs(const __grid_constant__ mxb200::ForwardParams p) { \
     mxb200::norm_forward<per_row, vecs>(p);                                                                                           \
-  }                                                                                                                                   \
-  __global__ void __launch_bounds__(mxb200::kThreads) mxb200_block_norm_bwd_##per_row##x##vecs(const __grid_constant__ mxb200::BackwardParams p) { \
-    mxb200::norm_backward<per_row, vecs>(p);                                                                                          \
   }
-MXB200_NORM_KERNELS(32, 2)
-MXB200_NORM_KERNELS(32, 4)
-MXB200_NORM_KERNELS(32, 6)
-MXB200_NORM_KERNELS(32, 8)
-MXB200_NORM_KERNELS(256, 2)
-MXB200_NORM_KERNELS(256, 4)
-MXB200_NORM_KERNELS(256, 8)
+#define MXB200_NORM_BACKWARD_KERNEL(vecs, rows)                                                                                       \
+  __global__ void __launch_bounds__(mxb200::kThreads) mxb200_block_norm_bwd_##vecs##x##rows(const __grid_constant__ mxb200::BackwardParams p) { \
+    mxb200::norm_backward<vecs, rows>(p);                                                                                             \
+  }
+MXB200_NORM_KERNEL(32, 2)
+MXB200_NORM_KERNEL(32, 4)
+MXB200_NORM_KERNEL(32, 6)
+MXB200_NORM_KERNEL(32, 8)
+MXB200_NORM_KERNEL(256, 2)
+MXB200_NORM_KERNEL(256, 4)
+MXB200_NORM_KERNEL(256, 8)
+MXB200_NORM_BACKWARD_KERNEL(1, 4)
+MXB200_NORM_BACKWARD_KERNEL(2, 2)
+MXB200_NORM_BACKWARD_KERNEL(4, 1)
+MXB200_NORM_BACKWARD_KERNEL(8, 1)
 
 // The rows of partial sums, in order: 32 columns and 8 interleaved shares of the rows per block.
 __global__ void __launch_bounds__(256) mxb200_block_norm_sum_gain(const float* partial, int parts, int cols, void* out, int out_bf16) {
@@ -312,29 +319,46 @@ namespace {
 
 constexpr int64_t kMost = int64_t{1} << 30;
 
-struct Variant {
-  void (*forward)(ForwardParams);
-  void (*backward)(BackwardParams);
+struct Forward {
+  void (*kernel)(ForwardParams);
   int rows_per_block;
 };
 
 // One warp per row as long as its registers hold it (64 values per lane), then the whole block.
-Variant variant(int cols) {
+Forward forward_of(int cols) {
   const int vecs = cols / 8;
   if (cols <= kWarpCols) {
     if (vecs <= 64)
-      return {mxb200_block_norm_32x2, mxb200_block_norm_bwd_32x2, kThreads / 32};
+      return {mxb200_block_norm_32x2, kThreads / 32};
     if (vecs <= 128)
-      return {mxb200_block_norm_32x4, mxb200_block_norm_bwd_32x4, kThreads / 32};
+      return {mxb200_block_norm_32x4, kThreads / 32};
     if (vecs <= 192)
-      return {mxb200_block_norm_32x6, mxb200_block_norm_bwd_32x6, kThreads / 32};
-    return {mxb200_block_norm_32x8, mxb200_block_norm_bwd_32x8, kThreads / 32};
+      return {mxb200_block_norm_32x6, kThreads / 32};
+    return {mxb200_block_norm_32x8, kThreads / 32};
   }
   if (vecs <= 512)
-    return {mxb200_block_norm_256x2, mxb200_block_norm_bwd_256x2, 1};
+    return {mxb200_block_norm_256x2, 1};
   if (vecs <= 1024)
-    return {mxb200_block_norm_256x4, mxb200_block_norm_bwd_256x4, 1};
-  return {mxb200_block_norm_256x8, mxb200_block_norm_bwd_256x8, 1};
+    return {mxb200_block_norm_256x4, 1};
+  return {mxb200_block_norm_256x8, 1};
+}
+
+struct Backward {
+  void (*kernel)(BackwardParams);
+  int threads, rows_per_step, blocks_per_sm;
+};
+
+// As many threads as a row has vectors of 8, up to 256, then more vectors per thread.
+Backward backward_of(int cols) {
+  const int vecs = cols / 8;
+  const int threads = std::min(kThreads, (vecs + 31) / 32 * 32);
+  if (vecs <= kThreads)
+    return {mxb200_block_norm_bwd_1x4, threads, 4, std::min(8, 768 / threads)};
+  if (vecs <= 2 * kThreads)
+    return {mxb200_block_norm_bwd_2x2, threads, 2, 2};
+  if (vecs <= 4 * kThreads)
+    return {mxb200_block_norm_bwd_4x1, threads, 1, 2};
+  return {mxb200_block_norm_bwd_8x1, threads, 1, 1};
 }
 
 int check_shape(int64_t rows, int32_t cols) {
@@ -353,9 +377,9 @@ int check_pointers(std::initializer_list<const void*> needed, std::initializer_l
   return MXB200_OK;
 }
 
-// CTAs of the backward: two for each SM, fewer where there are not the rows
-int64_t backward_blocks(int64_t rows, int rows_per_block, int sms) {
-  return std::max<int64_t>(1, std::min<int64_t>((rows + rows_per_block - 1) / rows_per_block, 2 * sms));
+// CTAs of the backward: one round of what the SMs hold, fewer where there are not the rows
+int64_t backward_blocks(int64_t rows, const Backward& v, int sms) {
+  return std::max<int64_t>(1, std::min<int64_t>((rows + v.rows_per_step - 1) / v.rows_per_step, static_cast<int64_t>(v.blocks_per_sm) * sms));
 }
 
 }  // namespace
@@ -376,10 +400,10 @@ extern "C" int mxb200_block_norm_fwd(const mxb200_block_norm_args* a, void* stre
     return st;
   if ((a->r == nullptr) != (a->res == nullptr))
     return MXB200_ERR_ARGUMENT;
-  const Variant v = variant(a->cols);
+  const Forward v = forward_of(a->cols);
   const ForwardParams p{a->x, a->r, a->gain, a->res, a->n, static_cast<uint8_t*>(a->q), a->scale, a->rstd,
                         a->rows, a->cols, a->gain_bf16, a->eps};
-  return launch_kernel(v.forward, static_cast<unsigned>((a->rows + v.rows_per_block - 1) / v.rows_per_block), kThreads, 0,
+  return launch_kernel(v.kernel, static_cast<unsigned>((a->rows + v.rows_per_block - 1) / v.rows_per_block), kThreads, 0,
                        static_cast<cudaStream_t>(stream), p);
 }
 
@@ -388,7 +412,7 @@ extern "C" size_t mxb200_block_norm_workspace_bytes(int64_t rows, int32_t cols) 
   DeviceInfo dev;
   if (check_shape(rows, cols) != MXB200_OK || current_device(&dev) != MXB200_OK)
     return 0;
-  return static_cast<size_t>(backward_blocks(rows, variant(cols).rows_per_block, dev.sms)) * cols * sizeof(float);
+  return static_cast<size_t>(backward_blocks(rows, backward_of(cols), dev.sms)) * cols * sizeof(float);
 }
 
 extern "C" int mxb200_block_norm_bwd(const mxb200_block_norm_bwd_args* a, void* workspace, size_t workspace_bytes, void* stream) {
@@ -412,11 +436,11 @@ extern "C" int mxb200_block_norm_bwd(const mxb200_block_norm_bwd_args* a, void* 
     return MXB200_ERR_ARGUMENT;
   if (a->dgain != nullptr && (workspace == nullptr || workspace_bytes < mxb200_block_norm_workspace_bytes(a->rows, a->cols)))
     return MXB200_ERR_WORKSPACE;
-  const Variant v = variant(a->cols);
-  const int blocks = static_cast<int>(backward_blocks(a->rows, v.rows_per_block, dev.sms));
+  const Backward v = backward_of(a->cols);
+  const int blocks = static_cast<int>(backward_blocks(a->rows, v, dev.sms));
   float* partial = a->dgain != nullptr ? static_cast<float*>(workspace) : nullptr;
   const BackwardParams p{a->dn, a->dres, a->res, a->rstd, a->gain, a->dx, partial, a->rows, a->cols, a->gain_bf16};
-  if (int st = launch_kernel(v.backward, static_cast<unsigned>(blocks), kThreads, 0, s, p); st != MXB200_OK || partial == nullptr)
+  if (int st = launch_kernel(v.kernel, static_cast<unsigned>(blocks), v.threads, 0, s, p); st != MXB200_OK || partial == nullptr)
     return st;
   return launch_kernel(mxb200_block_norm_sum_gain, static_cast<unsigned>((a->cols + 31) / 32), 256, 0, s,
                        static_cast<const float*>(partial), blocks, static_cast<int>(a->cols), a->dgain, static_cast<int>(a->gain_bf16));

@@ -47,19 +47,22 @@ inline int launch_status() {
 // Launches a kernel of this library, all of which begin with grid_dependency_wait() (ptx_sm100.cuh): its blocks may be
 // placed while the stream's previous kernel still runs, as that one's leave their SMs, and wait there for its end with
 // their set-up done. That takes 1 to 2 us of launch latency and ramp-up out of every step of a chain of small kernels.
+// cluster > 0: CTAs of a cluster, for kernels that do not fix it themselves.
 template <typename... Params>
-int launch_kernel(void (*kernel)(Params...), dim3 grid, unsigned block, size_t smem, cudaStream_t stream,
-                  const Params&... params) {
-  cudaLaunchAttribute attribute{};
-  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attribute.val.programmaticStreamSerializationAllowed = 1;
+int launch_kernel_clusters(unsigned cluster, void (*kernel)(Params...), dim3 grid, unsigned block, size_t smem, cudaStream_t stream,
+                           const Params&... params) {
+  cudaLaunchAttribute attributes[2] = {};
+  attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attributes[0].val.programmaticStreamSerializationAllowed = 1;
+  attributes[1].id = cudaLaunchAttributeClusterDimension;
+  attributes[1].val.clusterDim.x = cluster, attributes[1].val.clusterDim.y = attributes[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t config{};
   config.gridDim = grid;
   config.blockDim = dim3(block);
   config.dynamicSmemBytes = smem;
   config.stream = stream;
-  config.attrs = &attribute;
-  config.numAttrs = 1;
+  config.attrs = attributes;
+  config.numAttrs = cluster > 0 ? 2 : 1;
   void* arguments[] = {const_cast<void*>(static_cast<const void*>(&params))...};
   g_launches.fetch_add(1, std::memory_order_relaxed);
   if (cudaLaunchKernelExC(&config, reinterpret_cast<const void*>(kernel), arguments) != cudaSuccess) {
@@ -67,6 +70,12 @@ int launch_kernel(void (*kernel)(Params...), dim3 grid, unsigned block, size_t s
     return MXB200_ERR_LAUNCH;
   }
   return MXB200_OK;
+}
+
+template <typename... Params>
+int launch_kernel(void (*kernel)(Params...), dim3 grid, unsigned block, size_t smem, cudaStream_t stream,
+                  const Params&... params) {
+  return launch_kernel_clusters(0, kernel, grid, block, smem, stream, params...);
 }
 
 }  // namespace mxb200

@@ -1038,7 +1038,15 @@ Tensor readable_rows(const Tensor& x) {
 
 void block_product(int kind, const Block& a, const Block& b, const Tensor& d, const Experts& e, int64_t tokens, int64_t in, int64_t out) {
   const mxb200_block_gemm_args g{a.data.data_ptr(), a.scale.data_ptr(), b.data.data_ptr(), b.scale.data_ptr(), d.data_ptr(), e.ends, tokens, in, out, e.count, kind,
-                                 d.scalar_type() == at::kFloat ? MXB200_OUT_F32 : MXB200_OUT_BF16};
+                                 d.scalar_type() == at::kFloat ? MXB200_OUT_F32 : MXB200_OUT_BF16, 0};
+  check(mxb200_block_gemm(&g, stream()), "block_gemm");
+}
+
+// The forward product of so few tokens that it quantizes them itself rather than wait for a launch that does: one token of 1536
+// features takes 10.4 us in two launches and KQ1 in one, 32 tokens KQ32A and KQ32B.
+void block_product_of(const Tensor& x, const Block& w, const Tensor& y, const Experts& e, int64_t tokens, int64_t in, int64_t out) {
+  const mxb200_block_gemm_args g{w.data.data_ptr(), w.scale.data_ptr(), x.data_ptr(), nullptr, y.data_ptr(), e.ends, tokens, in, out,
+                                 e.count, MXB200_BLOCK_FORWARD, MXB200_OUT_BF16, tokens > 1 ? x.stride(0) : in};
   check(mxb200_block_gemm(&g, stream()), "block_gemm");
 }
 
@@ -1095,7 +1103,8 @@ struct BlockLinear : torch::autograd::Function<BlockLinear> {
     const bool grad_x = ctx != nullptr && c.x.defined() && c.x.requires_grad();
     const Experts e = c.experts();
     Block tokens;
-    if (!c.x_rows.data.defined()) {
+    const bool by_product = !grad_w && !c.ends.defined() && !c.x_rows.data.defined() && c.tokens <= MXB200_BLOCK_FEW_TOKENS;
+    if (!c.x_rows.data.defined() && !by_product) {
       c.x_rows = empty_row_blocks(c.tokens, c.in, c.device);
       if (grad_w)
         tokens = empty_token_blocks(c.tokens, c.in, e, c.device);
@@ -1104,7 +1113,10 @@ struct BlockLinear : torch::autograd::Function<BlockLinear> {
     if (!c.w_blocks.data.defined())
       c.w_blocks = quantize_weight_blocks(c.w);
     const Tensor y = empty({c.tokens, c.out}, at::kBFloat16, c.device);
-    block_product(MXB200_BLOCK_FORWARD, c.w_blocks, c.x_rows, y, e, c.tokens, c.in, c.out);
+    if (by_product)
+      block_product_of(readable_rows(c.x), c.w_blocks, y, e, c.tokens, c.in, c.out);
+    else
+      block_product(MXB200_BLOCK_FORWARD, c.w_blocks, c.x_rows, y, e, c.tokens, c.in, c.out);
     if (ctx != nullptr) {
       const Tensor none;
       ctx->save_for_backward({grad_x ? c.w_blocks.data : none, grad_x ? c.w_blocks.scale : none, tokens.data, tokens.scale,

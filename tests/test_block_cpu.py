@@ -12,7 +12,7 @@ PTR = 1 << 20  # any aligned address: refused calls never follow it
 
 def gemm(**change):
     a = dict(a=PTR, a_scale=PTR, b=PTR, b_scale=PTR, d=PTR, ends=None, tokens=8, in_features=128, out_features=128, experts=1,
-             kind=capi.BLOCK_FORWARD, out_kind=capi.OUT_BF16)
+             kind=capi.BLOCK_FORWARD, out_kind=capi.OUT_BF16, b_ld=0)
     a.update(change)
     args = capi.BlockGemmArgs(*(a[f[0]] for f in capi.BlockGemmArgs._fields_))
     return lib.mxb200_block_gemm(ctypes.byref(args), None)
@@ -24,6 +24,8 @@ def gemm(**change):
     (dict(tokens=-1), capi.ERR_SHAPE), (dict(tokens=1 << 31), capi.ERR_SHAPE), (dict(in_features=0), capi.ERR_SHAPE),
     (dict(in_features=24), capi.ERR_SHAPE), (dict(out_features=8), capi.ERR_SHAPE), (dict(experts=0), capi.ERR_SHAPE),
     (dict(experts=1025, ends=PTR), capi.ERR_SHAPE), (dict(experts=2), capi.ERR_NULL),
+    (dict(b_ld=128, kind=capi.BLOCK_INPUT_GRAD), capi.ERR_ARGUMENT), (dict(b_ld=112), capi.ERR_SHAPE), (dict(b_ld=132), capi.ERR_SHAPE),
+    (dict(b_ld=128, tokens=33), capi.ERR_SHAPE),
 ])
 def test_gemm_refusals(change, status):
     assert gemm(**change) == status

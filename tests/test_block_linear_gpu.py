@@ -99,6 +99,27 @@ def test_forward(nc, tokens, cin, cout):
     assert torch.equal(y, again)
 
 
+@pytest.mark.parametrize("tokens", [1, 5, 8, 17, 31, 32])
+@pytest.mark.parametrize("cin,cout", [(16, 16), (144, 272), (1536, 1536), (2064, 400), (6144, 128)])
+def test_quantized_by_the_product(nc, tokens, cin, cout):
+    """The C entry that takes bf16 rows: the bits of quantizing first, dense and by expert."""
+    import ctypes
+    g, capi = generator(16), nc.capi
+    x, w = activation(g, tokens, 2 * cin), given_weight(nc, g, 2, cout, cin)
+    x[0, 0], x[-1, 3] = float("nan"), float("inf")
+    for experts, ends in ((1, None), (2, ends_of([tokens // 3, tokens // 2]))):
+        data, scale = w.data[:experts].contiguous(), w.scale[:experts].contiguous()
+        got = torch.full((tokens, cout), 7.0, device="cuda", dtype=torch.bfloat16)
+        args = capi.BlockGemmArgs(data.data_ptr(), scale.data_ptr(), x.data_ptr(), None, got.data_ptr(),
+                                  ends.data_ptr() if ends is not None else None, tokens, cin, cout, experts, capi.BLOCK_FORWARD,
+                                  capi.OUT_BF16, 2 * cin)
+        capi.check(capi.lib.mxb200_block_gemm(ctypes.byref(args), torch.cuda.current_stream().cuda_stream), "block_gemm")
+        q, weight = nc.quantize_block(x[:, :cin]), nc.BlockTensor(data, scale)
+        want = nc.fp8_block_experts(None, weight, ends, x_block=q) if experts > 1 else nc.fp8_block_matmul(
+            None, nc.BlockTensor(data[0], scale[0]), x_block=q)
+        assert torch.equal(torch.nan_to_num(got, nan=1e9), torch.nan_to_num(want, nan=1e9))
+
+
 @pytest.mark.parametrize("tokens", [1, 16, 129, 384, 1000])
 @pytest.mark.parametrize("cin,cout", [(16, 16), (272, 144), (128, 640), (1040, 2000)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
