@@ -84,6 +84,20 @@ __device__ __forceinline__ uint32_t e4m3x4_scaled_fma(uint32_t w0, uint32_t w1, 
   return d;
 }
 
+// The same with a multiplier for each of the four values, packed as they are.
+__device__ __forceinline__ uint32_t e4m3x4_scaled_each(uint32_t w0, uint32_t w1, uint32_t m0, uint32_t m1) {
+  uint32_t d;
+  asm("{\n\t.reg .b16 a0, a1, b0, b1, s0, s1, t0, t1, lo, hi;\n\t.reg .f32 f0, f1, f2, f3;\n\t"
+      "mov.b32 {a0, a1}, %1;\n\tmov.b32 {b0, b1}, %2;\n\tmov.b32 {s0, s1}, %3;\n\tmov.b32 {t0, t1}, %4;\n\t"
+      "fma.rn.f32.bf16 f0, a0, s0, 0f80000000;\n\tfma.rn.f32.bf16 f1, a1, s1, 0f80000000;\n\t"
+      "fma.rn.f32.bf16 f2, b0, t0, 0f80000000;\n\tfma.rn.f32.bf16 f3, b1, t1, 0f80000000;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f32 lo, f1, f0;\n\tcvt.rn.satfinite.e4m3x2.f32 hi, f3, f2;\n\t"
+      "mov.b32 %0, {lo, hi};\n\t}\n"
+      : "=r"(d)
+      : "r"(w0), "r"(w1), "r"(m0), "r"(m1));
+  return d;
+}
+
 // Four packed words holding two interleaved series (low halves, high halves): the e4m3 of the four low halves times
 // mlo and of the four high halves times mhi, each as one word.
 __device__ __forceinline__ void e4m3x4_scaled_fma_split(uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3, uint16_t mlo,

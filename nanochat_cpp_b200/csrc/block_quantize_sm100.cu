@@ -8,7 +8,7 @@
 // count in the maximum and stays NaN; Inf saturates to 448 s.
 //
 // All three work on 128 x 128 tiles, 256 threads: 16 lanes hold a row's 128 values, 8 each, and a thread 8 rows 16 apart, all
-// loaded before the first is used. A row's maximum is a shuffle over 16 lanes, a column's goes through shared memory. Bound by
+// loaded before the first is used. A row's maximum is taken by shuffles over 16 lanes, a column's through shared memory. Bound by
 // memory: 2 bytes read and 1 written per value and layout; both layouts of an activation come from one read. Data never leaves
 // transposed, since the matrix product reads either orientation.
 #include <algorithm>
@@ -86,17 +86,29 @@ __device__ __forceinline__ void load_tile(const void* x, int64_t at, int64_t ld,
   }
 }
 
-// One block of rows at a time, all its column tiles with a stride of gridDim.y.
-template <bool kBf16, bool kRows, bool kTokens>
-__device__ __forceinline__ void quantize_activation(const QuantizeParams& p, int* first_row, int* first_tile, int* tmp, float (*partial)[kBlock]) {
+// What the threads of a block share of an activation's tile.
+struct TileShared {
+  uint16_t row_by[kBlock];                                  // bf16 multipliers of the tile's rows; a warp reads its own rows' only
+  float row_scale[kBlock];
+  __align__(16) uint32_t col_max[kThreads / 32][kBlock / 2];  // packed bf16: the warps' maxima of two columns
+  __align__(16) uint32_t col_by[kBlock / 2];                  // packed bf16 multipliers of two columns
+};
+
+__device__ __forceinline__ uint16_t by_of(int exponent) {
+  return static_cast<uint16_t>(mx_multiplier_bits(exponent) >> 16);
+}
+
+// A block of rows at a time, its column tiles with a stride of gridDim.y. The values stay packed bf16: maxima by
+// max.xorsign.abs.bf16x2, the product with the scale's reciprocal (a power of two, a bf16 number) by fma.rn.f32.bf16.
+template <bool kRows, bool kTokens>
+__device__ __forceinline__ void quantize_activation(const QuantizeParams& p, TileShared* s, int* first_row, int* first_tile, int* tmp) {
   grid_dependency_wait();
-  const int lane16 = threadIdx.x & 15, row = threadIdx.x >> 4;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, lane16 = lane & 15, row = threadIdx.x >> 4;
   int64_t row0 = static_cast<int64_t>(blockIdx.x) * kBlock;
   int rows_left;
   if constexpr (kTokens) {
     scan_experts(p.ends, p.experts, static_cast<int>(p.rows), kBlock, first_row, first_tile, tmp);
-    const int blocks = first_tile[p.experts];
-    if (static_cast<int>(blockIdx.x) >= blocks)
+    if (static_cast<int>(blockIdx.x) >= first_tile[p.experts])
       return;
     const int e = expert_of_tile(first_tile, p.experts, blockIdx.x);
     const int r = first_row[e] + (static_cast<int>(blockIdx.x) - first_tile[e]) * kBlock;
@@ -105,84 +117,92 @@ __device__ __forceinline__ void quantize_activation(const QuantizeParams& p, int
   } else {
     rows_left = static_cast<int>(min(static_cast<int64_t>(kBlock), p.rows - row0));
   }
+  const __nv_bfloat16* x = static_cast<const __nv_bfloat16*>(p.x) + (row0 + row) * p.ld;
   const int tiles = static_cast<int>((p.cols + kBlock - 1) / kBlock);
   for (int t = blockIdx.y; t < tiles; t += gridDim.y) {
     const int64_t col = static_cast<int64_t>(t) * kBlock + 8 * lane16;
     const bool col_ok = col < p.cols;
-    Values v[kRowsPerThread];
-    load_tile<kBf16>(p.x, (row0 + row) * p.ld + col, p.ld, row, rows_left, col_ok, v);
-    if constexpr (kRows) {
+    uint4 v[kRowsPerThread];
+#pragma unroll
+    for (int i = 0; i < kRowsPerThread; ++i)
+      v[i] = col_ok && row + 16 * i < rows_left ? *reinterpret_cast<const uint4*>(x + 16 * i * p.ld + col) : make_uint4(0, 0, 0, 0);
+    if constexpr (kTokens) {
+      uint32_t m[4] = {0, 0, 0, 0};
 #pragma unroll
       for (int i = 0; i < kRowsPerThread; ++i) {
-        float m = 0.f;
+        m[0] = max_abs_skip_nan_bf16x2(m[0], v[i].x), m[1] = max_abs_skip_nan_bf16x2(m[1], v[i].y);
+        m[2] = max_abs_skip_nan_bf16x2(m[2], v[i].z), m[3] = max_abs_skip_nan_bf16x2(m[3], v[i].w);
+      }
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-          m = fmaxf(m, fabsf(v[i].v[k]));
+      for (int k = 0; k < 4; ++k)
+        m[k] = max_abs_skip_nan_bf16x2(m[k], __shfl_xor_sync(0xffffffffu, m[k], 16));
+      if (lane < 16)
+        *reinterpret_cast<uint4*>(&s->col_max[warp][4 * lane]) = make_uint4(m[0], m[1], m[2], m[3]);
+    }
+    if constexpr (kRows) {
+      // eight rows' maxima over 16 lanes: each exchange halves the rows that a lane goes on with
+      uint32_t m[kRowsPerThread];
 #pragma unroll
-        for (int d = 8; d > 0; d >>= 1)
-          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-        const int e = exponent_of(m);
-        const float f = multiplier_of(e);
-        const int64_t r = row0 + row + 16 * i;
-        if (row + 16 * i < rows_left) {
-          if (col_ok)
-            *reinterpret_cast<uint2*>(p.row_data + r * p.cols + col) =
-                  make_uint2(e4m3x4_from_f32(v[i].v[0] * f, v[i].v[1] * f, v[i].v[2] * f, v[i].v[3] * f),
-                             e4m3x4_from_f32(v[i].v[4] * f, v[i].v[5] * f, v[i].v[6] * f, v[i].v[7] * f));
-          if (lane16 == 0)
-            p.row_scale[static_cast<int64_t>(t) * p.rows + r] = scale_of(e);
+      for (int i = 0; i < kRowsPerThread; ++i) {
+        const uint32_t w = max_abs_skip_nan_bf16x2(max_abs_skip_nan_bf16x2(max_abs_skip_nan_bf16x2(max_abs_skip_nan_bf16x2(0u, v[i].x), v[i].y), v[i].z), v[i].w) & 0x7fff7fffu;
+        m[i] = max(w & 0xffffu, w >> 16);
+      }
+#pragma unroll
+      for (int n = 4, d = 8; n > 0; n >>= 1, d >>= 1) {
+        const bool upper = (lane & d) != 0;
+#pragma unroll
+        for (int i = 0; i < n; ++i) {
+          const uint32_t sent = upper ? m[i] : m[i + n], kept = upper ? m[i + n] : m[i];
+          m[i] = max(kept, __shfl_xor_sync(0xffffffffu, sent, d));
         }
       }
+      m[0] = max(m[0], __shfl_xor_sync(0xffffffffu, m[0], 1));
+      const int e = block_exponent(m[0] << 16);
+      // lanes with bit 0 clear: row i of this half warp, i from lane bits 3, 2, 1
+      const int i = ((lane >> 3) & 1) * 4 + ((lane >> 2) & 1) * 2 + ((lane >> 1) & 1);
+      __syncwarp();  // the previous tile's multipliers have been read
+      if ((lane & 1) == 0)
+        s->row_by[row + 16 * i] = by_of(e), s->row_scale[row + 16 * i] = scale_of(e);
+      __syncwarp();
+#pragma unroll
+      for (int k = 0; k < kRowsPerThread; ++k)
+        if (col_ok && row + 16 * k < rows_left) {
+          const uint16_t by = s->row_by[row + 16 * k];
+          *reinterpret_cast<uint2*>(p.row_data + (row0 + row + 16 * k) * p.cols + col) =
+                make_uint2(e4m3x4_scaled_fma(v[k].x, v[k].y, by, by), e4m3x4_scaled_fma(v[k].z, v[k].w, by, by));
+        }
     }
+    __syncthreads();
+    if (kRows && threadIdx.x < rows_left)
+      p.row_scale[static_cast<int64_t>(t) * p.rows + row0 + threadIdx.x] = s->row_scale[threadIdx.x];
     if constexpr (kTokens) {
-      float m[8];
+      if (threadIdx.x < kBlock / 2) {
+        uint32_t m = s->col_max[0][threadIdx.x];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        m[k] = 0.f;
+        for (int w = 1; w < kThreads / 32; ++w)
+          m = max_abs_skip_nan_bf16x2(m, s->col_max[w][threadIdx.x]);
+        m &= 0x7fff7fffu;
+        const int e[2] = {block_exponent(m << 16), block_exponent(m & 0xffff0000u)};
+        s->col_by[threadIdx.x] = by_of(e[0]) | static_cast<uint32_t>(by_of(e[1])) << 16;
+        // a tile of 128 columns' scale bytes, each four times, in the order that the copy to tensor memory takes
+        uint32_t* words = p.col_scale_words + (static_cast<int64_t>(blockIdx.x) * tiles + t) * kBlock;
 #pragma unroll
-        for (int i = 0; i < kRowsPerThread; ++i)
-          m[k] = fmaxf(m[k], fabsf(v[i].v[k]));
-        m[k] = fmaxf(m[k], __shfl_xor_sync(0xffffffffu, m[k], 16));
-      }
-      __syncthreads();  // the previous tile's maxima have been read
-      if ((threadIdx.x & 16) == 0) {
-        float4* dst = reinterpret_cast<float4*>(&partial[threadIdx.x >> 5][8 * lane16]);
-        dst[0] = make_float4(m[0], m[1], m[2], m[3]);
-        dst[1] = make_float4(m[4], m[5], m[6], m[7]);
+        for (int k = 0; k < 2; ++k) {
+          const int c = 2 * threadIdx.x + k;
+          words[(c & 31) * 4 + (c >> 5)] = static_cast<uint32_t>(e[k]) * 0x01010101u;
+        }
       }
       __syncthreads();
-      float f[8];
-      int e[8];
-#pragma unroll
-      for (int k = 0; k < 8; ++k)
-        m[k] = 0.f;
-#pragma unroll
-      for (int w = 0; w < kThreads / 32; ++w) {
-        const float4* src = reinterpret_cast<const float4*>(&partial[w][8 * lane16]);
-        const float4 a = src[0], b = src[1];
-        m[0] = fmaxf(m[0], a.x), m[1] = fmaxf(m[1], a.y), m[2] = fmaxf(m[2], a.z), m[3] = fmaxf(m[3], a.w);
-        m[4] = fmaxf(m[4], b.x), m[5] = fmaxf(m[5], b.y), m[6] = fmaxf(m[6], b.z), m[7] = fmaxf(m[7], b.w);
-      }
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        e[k] = exponent_of(m[k]);
-        f[k] = multiplier_of(e[k]);
-      }
       if (col_ok) {
-        const int64_t out0 = static_cast<int64_t>(blockIdx.x) * kBlock + row;
+        const uint4 by = *reinterpret_cast<const uint4*>(&s->col_by[4 * lane16]);
+        uint8_t* out = p.col_data + (static_cast<int64_t>(blockIdx.x) * kBlock + row) * p.cols + col;
 #pragma unroll
-        for (int i = 0; i < kRowsPerThread; ++i)  // rows that do not exist are zeros: they count in the product
-          *reinterpret_cast<uint2*>(p.col_data + (out0 + 16 * i) * p.cols + col) =
-                make_uint2(e4m3x4_from_f32(v[i].v[0] * f[0], v[i].v[1] * f[1], v[i].v[2] * f[2], v[i].v[3] * f[3]),
-                           e4m3x4_from_f32(v[i].v[4] * f[4], v[i].v[5] * f[5], v[i].v[6] * f[6], v[i].v[7] * f[7]));
+        for (int k = 0; k < kRowsPerThread; ++k)  // rows that do not exist are zeros: they count in the product
+          *reinterpret_cast<uint2*>(out + 16 * k * p.cols) =
+                make_uint2(e4m3x4_scaled_each(v[k].x, v[k].y, by.x, by.y), e4m3x4_scaled_each(v[k].z, v[k].w, by.z, by.w));
       }
-      // a tile of 128 columns' scale bytes, each four times, in the order that the copy to tensor memory takes
-      const int c = 8 * lane16 + row;
-#pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (row == k)
-          p.col_scale_words[(static_cast<int64_t>(blockIdx.x) * tiles + t) * kBlock + (c & 31) * 4 + (c >> 5)] =
-                static_cast<uint32_t>(e[k]) * 0x01010101u;
+    } else if (gridDim.y < tiles) {
+      __syncthreads();  // the scales have been read
     }
   }
 }
@@ -230,17 +250,18 @@ __device__ __forceinline__ void quantize_weight(const QuantizeParams& p, float* 
 }  // namespace mxb200
 
 __global__ void __launch_bounds__(mxb200::kThreads) mxb200_block_quantize_rows(const __grid_constant__ mxb200::QuantizeParams p) {
-  mxb200::quantize_activation<true, true, false>(p, nullptr, nullptr, nullptr, nullptr);
+  __shared__ mxb200::TileShared s;
+  mxb200::quantize_activation<true, false>(p, &s, nullptr, nullptr, nullptr);
 }
 
 template <bool kRows>
 __device__ __forceinline__ void quantize_tokens(const mxb200::QuantizeParams& p) {
   __shared__ int first_row[mxb200::kMaxExperts + 1], first_tile[mxb200::kMaxExperts + 1];
-  __shared__ __align__(16) union {
+  __shared__ union {
     int tmp[mxb200::kMaxExperts];
-    float partial[mxb200::kThreads / 32][mxb200::kBlock];
+    mxb200::TileShared tile;
   } u;
-  mxb200::quantize_activation<true, kRows, true>(p, first_row, first_tile, u.tmp, u.partial);
+  mxb200::quantize_activation<kRows, true>(p, &u.tile, first_row, first_tile, u.tmp);
 }
 
 __global__ void __launch_bounds__(mxb200::kThreads) mxb200_block_quantize_tokens(const __grid_constant__ mxb200::QuantizeParams p) {
