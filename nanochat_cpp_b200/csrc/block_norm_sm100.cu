@@ -119,14 +119,18 @@ __device__ __forceinline__ void norm_forward(const ForwardParams& p) {
     v[i] = col < p.cols ? load16(p.x, row * p.cols + col) : make_uint4(0, 0, 0, 0);
   }
   if (p.r != nullptr) {
+    uint4 r[kVecs];  // all on their way before the first store
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) {
       const int col = 8 * (i * kPerRow + at);
-      if (col < p.cols) {
-        const uint4 r = load16(p.r, row * p.cols + col);
-        v[i] = make_uint4(add_bf16x2(v[i].x, r.x), add_bf16x2(v[i].y, r.y), add_bf16x2(v[i].z, r.z), add_bf16x2(v[i].w, r.w));
+      r[i] = col < p.cols ? load16(p.r, row * p.cols + col) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) {
+      const int col = 8 * (i * kPerRow + at);
+      v[i] = make_uint4(add_bf16x2(v[i].x, r[i].x), add_bf16x2(v[i].y, r[i].y), add_bf16x2(v[i].z, r[i].z), add_bf16x2(v[i].w, r[i].w));
+      if (col < p.cols)
         store16(p.res, row * p.cols + col, v[i]);
-      }
     }
   }
   float sum = 0.f;
@@ -194,65 +198,87 @@ __device__ __forceinline__ void norm_backward(const BackwardParams& p) {
     if (col < p.cols)
       load_gain(p.gain, p.gain_bf16, col, gain[i]);
   }
-  int half = 0;
-  for (int64_t row = static_cast<int64_t>(blockIdx.x) * kRows; row < p.rows; row += static_cast<int64_t>(gridDim.x) * kRows, half ^= 1) {
-    uint4 v[kRows][kVecs], d[kRows][kVecs], o[kRows][kVecs];
-    float rstd[kRows], sum[kRows];
+  // the next step's rows are on their way while this one's are worked on, as long as registers hold them
+  constexpr bool kAhead = kVecs < 8;
+  uint4 v[1 + kAhead][kRows][kVecs], d[1 + kAhead][kRows][kVecs], o[1 + kAhead][kRows][kVecs];
+  float rstd[1 + kAhead][kRows];
+  const auto load = [&](int64_t row, int to) {
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
       const bool there = row + r < p.rows;
-      rstd[r] = there ? p.rstd[row + r] : 0.f;
+      rstd[to][r] = there ? p.rstd[row + r] : 0.f;
 #pragma unroll
       for (int i = 0; i < kVecs; ++i) {
         const int col = 8 * (i * threads + threadIdx.x);
         const int64_t at = (row + r) * p.cols + col;
         const bool in = there && col < p.cols;
-        v[r][i] = in ? load16(p.res, at) : make_uint4(0, 0, 0, 0);
-        d[r][i] = in ? load16(p.dn, at) : make_uint4(0, 0, 0, 0);
-        o[r][i] = in && p.dres != nullptr ? load16(p.dres, at) : make_uint4(0, 0, 0, 0);
+        v[to][r][i] = in ? load16(p.res, at) : make_uint4(0, 0, 0, 0);
+        d[to][r][i] = in ? load16(p.dn, at) : make_uint4(0, 0, 0, 0);
+        o[to][r][i] = in && p.dres != nullptr ? load16(p.dres, at) : make_uint4(0, 0, 0, 0);
       }
     }
+  };
+  const auto work = [&](int64_t row, int at) {
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-      sum[r] = 0.f;
+      float sum = 0.f;
 #pragma unroll
       for (int i = 0; i < kVecs; ++i) {
         float f[8], h[8];
-        unpack(v[r][i], h);
-        unpack(d[r][i], f);
+        unpack(v[at][r][i], h);
+        unpack(d[at][r][i], f);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          const float t = f[k] * (h[k] * rstd[r]);
+          const float t = f[k] * (h[k] * rstd[at][r]);
           dgain[i][k] += t;
-          sum[r] = fmaf(t, gain[i][k], sum[r]);
+          sum = fmaf(t, gain[i][k], sum);
         }
       }
 #pragma unroll
       for (int s = 16; s > 0; s >>= 1)
-        sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], s);
+        sum += __shfl_xor_sync(0xffffffffu, sum, s);
       if (lane == 0)
-        parts[half][r][warp] = sum[r];
+        parts[at][r][warp] = sum;
     }
     __syncthreads();
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
       float mean = 0.f;
       for (int w = 0; w < warps; ++w)
-        mean += parts[half][r][w];
+        mean += parts[at][r][w];
       mean /= static_cast<float>(p.cols);
 #pragma unroll
       for (int i = 0; i < kVecs; ++i) {
         const int col = 8 * (i * threads + threadIdx.x);
         float f[8], h[8], e[8];
-        unpack(v[r][i], h);
-        unpack(d[r][i], f);
-        unpack(o[r][i], e);
+        unpack(v[at][r][i], h);
+        unpack(d[at][r][i], f);
+        unpack(o[at][r][i], e);
 #pragma unroll
         for (int k = 0; k < 8; ++k)
-          f[k] = rstd[r] * (f[k] * gain[i][k] - h[k] * rstd[r] * mean) + e[k];
+          f[k] = rstd[at][r] * (f[k] * gain[i][k] - h[k] * rstd[at][r] * mean) + e[k];
         if (row + r < p.rows && col < p.cols)
           store16(p.dx, (row + r) * p.cols + col, pack(f));
       }
+    }
+  };
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
+  int64_t row = static_cast<int64_t>(blockIdx.x) * kRows;
+  if constexpr (kAhead) {
+    load(row, 0);
+    for (; row < p.rows; row += 2 * step) {
+      load(row + step, 1);
+      work(row, 0);
+      if (row + step >= p.rows)
+        break;
+      load(row + 2 * step, 0);
+      work(row + step, 1);
+    }
+  } else {
+    for (; row < p.rows; row += step) {
+      load(row, 0);
+      work(row, 0);
+      __syncthreads();  // the rows' sums have been read
     }
   }
   if (p.partial == nullptr)
@@ -287,27 +313,29 @@ MXB200_NORM_KERNEL(32, 8)
 MXB200_NORM_KERNEL(256, 2)
 MXB200_NORM_KERNEL(256, 4)
 MXB200_NORM_KERNEL(256, 8)
-MXB200_NORM_BACKWARD_KERNEL(1, 4)
-MXB200_NORM_BACKWARD_KERNEL(2, 2)
+MXB200_NORM_BACKWARD_KERNEL(1, 2)
+MXB200_NORM_BACKWARD_KERNEL(2, 1)
 MXB200_NORM_BACKWARD_KERNEL(4, 1)
 MXB200_NORM_BACKWARD_KERNEL(8, 1)
 
-// The rows of partial sums, in order: 32 columns and 8 interleaved shares of the rows per block.
-__global__ void __launch_bounds__(256) mxb200_block_norm_sum_gain(const float* partial, int parts, int cols, void* out, int out_bf16) {
-  __shared__ float share[8][32];
+// The rows of partial sums: 32 columns per block, whose 32 warps each add every 32nd row in order, then the warps' sums in order.
+__global__ void __launch_bounds__(1024) mxb200_block_norm_sum_gain(const float* partial, int parts, int cols, void* out, int out_bf16) {
+  __shared__ float share[32][32];
   mxb200::grid_dependency_wait();
-  const int c = blockIdx.x * 32 + (threadIdx.x & 31), g = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31, c = blockIdx.x * 32 + lane, g = threadIdx.x >> 5;
   float sum = 0.f;
-  if (c < cols)
-    for (int i = g; i < parts; i += 8)
+  if (c < cols) {
+#pragma unroll 4
+    for (int i = g; i < parts; i += 32)
       sum += partial[static_cast<int64_t>(i) * cols + c];
-  share[g][threadIdx.x & 31] = sum;
+  }
+  share[g][lane] = sum;
   __syncthreads();
   if (g != 0 || c >= cols)
     return;
 #pragma unroll
-  for (int i = 1; i < 8; ++i)
-    sum += share[i][threadIdx.x & 31];
+  for (int i = 1; i < 32; ++i)
+    sum += share[i][lane];
   if (out_bf16)
     static_cast<__nv_bfloat16*>(out)[c] = __float2bfloat16_rn(sum);
   else
@@ -351,14 +379,14 @@ struct Backward {
 // As many threads as a row has vectors of 8, up to 256, then more vectors per thread.
 Backward backward_of(int cols) {
   const int vecs = cols / 8;
-  const int threads = std::min(kThreads, (vecs + 31) / 32 * 32);
+  const auto threads = [&](int per_thread) { return ((vecs + per_thread - 1) / per_thread + 31) / 32 * 32; };
   if (vecs <= kThreads)
-    return {mxb200_block_norm_bwd_1x4, threads, 4, std::min(8, 768 / threads)};
+    return {mxb200_block_norm_bwd_1x2, threads(1), 2, std::min(8, 768 / threads(1))};
   if (vecs <= 2 * kThreads)
-    return {mxb200_block_norm_bwd_2x2, threads, 2, 2};
+    return {mxb200_block_norm_bwd_2x1, threads(2), 1, 2};
   if (vecs <= 4 * kThreads)
-    return {mxb200_block_norm_bwd_4x1, threads, 1, 2};
-  return {mxb200_block_norm_bwd_8x1, threads, 1, 1};
+    return {mxb200_block_norm_bwd_4x1, threads(4), 1, 2};
+  return {mxb200_block_norm_bwd_8x1, threads(8), 1, 1};
 }
 
 int check_shape(int64_t rows, int32_t cols) {
@@ -442,6 +470,6 @@ extern "C" int mxb200_block_norm_bwd(const mxb200_block_norm_bwd_args* a, void* 
   const BackwardParams p{a->dn, a->dres, a->res, a->rstd, a->gain, a->dx, partial, a->rows, a->cols, a->gain_bf16};
   if (int st = launch_kernel(v.kernel, static_cast<unsigned>(blocks), v.threads, 0, s, p); st != MXB200_OK || partial == nullptr)
     return st;
-  return launch_kernel(mxb200_block_norm_sum_gain, static_cast<unsigned>((a->cols + 31) / 32), 256, 0, s,
+  return launch_kernel(mxb200_block_norm_sum_gain, static_cast<unsigned>((a->cols + 31) / 32), 1024, 0, s,
                        static_cast<const float*>(partial), blocks, static_cast<int>(a->cols), a->dgain, static_cast<int>(a->gain_bf16));
 }
