@@ -996,36 +996,56 @@ bool block_features(int64_t n) {
   return n > 0 && n % 16 == 0;
 }
 
-// E4M3 values and their fp32 scales; `like` in Python's BlockTensor.
+// E4M3 values and their scales by address, and what keeps them. Tensors that nobody outside sees are one byte buffer: data, then
+// scales.
 struct Block {
-  Tensor data, scale;
+  Tensor hold, hold_scale;
+  void* data = nullptr;
+  void* scale = nullptr;
+  explicit operator bool() const { return hold.defined(); }
 };
 
-using GivenBlock = std::optional<std::pair<Tensor, Tensor>>;
+constexpr int64_t up16(int64_t n) {
+  return (n + 15) / 16 * 16;
+}
 
-// Tokens' operands: (rows, cols) values in blocks along rows, and in blocks along each expert's tokens.
+Block in_buffer(Tensor buffer, int64_t data_bytes) {
+  auto* p = static_cast<unsigned char*>(buffer.data_ptr());
+  return {std::move(buffer), Tensor(), p, p + up16(data_bytes)};
+}
+
+Block new_block(int64_t data_bytes, int64_t scales, at::Device device) {
+  return in_buffer(empty({up16(data_bytes) + 4 * scales}, at::kByte, device), data_bytes);
+}
+
+Block of_tensors(const Tensor& data, const Tensor& scale) {
+  return {data, scale, data.data_ptr(), scale.data_ptr()};
+}
+
+// Rows sorted by expert, or all one's.
 struct Experts {
   const int32_t* ends = nullptr;
   int count = 1;
 };
 
-Block empty_row_blocks(int64_t rows, int64_t cols, at::Device device) {
-  return {empty({rows, cols}, kE4M3, device), empty({blocks_of(cols), rows}, at::kFloat, device)};
+// (rows, cols) in blocks along rows, and in blocks along each expert's tokens.
+Block new_row_blocks(int64_t rows, int64_t cols, at::Device device) {
+  return new_block(rows * cols, blocks_of(cols) * rows, device);
 }
 
-Block empty_token_blocks(int64_t rows, int64_t cols, const Experts& e, at::Device device) {
-  const int64_t blocks = mxb200_block_token_blocks(rows, e.count);
-  return {empty({128 * blocks, cols}, kE4M3, device), empty({blocks, blocks_of(cols), 128}, at::kInt, device)};
+int64_t token_bytes(int64_t rows, int64_t cols, const Experts& e) {
+  return 128 * mxb200_block_token_blocks(rows, e.count) * cols;
+}
+
+Block new_token_blocks(int64_t rows, int64_t cols, const Experts& e, at::Device device) {
+  return new_block(token_bytes(rows, cols, e), mxb200_block_token_blocks(rows, e.count) * blocks_of(cols) * 128, device);
 }
 
 // x (rows, cols) bf16 with contiguous columns into either layout or both.
-void quantize_blocks(const Tensor& x, const Experts& e, const Block* rows, const Block* tokens) {
+void quantize_blocks(const Tensor& x, const Experts& e, const Block& rows, const Block& tokens) {
   const int64_t ld = x.size(0) > 1 ? x.stride(0) : x.size(1);
-  check(mxb200_block_quantize(x.data_ptr(), x.size(0), x.size(1), ld, e.ends, e.count,
-                              rows != nullptr ? rows->data.data_ptr() : nullptr,
-                              rows != nullptr ? static_cast<float*>(rows->scale.data_ptr()) : nullptr,
-                              tokens != nullptr ? tokens->data.data_ptr() : nullptr,
-                              tokens != nullptr ? static_cast<uint32_t*>(tokens->scale.data_ptr()) : nullptr, stream()),
+  check(mxb200_block_quantize(x.data_ptr(), x.size(0), x.size(1), ld, e.ends, e.count, rows.data, static_cast<float*>(rows.scale), tokens.data,
+                              static_cast<uint32_t*>(tokens.scale), stream()),
         "quantize_block");
 }
 
@@ -1037,38 +1057,41 @@ Tensor readable_rows(const Tensor& x) {
 }
 
 void block_product(int kind, const Block& a, const Block& b, const Tensor& d, const Experts& e, int64_t tokens, int64_t in, int64_t out) {
-  const mxb200_block_gemm_args g{a.data.data_ptr(), a.scale.data_ptr(), b.data.data_ptr(), b.scale.data_ptr(), d.data_ptr(), e.ends, tokens, in, out, e.count, kind,
+  const mxb200_block_gemm_args g{a.data, a.scale, b.data, b.scale, d.data_ptr(), e.ends, tokens, in, out, e.count, kind,
                                  d.scalar_type() == at::kFloat ? MXB200_OUT_F32 : MXB200_OUT_BF16, 0};
   check(mxb200_block_gemm(&g, stream()), "block_gemm");
 }
 
 // The forward product of so few tokens that it quantizes them itself rather than wait for a launch that does: one token of 1536
-// features takes 10.4 us in two launches and KQ1 in one, 32 tokens KQ32A and KQ32B.
+// features to 1536 takes 8.5 us in two launches and 6.2 in one.
 void block_product_of(const Tensor& x, const Block& w, const Tensor& y, const Experts& e, int64_t tokens, int64_t in, int64_t out) {
-  const mxb200_block_gemm_args g{w.data.data_ptr(), w.scale.data_ptr(), x.data_ptr(), nullptr, y.data_ptr(), e.ends, tokens, in, out,
-                                 e.count, MXB200_BLOCK_FORWARD, MXB200_OUT_BF16, tokens > 1 ? x.stride(0) : in};
+  const mxb200_block_gemm_args g{w.data, w.scale, x.data_ptr(), nullptr, y.data_ptr(), e.ends, tokens, in, out, e.count,
+                                 MXB200_BLOCK_FORWARD, MXB200_OUT_BF16, tokens > 1 ? x.stride(0) : in};
   check(mxb200_block_gemm(&g, stream()), "block_gemm");
 }
 
-Block quantize_weight_blocks(const Tensor& w_in) {
+void quantize_weight(const Tensor& w_in, const Block& to) {
   const Tensor w = dense(w_in.detach());
-  const int64_t e = w.dim() == 3 ? w.size(0) : 1, n = w.size(-2), k = w.size(-1);
-  std::vector<int64_t> scales{blocks_of(n), blocks_of(k)};
-  if (w.dim() == 3)
-    scales.insert(scales.begin(), e);
-  const Block q{empty(w.sizes(), kE4M3, w.device()), empty(scales, at::kFloat, w.device())};
-  check(mxb200_block_quantize_weight(w.data_ptr(), w.scalar_type() == at::kBFloat16, static_cast<int>(e), n, k, q.data.data_ptr(),
-                                     static_cast<float*>(q.scale.data_ptr()), stream()),
+  check(mxb200_block_quantize_weight(w.data_ptr(), w.scalar_type() == at::kBFloat16, static_cast<int>(w.dim() == 3 ? w.size(0) : 1),
+                                     w.size(-2), w.size(-1), to.data, static_cast<float*>(to.scale), stream()),
         "quantize_block_weight");
-  return q;
+}
+
+[[noreturn]] void fail_in(const char* what, const char* message) {
+  throw std::runtime_error(std::string(what) + ": " + message);
+}
+
+inline void require_in(bool ok, const char* what, const char* message) {
+  if (!ok)
+    fail_in(what, message);
 }
 
 // A Linear's operands, checked.
 struct BlockLinearCall {
   Tensor x;        // undefined where only its blocks are given
   Tensor w;        // undefined where only its blocks are given
-  Block x_rows;    // undefined: to be made
-  Block w_blocks;  // undefined: to be made
+  Block x_rows;    // empty: to be made
+  Block w_blocks;  // empty: to be made
   Tensor ends;     // undefined: dense
   int64_t tokens = 0, in = 0, out = 0;
   at::Device device = at::kCPU;
@@ -1078,21 +1101,11 @@ struct BlockLinearCall {
   }
 };
 
-[[noreturn]] void fail_in(const char* what, const char* message) {
-  throw std::runtime_error(std::string(what) + ": " + message);
-}
-
-void require_in(bool ok, const char* what, const char* message) {
-  if (!ok)
-    fail_in(what, message);
-}
-
-Block given_block(const std::pair<Tensor, Tensor>& q, at::IntArrayRef data, at::IntArrayRef scale, at::Device device, const char* what) {
-  for (const Tensor* t : {&q.first, &q.second})
-    require_in(t->device() == device, what, "expected quantized operands on the input's device");
-  require_in(q.first.scalar_type() == kE4M3 && q.second.scalar_type() == at::kFloat, what, "expected e4m3 data with fp32 scales");
-  require_in(q.first.sizes() == data && q.second.sizes() == scale, what, "shape mismatch");
-  return {dense(q.first), q.second.contiguous()};
+Block given_block(const Tensor& data, const Tensor& scale, at::IntArrayRef sizes, at::IntArrayRef scales, at::Device device, const char* what) {
+  require_in(data.device() == device && scale.device() == device, what, "expected quantized operands on the input's device");
+  require_in(data.scalar_type() == kE4M3 && scale.scalar_type() == at::kFloat, what, "expected e4m3 data with fp32 scales");
+  require_in(data.sizes() == sizes && scale.sizes() == scales, what, "shape mismatch");
+  return of_tensors(dense(data), scale.contiguous());
 }
 
 struct BlockLinear : torch::autograd::Function<BlockLinear> {
@@ -1103,15 +1116,18 @@ struct BlockLinear : torch::autograd::Function<BlockLinear> {
     const bool grad_x = ctx != nullptr && c.x.defined() && c.x.requires_grad();
     const Experts e = c.experts();
     Block tokens;
-    const bool by_product = !grad_w && !c.ends.defined() && !c.x_rows.data.defined() && c.tokens <= MXB200_BLOCK_FEW_TOKENS;
-    if (!c.x_rows.data.defined() && !by_product) {
-      c.x_rows = empty_row_blocks(c.tokens, c.in, c.device);
+    const bool by_product = !grad_w && !c.ends.defined() && !c.x_rows && c.tokens <= MXB200_BLOCK_FEW_TOKENS;
+    if (!c.x_rows && !by_product) {
+      c.x_rows = new_row_blocks(c.tokens, c.in, c.device);
       if (grad_w)
-        tokens = empty_token_blocks(c.tokens, c.in, e, c.device);
-      quantize_blocks(readable_rows(c.x), grad_w ? e : Experts{}, &c.x_rows, grad_w ? &tokens : nullptr);
+        tokens = new_token_blocks(c.tokens, c.in, e, c.device);
+      quantize_blocks(readable_rows(c.x), grad_w ? e : Experts{}, c.x_rows, tokens);
     }
-    if (!c.w_blocks.data.defined())
-      c.w_blocks = quantize_weight_blocks(c.w);
+    if (!c.w_blocks) {
+      const int64_t matrices = c.w.dim() == 3 ? c.w.size(0) : 1;
+      c.w_blocks = new_block(matrices * c.out * c.in, matrices * blocks_of(c.out) * blocks_of(c.in), c.device);
+      quantize_weight(c.w, c.w_blocks);
+    }
     const Tensor y = empty({c.tokens, c.out}, at::kBFloat16, c.device);
     if (by_product)
       block_product_of(readable_rows(c.x), c.w_blocks, y, e, c.tokens, c.in, c.out);
@@ -1119,15 +1135,10 @@ struct BlockLinear : torch::autograd::Function<BlockLinear> {
       block_product(MXB200_BLOCK_FORWARD, c.w_blocks, c.x_rows, y, e, c.tokens, c.in, c.out);
     if (ctx != nullptr) {
       const Tensor none;
-      ctx->save_for_backward({grad_x ? c.w_blocks.data : none, grad_x ? c.w_blocks.scale : none, tokens.data, tokens.scale,
-                              grad_w && !tokens.data.defined() ? c.x : none, c.ends});
-      ctx->saved_data["tokens"] = c.tokens;
-      ctx->saved_data["in"] = c.in;
-      ctx->saved_data["out"] = c.out;
-      if (c.w.defined()) {
-        ctx->saved_data["w_sizes"] = c.w.sizes().vec();
-        ctx->saved_data["w_dtype"] = c.w.scalar_type();
-      }
+      ctx->save_for_backward({grad_x ? c.w_blocks.hold : none, grad_x ? c.w_blocks.hold_scale : none, tokens.hold,
+                              grad_w && !tokens ? c.x : none, c.ends});
+      const bool bf16 = grad_w && c.w.scalar_type() == at::kBFloat16;
+      ctx->saved_data["sizes"] = std::vector<int64_t>{c.tokens, c.in, c.out, c.ends.defined() ? c.ends.numel() : 0, bf16};
     }
     return y;
   }
@@ -1140,59 +1151,62 @@ struct BlockLinear : torch::autograd::Function<BlockLinear> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     require(!at::GradMode::is_enabled(), "block linear: its backward has no derivative (create_graph)");
     const auto saved = ctx->get_saved_variables();
-    const int64_t tokens = ctx->saved_data["tokens"].toInt(), in = ctx->saved_data["in"].toInt(), out = ctx->saved_data["out"].toInt();
+    const auto sizes = ctx->saved_data["sizes"].toIntVector();
+    const int64_t tokens = sizes[0], in = sizes[1], out = sizes[2], matrices = sizes[3];
     const Tensor go = readable_rows(grads[0]);
     const auto device = go.device();
-    BlockLinearCall c;
-    c.ends = saved[5];
-    const Experts e = c.experts();
-    const bool grad_x = saved[0].defined(), grad_w = saved[2].defined() || saved[4].defined();
+    const Experts e = matrices > 0 ? Experts{static_cast<const int32_t*>(saved[4].data_ptr()), static_cast<int>(matrices)} : Experts{};
+    const bool grad_x = saved[0].defined(), grad_w = saved[2].defined() || saved[3].defined();
     Block g_rows, g_tokens;
     if (grad_x)
-      g_rows = empty_row_blocks(tokens, out, device);
+      g_rows = new_row_blocks(tokens, out, device);
     if (grad_w)
-      g_tokens = empty_token_blocks(tokens, out, e, device);
+      g_tokens = new_token_blocks(tokens, out, e, device);
     if (grad_x || grad_w)
-      quantize_blocks(go, grad_w ? e : Experts{}, grad_x ? &g_rows : nullptr, grad_w ? &g_tokens : nullptr);
+      quantize_blocks(go, grad_w ? e : Experts{}, g_rows, g_tokens);
     Tensor dx, dw;
     if (grad_w) {
-      Block x_tokens{saved[2], saved[3]};
-      if (!x_tokens.data.defined()) {
-        x_tokens = empty_token_blocks(tokens, in, e, device);
-        quantize_blocks(readable_rows(saved[4]), e, nullptr, &x_tokens);
+      Block x_tokens;
+      if (saved[2].defined()) {
+        x_tokens = in_buffer(saved[2], token_bytes(tokens, in, e));
+      } else {
+        x_tokens = new_token_blocks(tokens, in, e, device);
+        quantize_blocks(readable_rows(saved[3]), e, Block{}, x_tokens);
       }
       // bf16 weights: rounded once in the epilogue, as the cast of an fp32 result would round it
-      dw = empty(ctx->saved_data["w_sizes"].toIntVector(), ctx->saved_data["w_dtype"].toScalarType(), device);
+      const auto dtype = sizes[4] != 0 ? at::kBFloat16 : at::kFloat;
+      dw = matrices > 0 ? empty({matrices, out, in}, dtype, device) : empty({out, in}, dtype, device);
       block_product(MXB200_BLOCK_WEIGHT_GRAD, g_tokens, x_tokens, dw, e, tokens, in, out);
     }
     if (grad_x) {
       dx = empty({tokens, in}, at::kBFloat16, device);
-      block_product(MXB200_BLOCK_INPUT_GRAD, {saved[0], saved[1]}, g_rows, dx, e, tokens, in, out);
+      const Block w = saved[1].defined() ? of_tensors(saved[0], saved[1]) : in_buffer(saved[0], (matrices > 0 ? matrices : 1) * out * in);
+      block_product(MXB200_BLOCK_INPUT_GRAD, w, g_rows, dx, e, tokens, in, out);
     }
     return {dx, dw, Tensor()};
   }
 };
 
-Tensor block_linear(const std::optional<Tensor>& x, const std::optional<Tensor>& w, const GivenBlock& x_block, const GivenBlock& w_block,
-                    const std::optional<Tensor>& ends, const char* what) {
-  require_in(x.has_value() || x_block.has_value(), what, "expected an input");
-  require_in(w.has_value() || w_block.has_value(), what, "expected a weight");
-  const Tensor& first = x.has_value() ? *x : x_block->first;
+using MaybeTensor = std::optional<Tensor>;
+
+Tensor block_linear(const MaybeTensor& x, const MaybeTensor& w, const MaybeTensor& x_data, const MaybeTensor& x_scale,
+                    const MaybeTensor& w_data, const MaybeTensor& w_scale, const Tensor* ends, const char* what) {
+  require_in(x.has_value() || x_data.has_value(), what, "expected an input");
+  require_in(w.has_value() || w_data.has_value(), what, "expected a weight");
+  const Tensor& first = x.has_value() ? *x : *x_data;
   require_cuda(first, what);
-  const Tensor& weight = w.has_value() ? *w : w_block->first;
-  require_in(first.dim() == 2 && weight.dim() == (ends.has_value() ? 3 : 2) && first.size(1) == weight.size(-1), what, "shape mismatch");
+  const Tensor& weight = w.has_value() ? *w : *w_data;
+  require_in(first.dim() == 2 && weight.dim() == (ends != nullptr ? 3 : 2) && first.size(1) == weight.size(-1), what, "shape mismatch");
   BlockLinearCall c;
   c.device = first.device();
   c.tokens = first.size(0), c.in = first.size(1), c.out = weight.size(-2);
   require_in(block_features(c.in) && block_features(c.out), what, "in and out features must be multiples of 16");
   require_in(weight.device() == c.device, what, "expected the weight on the input's device");
-  std::vector<int64_t> w_scale{blocks_of(c.out), blocks_of(c.in)};
-  if (ends.has_value()) {
+  if (ends != nullptr) {
     require_in(ends->device() == c.device && ends->scalar_type() == at::kInt && ends->dim() == 1 && ends->is_contiguous() &&
                      ends->numel() == weight.size(0) && ends->numel() >= 1 && ends->numel() <= 1024,
                what, "ends must be int32 on the input's device, one per expert, 1 to 1024 of them");
     c.ends = *ends;
-    w_scale.insert(w_scale.begin(), weight.size(0));
   }
   if (x.has_value()) {
     require_in(x->scalar_type() == at::kBFloat16, what, "expected a bf16 input");
@@ -1202,11 +1216,13 @@ Tensor block_linear(const std::optional<Tensor>& x, const std::optional<Tensor>&
     require_in(w->scalar_type() == at::kBFloat16 || w->scalar_type() == at::kFloat, what, "expected a bf16 or fp32 weight");
     c.w = *w;
   }
-  if (x_block.has_value())
-    c.x_rows = given_block(*x_block, {c.tokens, c.in}, {blocks_of(c.in), c.tokens}, c.device, what);
-  if (w_block.has_value())
-    c.w_blocks = given_block(*w_block, weight.sizes(), w_scale, c.device, what);
-  const Tensor none;
+  if (x_data.has_value())
+    c.x_rows = given_block(*x_data, x_scale.value(), {c.tokens, c.in}, {blocks_of(c.in), c.tokens}, c.device, what);
+  if (w_data.has_value()) {
+    const int64_t scales[3] = {ends != nullptr ? weight.size(0) : 1, blocks_of(c.out), blocks_of(c.in)};
+    c.w_blocks = given_block(*w_data, w_scale.value(), weight.sizes(), ends != nullptr ? at::IntArrayRef(scales, 3) : at::IntArrayRef(scales + 1, 2),
+                             c.device, what);
+  }
   bool grad = false;
   for (const Tensor* t : {&c.x, &c.w})
     if (t->defined())
@@ -1225,9 +1241,9 @@ std::pair<Tensor, Tensor> quantize_block(const Tensor& x) {
           "quantize_block: expected a 2-D bf16 tensor whose columns are a multiple of 16");
   const c10::cuda::CUDAGuard guard(x.device());
   const py::gil_scoped_release nogil;
-  const Block q = empty_row_blocks(x.size(0), x.size(1), x.device());
-  quantize_blocks(readable_rows(x), Experts{}, &q, nullptr);
-  return {q.data, q.scale};
+  const Tensor data = empty(x.sizes(), kE4M3, x.device()), scale = empty({blocks_of(x.size(1)), x.size(0)}, at::kFloat, x.device());
+  quantize_blocks(readable_rows(x), Experts{}, of_tensors(data, scale), Block{});
+  return {data, scale};
 }
 
 std::pair<Tensor, Tensor> quantize_block_weight(const Tensor& w) {
@@ -1237,8 +1253,11 @@ std::pair<Tensor, Tensor> quantize_block_weight(const Tensor& w) {
           "quantize_block_weight: expected a bf16 or fp32 (out, in) or (experts, out, in) with features a multiple of 16");
   const c10::cuda::CUDAGuard guard(w.device());
   const py::gil_scoped_release nogil;
-  const Block q = quantize_weight_blocks(w);
-  return {q.data, q.scale};
+  const int64_t scales[3] = {w.size(0), blocks_of(w.size(-2)), blocks_of(w.size(-1))};
+  const Tensor data = empty(w.sizes(), kE4M3, w.device());
+  const Tensor scale = empty(w.dim() == 3 ? at::IntArrayRef(scales, 3) : at::IntArrayRef(scales + 1, 2), at::kFloat, w.device());
+  quantize_weight(w, of_tensors(data, scale));
+  return {data, scale};
 }
 
 // (res, n, q data, q scale, rstd); res is x where there is no r, n undefined where it is not wanted.
@@ -1248,7 +1267,7 @@ struct ResidualNormBlock : torch::autograd::Function<ResidualNormBlock> {
     const int64_t cols = x.size(-1), rows = x.numel() / cols;
     const Tensor res = r.defined() ? empty(x.sizes(), at::kBFloat16, device) : x;
     const Tensor n = with_n ? empty(x.sizes(), at::kBFloat16, device) : Tensor();
-    const Block q = empty_row_blocks(rows, cols, device);
+    const Tensor data = empty({rows, cols}, kE4M3, device), scale = empty({blocks_of(cols), rows}, at::kFloat, device);
     const Tensor rstd = empty({rows}, at::kFloat, device);
     mxb200_block_norm_args a{};
     a.x = x.data_ptr();
@@ -1256,12 +1275,12 @@ struct ResidualNormBlock : torch::autograd::Function<ResidualNormBlock> {
     a.gain = gain.defined() ? gain.data_ptr() : nullptr;
     a.res = r.defined() ? res.data_ptr() : nullptr;
     a.n = with_n ? n.data_ptr() : nullptr;
-    a.q = q.data.data_ptr(), a.scale = static_cast<float*>(q.scale.data_ptr()), a.rstd = static_cast<float*>(rstd.data_ptr());
+    a.q = data.data_ptr(), a.scale = static_cast<float*>(scale.data_ptr()), a.rstd = static_cast<float*>(rstd.data_ptr());
     a.rows = rows, a.cols = static_cast<int32_t>(cols);
     a.gain_bf16 = gain.defined() && gain.scalar_type() == at::kBFloat16;
     a.eps = static_cast<float>(eps);
     check(mxb200_block_norm_fwd(&a, stream()), "residual_norm_block");
-    return {res, n, q.data, q.scale, rstd};
+    return {res, n, data, scale, rstd};
   }
 
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const std::optional<Tensor>& r_in,
@@ -1438,11 +1457,14 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("softcap_cross_entropy", &softcap_cross_entropy);
   m.def("residual_norm_mx", &residual_norm_mx, py::call_guard<py::gil_scoped_release>());
   m.def("quantize_mx_batch_into", &quantize_mx_batch_into);
-  m.def("fp8_block_matmul", [](const std::optional<Tensor>& x, const std::optional<Tensor>& w, const GivenBlock& x_block, const GivenBlock& w_block) {
-    return block_linear(x, w, x_block, w_block, std::nullopt, "fp8_block_matmul");
+  m.def("fp8_block_matmul", [](const MaybeTensor& x, const MaybeTensor& w, const MaybeTensor& x_data, const MaybeTensor& x_scale,
+                               const MaybeTensor& w_data, const MaybeTensor& w_scale) {
+    return block_linear(x, w, x_data, x_scale, w_data, w_scale, nullptr, "fp8_block_matmul");
   });
-  m.def("fp8_block_experts", [](const std::optional<Tensor>& x, const std::optional<Tensor>& w, const Tensor& ends, const GivenBlock& x_block,
-                                const GivenBlock& w_block) { return block_linear(x, w, x_block, w_block, ends, "fp8_block_experts"); });
+  m.def("fp8_block_experts", [](const MaybeTensor& x, const MaybeTensor& w, const MaybeTensor& x_data, const MaybeTensor& x_scale,
+                                const MaybeTensor& w_data, const MaybeTensor& w_scale, const Tensor& ends) {
+    return block_linear(x, w, x_data, x_scale, w_data, w_scale, &ends, "fp8_block_experts");
+  });
   m.def("quantize_block", &quantize_block);
   m.def("quantize_block_weight", &quantize_block_weight);
   m.def("residual_norm_block", &residual_norm_block);

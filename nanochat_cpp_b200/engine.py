@@ -560,10 +560,6 @@ class BlockTensor:
     scale: torch.Tensor
 
 
-def _pair(q: Optional[BlockTensor]):
-    return None if q is None else (q.data, q.scale)
-
-
 def quantize_block(x: torch.Tensor) -> BlockTensor:
     """A (T, C) bf16 activation in blocks of 128 along its rows, C % 16 == 0, any T. The scale of a block is the smallest power
     of two s >= 2^-126 with max|block| <= 448 s, so only the rounding to E4M3 loses bits. NaN stays NaN, Inf becomes 448 s."""
@@ -576,14 +572,15 @@ def quantize_block_weight(w: torch.Tensor) -> BlockTensor:
     return BlockTensor(*native.quantize_block_weight(w))
 
 
-def _block_weight(w, cache):
-    """(the weight for autograd or None, its blocks or None)"""
+def _block_operands(w, x_block, cache):
+    """(the weight for autograd or None, x_block's data and scale, the weight's)"""
+    x_data, x_scale = (None, None) if x_block is None else (x_block.data, x_block.scale)
     if isinstance(w, BlockTensor):
-        return None, _pair(w)
+        return None, x_data, x_scale, w.data, w.scale
     if cache is None:
-        return w, None
-    q = cache.get(2, [w], lambda: list(native.quantize_block_weight(w)))
-    return w, (q[0], q[1])
+        return w, x_data, x_scale, None, None
+    w_data, w_scale = cache.get(2, [w], lambda: list(native.quantize_block_weight(w)))
+    return w, x_data, x_scale, w_data, w_scale
 
 
 def fp8_block_matmul(x: Optional[torch.Tensor], w, x_block: Optional[BlockTensor] = None,
@@ -595,8 +592,7 @@ def fp8_block_matmul(x: Optional[torch.Tensor], w, x_block: Optional[BlockTensor
 
     Gradients come through autograd, the weight's in its own type. They use the incoming gradient in blocks along its rows for
     dx, and gradient and input in blocks of 128 tokens for dw."""
-    w, w_block = _block_weight(w, cache)
-    return native.fp8_block_matmul(x, w, _pair(x_block), w_block)
+    return native.fp8_block_matmul(x, *_block_operands(w, x_block, cache))
 
 
 def fp8_block_experts(x: Optional[torch.Tensor], w, ends: torch.Tensor, x_block: Optional[BlockTensor] = None,
@@ -606,8 +602,7 @@ def fp8_block_experts(x: Optional[torch.Tensor], w, ends: torch.Tensor, x_block:
     [ends[e - 1], ends[e]), which may be none; rows behind the last end belong to nobody, their outputs and gradients are
     zeros. ends is never read on the host; an end below the previous one, or above T, counts as that. At most 1024 experts.
     Token blocks of the weight's gradient start over at every expert."""
-    w, w_block = _block_weight(w, cache)
-    return native.fp8_block_experts(x, w, ends, _pair(x_block), w_block)
+    return native.fp8_block_experts(x, *_block_operands(w, x_block, cache), ends)
 
 
 def residual_norm_block(x: torch.Tensor, r: Optional[torch.Tensor] = None, gain: Optional[torch.Tensor] = None,
