@@ -272,25 +272,34 @@ MXB200_API int mxb200_gemm_group(const mxb200_gemm_desc* g, int n, void* workspa
  * operands of a weight gradient have 128 times as many rows. */
 MXB200_API int64_t mxb200_block_token_blocks(int64_t tokens, int experts);
 
-/* x: (rows, cols) bf16 with ld >= cols values between rows (ld % 8 == 0). row_data (rows, cols) e4m3 and row_scale
- * (ceil(cols / 128), rows): blocks along rows. token_data (128 * token blocks, cols) and token_scale (token blocks,
- * ceil(cols / 128), 128): blocks along each expert's tokens, whose last block is filled up with zeros. Their scales, always
- * powers of two, are kept as the tensor core takes them: for each 128 columns a tile of 128 words, the word of column c at
- * 4 (c % 32) + c / 32 within the tile, its four bytes the scale's biased exponent. Either output may be null. With token_data,
- * rows of no expert are written to neither. */
+/* Scale tiles: powers of two as the tensor core takes them, 128 words for 128 rows (or columns) of one block of the contraction,
+ * the word of the r-th at 4 (r % 32) + r / 32, its four bytes the scale's biased exponent.
+ *
+ * x: (rows, cols) bf16 with ld >= cols values between rows (ld % 8 == 0). row_data (rows, cols) e4m3 and row_scale
+ * (ceil(cols / 128), rows) fp32: blocks along rows. token_data (128 * token blocks, cols) and token_scale, tiles (token blocks,
+ * ceil(cols / 128), 128): blocks along each expert's tokens, whose last block is filled up with zeros. Either may be null; with
+ * token_data, rows of no expert are written to neither. rows_in_blocks != 0 (both wanted): row_data is (128 * token blocks, cols),
+ * every expert's rows from the first of a token block on, and row_scale its tiles (token blocks, ceil(cols / 128), 128). */
 MXB200_API int mxb200_block_quantize(const void* x, int64_t rows, int64_t cols, int64_t ld, const int32_t* ends, int experts,
-                                     void* row_data, float* row_scale, void* token_data, uint32_t* token_scale, void* stream);
+                                     void* row_data, void* row_scale, int rows_in_blocks, void* token_data, uint32_t* token_scale,
+                                     void* stream);
 
 /* w: (experts, rows, cols) contiguous, bf16 (w_bf16 != 0) or fp32, to data of that shape and scale
- * (experts, ceil(rows / 128), ceil(cols / 128)). */
+ * (experts, ceil(rows / 128), ceil(cols / 128)) fp32, or with in_tiles != 0 a tile for each. */
 MXB200_API int mxb200_block_quantize_weight(const void* w, int w_bf16, int experts, int64_t rows, int64_t cols, void* data,
-                                            float* scale, void* stream);
+                                            void* scale, int in_tiles, void* stream);
 
 typedef enum mxb200_block_kind {
   MXB200_BLOCK_FORWARD = 0,     /* d (tokens, out) bf16 = b (tokens, in), rows . a (experts, out, in)^T, weight */
   MXB200_BLOCK_INPUT_GRAD = 1,  /* d (tokens, in) bf16 = b (tokens, out), rows . a (experts, out, in), weight */
-  MXB200_BLOCK_WEIGHT_GRAD = 2  /* d (experts, out, in) bf16 or fp32 = a (., out)^T, tokens . b (., in), tokens */
+  MXB200_BLOCK_WEIGHT_GRAD = 2, /* d (experts, out, in) bf16 or fp32 = a (., out)^T, tokens . b (., in), tokens */
+  /* the first two of rows in blocks and a weight with scale tiles; faster where mxb200_block_scaled says so */
+  MXB200_BLOCK_FORWARD_SCALED = 3,
+  MXB200_BLOCK_INPUT_GRAD_SCALED = 4
 } mxb200_block_kind;
+
+/* Whether the scaled kinds are the faster ones for a Linear's forward and input gradient of this size on the current device. */
+MXB200_API int mxb200_block_scaled(int64_t tokens, int64_t in_features, int64_t out_features, int experts);
 
 #define MXB200_BLOCK_FEW_TOKENS 32
 
@@ -298,7 +307,7 @@ typedef enum mxb200_block_kind {
  * expert without rows: zeros. Needs no workspace. tokens may be 0. */
 typedef struct mxb200_block_gemm_args {
   const void* a;
-  const void* a_scale; /* fp32; the weight gradient's as mxb200_block_quantize makes token_scale */
+  const void* a_scale; /* fp32; scale tiles for the weight gradient and the scaled kinds */
   const void* b;
   const void* b_scale;
   void* d;

@@ -16,7 +16,7 @@ ERR_SHAPE, ERR_ALIGNMENT, ERR_NULL, ERR_ARGUMENT, ERR_WORKSPACE, ERR_DEVICE, ERR
 SCALE_REFERENCE, SCALE_OCP_FLOOR = 0, 1
 PROLOGUE_NONE, PROLOGUE_RELU_SQUARE = 0, 1
 OUT_BF16, OUT_F32 = 0, 1
-BLOCK_FORWARD, BLOCK_INPUT_GRAD, BLOCK_WEIGHT_GRAD = 0, 1, 2
+BLOCK_FORWARD, BLOCK_INPUT_GRAD, BLOCK_WEIGHT_GRAD, BLOCK_FORWARD_SCALED, BLOCK_INPUT_GRAD_SCALED = range(5)
 STATIC_SCRATCH_BYTES = 32 << 20
 
 # every symbol include/mxb200.h declares
@@ -28,7 +28,7 @@ SYMBOLS = (
     "mxb200_count_valid", "mxb200_reduce_losses", "mxb200_scale_bf16",
     "mxb200_gemm_group_workspace_bytes", "mxb200_gemm_group",
     "mxb200_gemm_splits", "mxb200_gemm_workspace_bytes", "mxb200_gemm_splitk", "mxb200_gemm_splitk_static",
-    "mxb200_block_token_blocks", "mxb200_block_quantize", "mxb200_block_quantize_weight", "mxb200_block_gemm",
+    "mxb200_block_token_blocks", "mxb200_block_quantize", "mxb200_block_quantize_weight", "mxb200_block_gemm", "mxb200_block_scaled",
     "mxb200_block_norm_fwd", "mxb200_block_norm_workspace_bytes", "mxb200_block_norm_bwd",
     "mxb200_strerror",
     "mxb200_device_status", "mxb200_selftest_bounded_wait", "mxb200_set_gemm_config", "mxb200_launch_count", "mxb200_version",
@@ -127,8 +127,9 @@ def _load() -> ctypes.CDLL:
     lib.mxb200_gemm_splitk_static.argtypes = [vp, vp, vp, vp, vp, i32, vp, i64, i64, i64, vp, i32, i32, vp]
     lib.mxb200_block_token_blocks.argtypes = [i64, i32]
     lib.mxb200_block_token_blocks.restype = i64
-    lib.mxb200_block_quantize.argtypes = [vp, i64, i64, i64, vp, i32, vp, vp, vp, vp, vp]
-    lib.mxb200_block_quantize_weight.argtypes = [vp, i32, i32, i64, i64, vp, vp, vp]
+    lib.mxb200_block_quantize.argtypes = [vp, i64, i64, i64, vp, i32, vp, vp, i32, vp, vp, vp]
+    lib.mxb200_block_quantize_weight.argtypes = [vp, i32, i32, i64, i64, vp, vp, i32, vp]
+    lib.mxb200_block_scaled.argtypes = [i64, i64, i64, i32]
     lib.mxb200_block_gemm.argtypes = [ctypes.POINTER(BlockGemmArgs), vp]
     lib.mxb200_block_norm_fwd.argtypes = [ctypes.POINTER(BlockNormArgs), vp]
     lib.mxb200_block_norm_workspace_bytes.argtypes = [i64, ctypes.c_int32]

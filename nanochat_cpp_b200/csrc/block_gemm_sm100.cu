@@ -19,8 +19,9 @@
 //     rows, and an expert's last tile is as narrow as its last rows. Scales differ by column: fragments (16x256b) give a thread
 //     8 columns of 4 rows each 32, so that a scale read from shared memory serves 4 values.
 //
-// The weight gradient's scales are this library's own, powers of two, and differ by row and by column: here the tensor core
-// applies them (kind::mxf8f6f4, the four K = 32 steps of a block under the same scale byte) and sums up in tensor memory.
+// Where all scales are this library's own, powers of two, the tensor core applies them itself (kind::mxf8f6f4, the four K = 32
+// steps of a block under the same scale byte) and sums up in tensor memory: the weight gradient, always, and the other two in
+// training passes of many tokens.
 #include <algorithm>
 #include <cstddef>
 #include <cstdint>
@@ -87,6 +88,7 @@ struct Params {
   int64_t token_ld;
   int64_t w_scale_expert;
   int w_scale_f, w_scale_b;   // strides of the weight's scale over feature tiles of 128 and over blocks
+  int w_scale_rows;           // scales in the tensor core: rows of scale tiles of an expert's weight
   void* d;
   const int32_t* ends;
   int experts;   // 1 where ends is null
@@ -171,9 +173,10 @@ struct SetUp {
 
 // Barriers, tensor memory and the experts' rows; the operand stages at `base` hold the scan's words meanwhile. All threads.
 // kCtas: that share tensor memory operations. cluster: the CTAs of a cluster signal one another.
+// first_block: where given, the blocks of 128 tokens before each expert's.
 template <int kCtas, typename S>
 __device__ __forceinline__ uint32_t set_up(const Params& p, const CUtensorMap* map_a, const CUtensorMap* map_b, S* s, unsigned char* base,
-                                           int warp, const SetUp& set, bool cluster) {
+                                           int warp, const SetUp& set, bool cluster, int* first_block = nullptr) {
   if (threadIdx.x == 0) {
     for (int i = 0; i < S::kStages; ++i) {
       mbar_init(&s->full[i], set.full_arrivals);
@@ -205,6 +208,8 @@ __device__ __forceinline__ uint32_t set_up(const Params& p, const CUtensorMap* m
   tcgen05_fence_before_sync();
   grid_dependency_wait();
   scan_experts(p.ends, p.experts, p.rows, set.tile_rows, s->first_row, s->first_tile, reinterpret_cast<int*>(base));
+  if (first_block != nullptr)
+    scan_experts(p.ends, p.experts, p.rows, kBlock, s->first_row, first_block, reinterpret_cast<int*>(base));
   if (set.rest_is_a_tile && p.ends != nullptr && threadIdx.x == 0) {
     s->first_row[p.experts + 1] = p.rows;
     s->first_tile[p.experts + 1] = s->first_tile[p.experts] + (p.rows - s->first_row[p.experts] + set.tile_rows - 1) / set.tile_rows;
@@ -892,15 +897,15 @@ __device__ __forceinline__ void body(const Params& p, const CUtensorMap* map_t, 
 
 }  // namespace many
 
-// ==================================================================================================== weight gradient
+// ==================================================================================================== scales in the tensor core
 //
-// A CTA pair, 256 x 256 of one expert's dw: operand A gradients (128 of their columns per CTA), B inputs, both MN-major, with
-// scale tiles (512 bytes: a word for each of 128 columns, the E8M0 byte four times, in the order of the copy to tensor
-// memory) through shared into tensor memory. Two
-// accumulator buffers share 32 columns, so that the scales find room beside them: [0, 256), [224, 480), scales at [480, 492);
-// the epilogue drains the shared columns first.
+// All three products where every scale is this library's own, a power of two: a CTA pair, 256 x 256. Operand A has the output's
+// rows (tokens; a weight gradient's features), 128 per CTA, B its columns, each CTA half of them. Scale tiles (512 bytes: a word
+// for each of 128 rows or columns, the E8M0 byte four times, in the order of the copy to tensor memory) go through shared into
+// tensor memory. Two accumulator buffers share 32 columns, so that the scales find room beside them: [0, 256), [224, 480),
+// scales at [480, 492); the epilogue drains the shared columns first.
 
-namespace wgrad {
+namespace scaled {
 
 constexpr int kTile = 256;
 constexpr uint32_t kScaleTile = 512, kScaleBytes = 3 * kScaleTile;
@@ -908,6 +913,7 @@ constexpr uint32_t kAcc1 = 224;  // the second accumulator buffer; the first is 
 constexpr uint32_t kScaleA = 480, kScaleB = 484;
 
 struct Shared : Common<5> {
+  int first_block[kMaxExperts + 2];  // blocks of 128 tokens before an expert's
   LineStage out[kEpilogueWarps];
 };
 
@@ -916,24 +922,40 @@ constexpr size_t kSmemBytes = 1024 + Shared::kStages * kStageBytes + sizeof(Shar
 static_assert(kSmemBytes <= 232448, "shared memory of one CTA");
 
 struct Unit {
-  int expert, m0, n0, block0, blocks;
+  int expert;
+  int block0, blocks;  // weight gradient: the expert's token blocks; else the tile's first token block, and the blocks of the contraction
+  int m0, rows;        // first row of the output (of the expert's dw), and how many there are
+  int n0;              // first column
 };
 
+template <int kMode>
 __device__ __forceinline__ Unit unit_at(const Params& p, const Shared* s, int u) {
-  const int mt = (p.features + kTile - 1) / kTile, nt = (p.n + kTile - 1) / kTile;
   Unit x;
-  x.expert = u / (mt * nt);
-  int v = u - x.expert * mt * nt;
-  const int panel = v / (kPanel * nt);
-  v -= panel * kPanel * nt;
-  const int width = min(kPanel, mt - panel * kPanel);
-  x.n0 = v / width * kTile;
-  x.m0 = (panel * kPanel + v % width) * kTile;
-  x.block0 = s->first_tile[x.expert];
-  x.blocks = s->first_tile[x.expert + 1] - x.block0;
+  if constexpr (kMode == kWeightGrad) {
+    const int mt = (p.features + kTile - 1) / kTile, nt = (p.n + kTile - 1) / kTile;
+    x.expert = u / (mt * nt);
+    int v = u - x.expert * mt * nt;
+    const int panel = v / (kPanel * nt);
+    v -= panel * kPanel * nt;
+    const int width = min(kPanel, mt - panel * kPanel);
+    x.n0 = v / width * kTile;
+    x.m0 = (panel * kPanel + v % width) * kTile;
+    x.rows = min(kTile, p.features - x.m0);
+    x.block0 = s->first_block[x.expert];
+    x.blocks = s->first_block[x.expert + 1] - x.block0;
+  } else {
+    const mxb200::Unit y = mxb200::unit_at<kTile, kTile>(p, s, u);
+    x.expert = y.expert;
+    x.n0 = y.f0;
+    x.m0 = y.row0;
+    x.rows = y.rows;
+    x.blocks = y.blocks;
+    x.block0 = y.blocks > 0 ? s->first_block[y.expert] + (y.row0 - s->first_row[y.expert]) / kBlock : 0;
+  }
   return x;
 }
 
+template <int kMode>
 __device__ __forceinline__ void load_operands(const Params& p, const Maps& maps, Shared* s, uint32_t a0, int rank, int first, int step, int units) {
   const uint32_t el = elect_one() ? 1u : 0u, el_leader = rank == 0 ? el : 0u;
   const uint32_t empty0 = smem_u32(&s->empty[0]), full0 = smem_u32(&s->full[0]);
@@ -941,25 +963,39 @@ __device__ __forceinline__ void load_operands(const Params& p, const Maps& maps,
   const uint32_t b0 = a0 + Shared::kStages * kABytes, sf0 = b0 + Shared::kStages * kBBytes;
   uint32_t stage = 0, phase = 0;
   for (int u = first; u < units; u += step) {
-    const Unit x = unit_at(p, s, u);
+    const Unit x = unit_at<kMode>(p, s, u);
     for (int b = 0; b < x.blocks; ++b) {
       if (!wait_bounded(empty0 + stage * 8, phase ^ 1u, &s->abort_flag, kSiteStageEmpty))
         return;
       mbar_arrive_expect_tx(el_leader, full0 + stage * 8, 2 * kStageBytes);
-      const uint32_t full = full_leader0 + stage * 8, sf = sf0 + stage * kScaleBytes;
-      const int block = x.block0 + b;
-      tma_load_3d_pair(el, a0 + stage * kABytes, &maps.a, full, x.m0 + rank * 128, block * kBlock, 0);
-      tma_load_3d_pair(el, b0 + stage * kBBytes, &maps.b, full, x.n0 + rank * 128, block * kBlock, 0);
-      tma_load_3d_pair(el, sf, &maps.a_scale, full, 0, (x.m0 >> 7) + rank, block);
-      tma_load_3d_pair(el, sf + kScaleTile, &maps.b_scale, full, 0, x.n0 >> 7, block);
+      const uint32_t full = full_leader0 + stage * 8, a = a0 + stage * kABytes, bs = b0 + stage * kBBytes, sf = sf0 + stage * kScaleBytes;
+      if constexpr (kMode == kWeightGrad) {
+        const int block = x.block0 + b;
+        tma_load_3d_pair(el, a, &maps.a, full, x.m0 + rank * 128, block * kBlock, 0);
+        tma_load_3d_pair(el, bs, &maps.b, full, x.n0 + rank * 128, block * kBlock, 0);
+        tma_load_3d_pair(el, sf, &maps.a_scale, full, 0, (x.m0 >> 7) + rank, block);
+        tma_load_3d_pair(el, sf + kScaleTile, &maps.b_scale, full, 0, x.n0 >> 7, block);
+      } else {
+        const int k = b * kBlock, block = x.block0 + rank, feature = x.n0 + rank * 128;
+        const int weight0 = x.expert * p.w_scale_rows;  // the expert's first row of scale tiles
+        tma_load_3d_pair(el, a, &maps.a, full, k, block * kBlock, 0);
+        tma_load_3d_pair(el, bs, &maps.b, full, kMode == kForward ? k : feature, kMode == kForward ? feature : k, x.expert);
+        tma_load_3d_pair(el, sf, &maps.a_scale, full, 0, b, block);
+        tma_load_3d_pair(el, sf + kScaleTile, &maps.b_scale, full, 0, kMode == kForward ? b : x.n0 >> 7,
+                         weight0 + (kMode == kForward ? x.n0 >> 7 : b));
+      }
       if (++stage == Shared::kStages)
         stage = 0, phase ^= 1u;
     }
   }
 }
 
+template <int kMode>
 __device__ __forceinline__ void issue_mmas(const Params& p, Shared* s, uint32_t a0, uint32_t tmem_base, int first, int step, int units) {
-  constexpr uint32_t idesc = make_idesc_mxf8(kTile, kTile) | kIdescAMn | kIdescBMn;
+  constexpr bool kAMn = kMode == kWeightGrad, kBMn = kMode != kForward;
+  // K = 32: 32 bytes within K-major rows, 32 rows of MN-major ones
+  constexpr uint32_t kAStep = kAMn ? 4096 >> 4 : 32 >> 4, kBStep = kBMn ? 4096 >> 4 : 32 >> 4;
+  constexpr uint32_t idesc = make_idesc_mxf8(kTile, kTile) | (kAMn ? kIdescAMn : 0u) | (kBMn ? kIdescBMn : 0u);
   const uint32_t el = elect_one() ? 1u : 0u;
   const uint32_t full0 = smem_u32(&s->full[0]), empty0 = smem_u32(&s->empty[0]);
   const uint32_t b0 = a0 + Shared::kStages * kABytes, sf0 = b0 + Shared::kStages * kBBytes;
@@ -968,7 +1004,7 @@ __device__ __forceinline__ void issue_mmas(const Params& p, Shared* s, uint32_t 
   const uint32_t sfa = tmem_base + kScaleA, sfb = tmem_base + kScaleB;
   uint32_t stage = 0, phase = 0, local = 0;
   for (int u = first; u < units; u += step) {
-    const int blocks = unit_at(p, s, u).blocks;
+    const int blocks = unit_at<kMode>(p, s, u).blocks;
     if (blocks == 0)
       continue;
     const uint32_t buf = local & 1u;
@@ -986,8 +1022,8 @@ __device__ __forceinline__ void issue_mmas(const Params& p, Shared* s, uint32_t 
       tcgen05_cp_32x128b_warpx4_pair(el, sfb + 4, sf + 2 * (kScaleTile >> 4));
       const uint64_t a = a_desc0 + stage * (kABytes >> 4), bd = b_desc0 + stage * (kBBytes >> 4);
 #pragma unroll
-      for (uint32_t k = 0; k < 4; ++k)  // K = 32: 32 rows of 128 bytes
-        tcgen05_mma_mxf8_pair(el, tmem_base + buf * kAcc1, a + k * (4096 >> 4), bd + k * (4096 >> 4), idesc, sfa, sfb, b > 0 || k > 0);
+      for (uint32_t k = 0; k < 4; ++k)
+        tcgen05_mma_mxf8_pair(el, tmem_base + buf * kAcc1, a + k * kAStep, bd + k * kBStep, idesc, sfa, sfb, b > 0 || k > 0);
       tcgen05_commit_pair(el, empty0 + stage * 8, 3);
       if (++stage == Shared::kStages)
         stage = 0, phase ^= 1u;
@@ -996,13 +1032,17 @@ __device__ __forceinline__ void issue_mmas(const Params& p, Shared* s, uint32_t 
   }
 }
 
+template <int kMode>
 __device__ __forceinline__ void store(const Params& p, Shared* s, uint32_t tmem_base, int rank, int first, int step, int units, int warp, int lane) {
   const int quarter = warp & 3, part = (warp - kFirstEpilogueWarp) >> 2;
   const uint32_t t0 = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
   const uint32_t acc_empty0 = map_to_cta(smem_u32(&s->acc_empty[0]), 0), overlap_free = map_to_cta(smem_u32(&s->overlap_free), 0);
+  const int columns = kMode == kWeightGrad ? p.n : p.features;
+  const bool bf16 = kMode != kWeightGrad || p.out_bf16;
+  LineStage* stage = &s->out[warp - kFirstEpilogueWarp];
   uint32_t local = 0;
   for (int u = first; u < units; u += step) {
-    const Unit x = unit_at(p, s, u);
+    const Unit x = unit_at<kMode>(p, s, u);
     const uint32_t buf = local & 1u;
     if (x.blocks > 0) {
       if (!wait_bounded(smem_u32(&s->acc_full[buf]), (local >> 1) & 1u, &s->abort_flag, kSiteAccFull))
@@ -1010,11 +1050,10 @@ __device__ __forceinline__ void store(const Params& p, Shared* s, uint32_t tmem_
       tcgen05_fence_after_sync();
       ++local;
     }
-    const int row = x.m0 + rank * 128 + quarter * 32;
-    const int64_t at = (static_cast<int64_t>(x.expert) * p.features + row) * p.n + x.n0;
-    const int value = p.out_bf16 ? 2 : 4;
-    unsigned char* d = static_cast<unsigned char*>(p.d) + at * value;
-    LineStage* stage = &s->out[warp - kFirstEpilogueWarp];
+    const int row = rank * 128 + quarter * 32, rows = x.rows - row;
+    const int64_t line = static_cast<int64_t>(columns) * (bf16 ? 2 : 4);
+    unsigned char* d = static_cast<unsigned char*>(p.d) + ((kMode == kWeightGrad ? static_cast<int64_t>(x.expert) * p.features : 0) + x.m0 + row) * line +
+                       static_cast<int64_t>(x.n0) * (bf16 ? 2 : 4);
     uint32_t half[16];  // bf16: the first 32 columns of a line
 #pragma unroll 1
     for (int i = 0; i < 4; ++i) {
@@ -1042,8 +1081,8 @@ __device__ __forceinline__ void store(const Params& p, Shared* s, uint32_t tmem_
         for (int k = 0; k < 32; ++k)
           v[k] = 0;
       }
-      if (!p.out_bf16) {
-        store_lines(stage, lane, d + 128 * c, static_cast<int64_t>(p.n) * 4, p.features - row, (p.n - x.n0 - 32 * c) * 4,
+      if (!bf16) {
+        store_lines(stage, lane, d + 128 * c, line, rows, (columns - x.n0 - 32 * c) * 4,
                     [&](int q) { return make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]); });
         continue;
       }
@@ -1057,7 +1096,7 @@ __device__ __forceinline__ void store(const Params& p, Shared* s, uint32_t tmem_
           half[j] = h[j];
       } else {
         const bool swapped = buf == 0;
-        store_lines(stage, lane, d + 64 * (c & ~1), static_cast<int64_t>(p.n) * 2, p.features - row, (p.n - x.n0 - 32 * (c & ~1)) * 2,
+        store_lines(stage, lane, d + 64 * (c & ~1), line, rows, (columns - x.n0 - 32 * (c & ~1)) * 2,
                     [&](int q) {
                       const int k = 4 * (q & 3);
                       const bool from_half = (q < 4) != swapped;
@@ -1069,6 +1108,7 @@ __device__ __forceinline__ void store(const Params& p, Shared* s, uint32_t tmem_
   }
 }
 
+template <int kMode>
 __device__ __forceinline__ void body(const Params& p, const Maps& maps) {
   extern __shared__ unsigned char smem_raw[];
   unsigned char* base = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
@@ -1076,20 +1116,20 @@ __device__ __forceinline__ void body(const Params& p, const Maps& maps) {
   Shared* s = reinterpret_cast<Shared*>(base + Shared::kStages * kStageBytes);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = static_cast<int>(cluster_ctarank());
-  const SetUp set{1, 1, 2 * kEpilogueWarps, 2, 1, kBlock, false};
-  const uint32_t tmem_base = set_up<2>(p, &maps.a, &maps.b, s, base, warp, set, true);
-  const int units = p.experts * ((p.features + kTile - 1) / kTile) * ((p.n + kTile - 1) / kTile);
+  const SetUp set{1, 1, 2 * kEpilogueWarps, 2, 1, kTile, kMode != kWeightGrad};
+  const uint32_t tmem_base = set_up<2>(p, &maps.a, &maps.b, s, base, warp, set, true, s->first_block);
+  const int units = kMode == kWeightGrad ? p.experts * ((p.features + kTile - 1) / kTile) * ((p.n + kTile - 1) / kTile) : units_of(p, s, kTile);
   const int first = blockIdx.x / 2, step = gridDim.x / 2;
   if (warp == 0)
-    load_operands(p, maps, s, a0, rank, first, step, units);
+    load_operands<kMode>(p, maps, s, a0, rank, first, step, units);
   else if (warp == 1 && rank == 0)
-    issue_mmas(p, s, a0, tmem_base, first, step, units);
+    issue_mmas<kMode>(p, s, a0, tmem_base, first, step, units);
   else if (warp >= kFirstEpilogueWarp)
-    store(p, s, tmem_base, rank, first, step, units, warp, lane);
+    store<kMode>(p, s, tmem_base, rank, first, step, units, warp, lane);
   tear_down<2>(s, tmem_base, warp, true);
 }
 
-}  // namespace wgrad
+}  // namespace scaled
 
 struct Launch {
   Maps maps;
@@ -1121,7 +1161,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(mxb200::kThreads, 1)
 }
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(mxb200::kThreads, 1)
       mxb200_block_gemm_weight_grad(const __grid_constant__ mxb200::Launch args) {
-  mxb200::wgrad::body(args.p, args.maps);
+  mxb200::scaled::body<mxb200::kWeightGrad>(args.p, args.maps);
+}
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(mxb200::kThreads, 1)
+      mxb200_block_gemm_forward_scaled(const __grid_constant__ mxb200::Launch args) {
+  mxb200::scaled::body<mxb200::kForward>(args.p, args.maps);
+}
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(mxb200::kThreads, 1)
+      mxb200_block_gemm_input_grad_scaled(const __grid_constant__ mxb200::Launch args) {
+  mxb200::scaled::body<mxb200::kInputGrad>(args.p, args.maps);
 }
 
 namespace mxb200 {
@@ -1146,15 +1194,14 @@ int64_t up(int64_t n, int64_t d) {
   return (n + d - 1) / d;
 }
 
-// Scale tiles of (tokens, columns): 128 words for each block of tokens and each 128 columns, `tiles` of a block's at a time.
-int make_scale_map(CUtensorMap* map, const void* base, int64_t columns, int64_t tokens, int tiles) {
+// (z, y) scale tiles of 128 words, `box_z` x `box_y` at a time.
+int make_scale_map(CUtensorMap* map, const void* base, int64_t y, int64_t z, int box_y, int box_z) {
   EncodeTiledFn fn = encode_fn();
   if (fn == nullptr)
     return MXB200_ERR_DRIVER;
-  const cuuint64_t n = static_cast<cuuint64_t>(up(columns, kBlock));
-  const cuuint64_t dims[3] = {kBlock, n, static_cast<cuuint64_t>(tokens / kBlock)};
-  const cuuint64_t strides[2] = {kBlock * 4, n * kBlock * 4};
-  const cuuint32_t box[3] = {kBlock, static_cast<cuuint32_t>(tiles), 1};
+  const cuuint64_t dims[3] = {kBlock, static_cast<cuuint64_t>(y), static_cast<cuuint64_t>(z)};
+  const cuuint64_t strides[2] = {kBlock * 4, static_cast<cuuint64_t>(y) * kBlock * 4};
+  const cuuint32_t box[3] = {kBlock, static_cast<cuuint32_t>(box_y), static_cast<cuuint32_t>(box_z)};
   const cuuint32_t estr[3] = {1, 1, 1};
   const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, const_cast<void*>(base), dims, strides, box, estr,
                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_NONE,
@@ -1171,7 +1218,7 @@ struct Variant {
   int tokens, features; // of a unit
 };
 
-enum VariantId : int { kForwardFew, kForward32, kForwardMany, kForwardQuantizing, kInputGradFew, kInputGradMany, kWeightGradPair, kVariants };
+enum VariantId : int { kForwardFew, kForward32, kForwardMany, kForwardQuantizing, kInputGradFew, kInputGradMany, kWeightGradPair, kForwardScaled, kInputGradScaled, kVariants };
 
 const Variant& variant(VariantId id) {
   static const Variant variants[kVariants] = {
@@ -1181,7 +1228,9 @@ const Variant& variant(VariantId id) {
         {mxb200_block_gemm_quantize_few, few::Quantizing::kSmemBytes, 1, few::Quantizing::kTileT, few::kTileF},
         {mxb200_block_gemm_input_grad_few, few::Tile128::kSmemBytes, 1, few::Tile128::kTileT, few::kTileF},
         {mxb200_block_gemm_input_grad_many, many::kSmemBytes, 2, many::kTileT, many::kTileF},
-        {mxb200_block_gemm_weight_grad, wgrad::kSmemBytes, 2, 0, wgrad::kTile}};
+        {mxb200_block_gemm_weight_grad, scaled::kSmemBytes, 2, scaled::kTile, scaled::kTile},
+        {mxb200_block_gemm_forward_scaled, scaled::kSmemBytes, 2, scaled::kTile, scaled::kTile},
+        {mxb200_block_gemm_input_grad_scaled, scaled::kSmemBytes, 2, scaled::kTile, scaled::kTile}};
   return variants[id];
 }
 
@@ -1256,7 +1305,7 @@ int share_blocks(int64_t units, int blocks, int tile_tokens, const Configured& c
 }
 
 int block_gemm(const mxb200_block_gemm_args& g, cudaStream_t stream) {
-  if (g.kind < MXB200_BLOCK_FORWARD || g.kind > MXB200_BLOCK_WEIGHT_GRAD ||
+  if (g.kind < MXB200_BLOCK_FORWARD || g.kind > MXB200_BLOCK_INPUT_GRAD_SCALED ||
       (g.out_kind != MXB200_OUT_BF16 && (g.out_kind != MXB200_OUT_F32 || g.kind != MXB200_BLOCK_WEIGHT_GRAD)))
     return MXB200_ERR_ARGUMENT;
   constexpr int64_t kMost = int64_t{1} << 30;
@@ -1273,6 +1322,7 @@ int block_gemm(const mxb200_block_gemm_args& g, cudaStream_t stream) {
   if (int st = current_device(&dev); st != MXB200_OK)
     return st;
   const bool wgrad = g.kind == MXB200_BLOCK_WEIGHT_GRAD;
+  const bool scaled = g.kind == MXB200_BLOCK_FORWARD_SCALED || g.kind == MXB200_BLOCK_INPUT_GRAD_SCALED;
   if (g.tokens == 0) {
     if (!wgrad)
       return MXB200_OK;
@@ -1286,10 +1336,10 @@ int block_gemm(const mxb200_block_gemm_args& g, cudaStream_t stream) {
     return MXB200_ERR_NULL;
   const auto bits = [](const void* q) { return reinterpret_cast<uintptr_t>(q); };
   if (!aligned16(g.a) || !aligned16(g.b) || !aligned16(g.d) || (bits(g.ends) & 3) != 0 ||
-      ((bits(g.a_scale) | bits(g.b_scale)) & (wgrad ? 15 : 3)) != 0)
+      ((bits(g.a_scale) | bits(g.b_scale)) & (wgrad || scaled ? 15 : 3)) != 0)
     return MXB200_ERR_ALIGNMENT;
   const int64_t in = g.in_features, out = g.out_features;
-  const bool forward = g.kind == MXB200_BLOCK_FORWARD;
+  const bool forward = g.kind == MXB200_BLOCK_FORWARD || g.kind == MXB200_BLOCK_FORWARD_SCALED;
   const int from = static_cast<int>(forward ? in : out), to = static_cast<int>(forward ? out : in);
   const int blocks = static_cast<int>(up(from, kBlock));
   Launch l{};
@@ -1297,6 +1347,10 @@ int block_gemm(const mxb200_block_gemm_args& g, cudaStream_t stream) {
   p.d = g.d, p.ends = g.ends, p.experts = g.experts, p.rows = static_cast<int>(g.tokens);
   p.out_bf16 = g.out_kind == MXB200_OUT_BF16;
   p.splits = 1;
+  // token tiles are known on the device only; this many at most
+  const auto most_tiles = [&](int64_t tile) {
+    return g.ends == nullptr ? up(g.tokens, tile) : (g.tokens + (tile - 1) * std::min<int64_t>(g.experts + 1, g.tokens)) / tile;
+  };
   VariantId id = kWeightGradPair;
   Configured configured;
   int64_t units;
@@ -1306,11 +1360,22 @@ int block_gemm(const mxb200_block_gemm_args& g, cudaStream_t stream) {
       return st;
     const int64_t capacity = mxb200_block_token_blocks(g.tokens, g.experts) * kBlock;
     p.features = static_cast<int>(out), p.n = static_cast<int>(in);
-    units = g.experts * up(out, wgrad::kTile) * up(in, wgrad::kTile);
+    units = g.experts * up(out, mxb200::scaled::kTile) * up(in, mxb200::scaled::kTile);
     st = make_map(&l.maps.a, g.a, out, capacity, 1, 128);
     st = st != MXB200_OK ? st : make_map(&l.maps.b, g.b, in, capacity, 1, 128);
-    st = st != MXB200_OK ? st : make_scale_map(&l.maps.a_scale, g.a_scale, out, capacity, 1);
-    st = st != MXB200_OK ? st : make_scale_map(&l.maps.b_scale, g.b_scale, in, capacity, 2);
+    st = st != MXB200_OK ? st : make_scale_map(&l.maps.a_scale, g.a_scale, up(out, kBlock), capacity / kBlock, 1, 1);
+    st = st != MXB200_OK ? st : make_scale_map(&l.maps.b_scale, g.b_scale, up(in, kBlock), capacity / kBlock, 2, 1);
+  } else if (scaled) {
+    id = forward ? kForwardScaled : kInputGradScaled;
+    if (st = configure(id, dev, &configured); st != MXB200_OK)
+      return st;
+    const int64_t capacity = mxb200_block_token_blocks(g.tokens, g.experts) * kBlock;
+    p.features = to, p.blocks = blocks, p.w_scale_rows = static_cast<int>(up(out, kBlock));
+    units = most_tiles(mxb200::scaled::kTile) * up(to, mxb200::scaled::kTile);
+    st = make_map(&l.maps.a, g.b, from, capacity, 1, 128);
+    st = st != MXB200_OK ? st : make_map(&l.maps.b, g.a, in, out, g.experts, 128);
+    st = st != MXB200_OK ? st : make_scale_map(&l.maps.a_scale, g.b_scale, blocks, capacity / kBlock, 1, 1);
+    st = st != MXB200_OK ? st : make_scale_map(&l.maps.b_scale, g.a_scale, up(in, kBlock), up(out, kBlock) * g.experts, forward ? 1 : 2, forward ? 2 : 1);
   } else {
     const bool many = !quantize && many_tokens(g.tokens, g.experts, to, blocks, dev.sms);
     // at most half a small tile per expert expected, so that few experts need a second one
@@ -1322,10 +1387,7 @@ int block_gemm(const mxb200_block_gemm_args& g, cudaStream_t stream) {
     p.input = g.b, p.input_cols = from;
     p.w_scale_expert = up(out, kBlock) * up(in, kBlock);
     p.w_scale_f = forward ? static_cast<int>(up(in, kBlock)) : 1, p.w_scale_b = forward ? 1 : static_cast<int>(up(in, kBlock));
-    // token tiles are known on the device only; this many at most
-    const int64_t token_tiles = g.ends == nullptr ? up(g.tokens, v.tokens)
-                                                  : (g.tokens + (v.tokens - 1) * std::min<int64_t>(g.experts + 1, g.tokens)) / v.tokens;
-    units = token_tiles * up(to, v.features);
+    units = most_tiles(v.tokens) * up(to, v.features);
     if (st = configure(id, dev, &configured); st != MXB200_OK)
       return st;
     if (!many)
@@ -1363,6 +1425,15 @@ extern "C" int64_t mxb200_block_token_blocks(int64_t tokens, int experts) {
   if (tokens <= 0 || experts <= 0)
     return 0;
   return (tokens + 127 * std::min<int64_t>(experts, tokens)) / 128;
+}
+
+extern "C" int mxb200_block_scaled(int64_t tokens, int64_t in_features, int64_t out_features, int experts) {
+  using namespace mxb200;
+  DeviceInfo dev;
+  if (tokens <= 0 || in_features <= 0 || out_features <= 0 || experts <= 0 || current_device(&dev) != MXB200_OK)
+    return 0;
+  return many_tokens(tokens, experts, static_cast<int>(out_features), static_cast<int>(up(in_features, kBlock)), dev.sms) &&
+         many_tokens(tokens, experts, static_cast<int>(in_features), static_cast<int>(up(out_features, kBlock)), dev.sms);
 }
 
 extern "C" int mxb200_block_gemm(const mxb200_block_gemm_args* args, void* stream) {

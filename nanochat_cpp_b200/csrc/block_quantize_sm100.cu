@@ -38,7 +38,8 @@ struct QuantizeParams {
   float* row_scale;     // (cols / 128, rows)
   uint8_t* col_data;    // tokens: (token blocks * 128, cols); weight: (experts, rows, cols)
   float* col_scale;     // weight: (experts, rows / 128, cols / 128)
-  uint32_t* col_scale_words;  // tokens: (token blocks, cols / 128, 128)
+  uint32_t* col_scale_words;  // tokens: (token blocks, cols / 128, 128); weight: (experts, rows / 128, cols / 128, 128) or null
+  uint32_t* row_scale_words;  // rows in the experts' token blocks: (token blocks, cols / 128, 128)
 };
 
 struct Values {
@@ -89,7 +90,7 @@ __device__ __forceinline__ void load_tile(const void* x, int64_t at, int64_t ld,
 // What the threads of a block share of an activation's tile.
 struct TileShared {
   uint16_t row_by[kBlock];                                  // bf16 multipliers of the tile's rows; a warp reads its own rows' only
-  float row_scale[kBlock];
+  uint8_t row_exponent[kBlock];
   __align__(16) uint32_t col_max[kThreads / 32][kBlock / 2];  // packed bf16: the warps' maxima of two columns
   __align__(16) uint32_t col_by[kBlock / 2];                  // packed bf16 multipliers of two columns
 };
@@ -100,7 +101,9 @@ __device__ __forceinline__ uint16_t by_of(int exponent) {
 
 // A block of rows at a time, its column tiles with a stride of gridDim.y. The values stay packed bf16: maxima by
 // max.xorsign.abs.bf16x2, the product with the scale's reciprocal (a power of two, a bf16 number) by fma.rn.f32.bf16.
-template <bool kRows, bool kTokens>
+enum Rows : int { kNoRows, kRowsInPlace, kRowsInBlocks };
+
+template <int kRows, bool kTokens>
 __device__ __forceinline__ void quantize_activation(const QuantizeParams& p, TileShared* s, int* first_row, int* first_tile, int* tmp) {
   grid_dependency_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, lane16 = lane & 15, row = threadIdx.x >> 4;
@@ -118,6 +121,7 @@ __device__ __forceinline__ void quantize_activation(const QuantizeParams& p, Til
     rows_left = static_cast<int>(min(static_cast<int64_t>(kBlock), p.rows - row0));
   }
   const __nv_bfloat16* x = static_cast<const __nv_bfloat16*>(p.x) + (row0 + row) * p.ld;
+  uint8_t* row_out = p.row_data + ((kRows == kRowsInBlocks ? static_cast<int64_t>(blockIdx.x) * kBlock : row0) + row) * p.cols;
   const int tiles = static_cast<int>((p.cols + kBlock - 1) / kBlock);
   for (int t = blockIdx.y; t < tiles; t += gridDim.y) {
     const int64_t col = static_cast<int64_t>(t) * kBlock + 8 * lane16;
@@ -139,7 +143,7 @@ __device__ __forceinline__ void quantize_activation(const QuantizeParams& p, Til
       if (lane < 16)
         *reinterpret_cast<uint4*>(&s->col_max[warp][4 * lane]) = make_uint4(m[0], m[1], m[2], m[3]);
     }
-    if constexpr (kRows) {
+    if constexpr (kRows != kNoRows) {
       // eight rows' maxima over 16 lanes: each exchange halves the rows that a lane goes on with
       uint32_t m[kRowsPerThread];
 #pragma unroll
@@ -162,19 +166,22 @@ __device__ __forceinline__ void quantize_activation(const QuantizeParams& p, Til
       const int i = ((lane >> 3) & 1) * 4 + ((lane >> 2) & 1) * 2 + ((lane >> 1) & 1);
       __syncwarp();  // the previous tile's multipliers have been read
       if ((lane & 1) == 0)
-        s->row_by[row + 16 * i] = by_of(e), s->row_scale[row + 16 * i] = scale_of(e);
+        s->row_by[row + 16 * i] = by_of(e), s->row_exponent[row + 16 * i] = static_cast<uint8_t>(e);
       __syncwarp();
 #pragma unroll
       for (int k = 0; k < kRowsPerThread; ++k)
-        if (col_ok && row + 16 * k < rows_left) {
+        if (col_ok && (kRows == kRowsInBlocks || row + 16 * k < rows_left)) {
           const uint16_t by = s->row_by[row + 16 * k];
-          *reinterpret_cast<uint2*>(p.row_data + (row0 + row + 16 * k) * p.cols + col) =
+          *reinterpret_cast<uint2*>(row_out + 16 * k * p.cols + col) =
                 make_uint2(e4m3x4_scaled_fma(v[k].x, v[k].y, by, by), e4m3x4_scaled_fma(v[k].z, v[k].w, by, by));
         }
     }
     __syncthreads();
-    if (kRows && threadIdx.x < rows_left)
-      p.row_scale[static_cast<int64_t>(t) * p.rows + row0 + threadIdx.x] = s->row_scale[threadIdx.x];
+    if (kRows == kRowsInPlace && threadIdx.x < rows_left)
+      p.row_scale[static_cast<int64_t>(t) * p.rows + row0 + threadIdx.x] = scale_of(s->row_exponent[threadIdx.x]);
+    if (kRows == kRowsInBlocks && threadIdx.x < kBlock)
+      p.row_scale_words[(static_cast<int64_t>(blockIdx.x) * tiles + t) * kBlock + (threadIdx.x & 31) * 4 + (threadIdx.x >> 5)] =
+            s->row_exponent[threadIdx.x] * 0x01010101u;
     if constexpr (kTokens) {
       if (threadIdx.x < kBlock / 2) {
         uint32_t m = s->col_max[0][threadIdx.x];
@@ -242,8 +249,12 @@ __device__ __forceinline__ void quantize_weight(const QuantizeParams& p, float* 
       *reinterpret_cast<uint2*>(p.col_data + (e * p.rows + row0 + row + 16 * i) * p.cols + col) =
             make_uint2(e4m3x4_from_f32(v[i].v[0] * f, v[i].v[1] * f, v[i].v[2] * f, v[i].v[3] * f),
                        e4m3x4_from_f32(v[i].v[4] * f, v[i].v[5] * f, v[i].v[6] * f, v[i].v[7] * f));
-  if (threadIdx.x == 0)
-    p.col_scale[tile] = scale_of(ex);
+  if (p.col_scale_words == nullptr) {
+    if (threadIdx.x == 0)
+      p.col_scale[tile] = scale_of(ex);
+  } else if (threadIdx.x < kBlock) {
+    p.col_scale_words[tile * kBlock + threadIdx.x] = static_cast<uint32_t>(ex) * 0x01010101u;
+  }
 }
 
 }  // namespace
@@ -251,10 +262,10 @@ __device__ __forceinline__ void quantize_weight(const QuantizeParams& p, float* 
 
 __global__ void __launch_bounds__(mxb200::kThreads) mxb200_block_quantize_rows(const __grid_constant__ mxb200::QuantizeParams p) {
   __shared__ mxb200::TileShared s;
-  mxb200::quantize_activation<true, false>(p, &s, nullptr, nullptr, nullptr);
+  mxb200::quantize_activation<mxb200::kRowsInPlace, false>(p, &s, nullptr, nullptr, nullptr);
 }
 
-template <bool kRows>
+template <int kRows>
 __device__ __forceinline__ void quantize_tokens(const mxb200::QuantizeParams& p) {
   __shared__ int first_row[mxb200::kMaxExperts + 1], first_tile[mxb200::kMaxExperts + 1];
   __shared__ union {
@@ -265,11 +276,15 @@ __device__ __forceinline__ void quantize_tokens(const mxb200::QuantizeParams& p)
 }
 
 __global__ void __launch_bounds__(mxb200::kThreads) mxb200_block_quantize_tokens(const __grid_constant__ mxb200::QuantizeParams p) {
-  quantize_tokens<false>(p);
+  quantize_tokens<mxb200::kNoRows>(p);
 }
 
 __global__ void __launch_bounds__(mxb200::kThreads) mxb200_block_quantize_both(const __grid_constant__ mxb200::QuantizeParams p) {
-  quantize_tokens<true>(p);
+  quantize_tokens<mxb200::kRowsInPlace>(p);
+}
+
+__global__ void __launch_bounds__(mxb200::kThreads) mxb200_block_quantize_both_in_blocks(const __grid_constant__ mxb200::QuantizeParams p) {
+  quantize_tokens<mxb200::kRowsInBlocks>(p);
 }
 
 __global__ void __launch_bounds__(mxb200::kThreads) mxb200_block_quantize_weight_bf16(const __grid_constant__ mxb200::QuantizeParams p) {
@@ -306,7 +321,7 @@ int check_pointers(std::initializer_list<const void*> pointers) {
 }  // namespace mxb200
 
 extern "C" int mxb200_block_quantize(const void* x, int64_t rows, int64_t cols, int64_t ld, const int32_t* ends, int experts,
-                                     void* row_data, float* row_scale, void* token_data, uint32_t* token_scale, void* stream) {
+                                     void* row_data, void* row_scale, int rows_in_blocks, void* token_data, uint32_t* token_scale, void* stream) {
   using namespace mxb200;
   if (rows < 0 || rows > kMost || cols <= 0 || cols > kMost || cols % 16 || ld < cols || ld % 8 || experts < 1 || experts > kMaxExperts)
     return MXB200_ERR_SHAPE;
@@ -317,6 +332,8 @@ extern "C" int mxb200_block_quantize(const void* x, int64_t rows, int64_t cols, 
   const bool want_rows = row_data != nullptr, want_tokens = token_data != nullptr;
   if (!want_rows && !want_tokens)
     return MXB200_ERR_NULL;
+  if (rows_in_blocks != 0 && !(want_rows && want_tokens))
+    return MXB200_ERR_ARGUMENT;
   DeviceInfo dev;
   if (int st = current_device(&dev); st != MXB200_OK)
     return st;
@@ -326,18 +343,27 @@ extern "C" int mxb200_block_quantize(const void* x, int64_t rows, int64_t cols, 
     return st;
   if (int st = want_tokens ? check_pointers({token_data, token_scale}) : MXB200_OK; st != MXB200_OK)
     return st;
-  QuantizeParams p{x, ld, 0, rows, cols, ends, experts, static_cast<uint8_t*>(row_data), row_scale,
-                   static_cast<uint8_t*>(token_data), nullptr, token_scale};
+  QuantizeParams p{};
+  p.x = x, p.ld = ld, p.rows = rows, p.cols = cols, p.ends = ends, p.experts = experts;
+  p.row_data = static_cast<uint8_t*>(row_data);
+  if (rows_in_blocks != 0)
+    p.row_scale_words = static_cast<uint32_t*>(row_scale);
+  else
+    p.row_scale = static_cast<float*>(row_scale);
+  p.col_data = static_cast<uint8_t*>(token_data), p.col_scale_words = token_scale;
   // enough blocks to fill the machine; beyond that a block goes on to its rows' next columns, with its experts looked up once
   const int64_t blocks = want_tokens ? mxb200_block_token_blocks(rows, experts) : up(rows, kBlock);
   const int64_t parts = std::min<int64_t>(up(cols, kBlock), std::max<int64_t>(1, up(8 * dev.sms, blocks)));
   const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(std::min<int64_t>(parts, 65535)));
-  const auto kernel = !want_tokens ? mxb200_block_quantize_rows : want_rows ? mxb200_block_quantize_both : mxb200_block_quantize_tokens;
+  const auto kernel = !want_tokens     ? mxb200_block_quantize_rows
+                      : rows_in_blocks ? mxb200_block_quantize_both_in_blocks
+                      : want_rows      ? mxb200_block_quantize_both
+                                       : mxb200_block_quantize_tokens;
   return launch_kernel(kernel, grid, kThreads, 0, static_cast<cudaStream_t>(stream), p);
 }
 
 extern "C" int mxb200_block_quantize_weight(const void* w, int w_bf16, int experts, int64_t rows, int64_t cols, void* data,
-                                            float* scale, void* stream) {
+                                            void* scale, int in_tiles, void* stream) {
   using namespace mxb200;
   if (rows <= 0 || rows > kMost || cols <= 0 || cols > kMost || rows % 16 || cols % 16 || experts < 1 || experts > kMaxExperts)
     return MXB200_ERR_SHAPE;
@@ -349,7 +375,8 @@ extern "C" int mxb200_block_quantize_weight(const void* w, int w_bf16, int exper
     return st;
   if (int st = check_pointers({w, data, scale}); st != MXB200_OK)
     return st;
-  QuantizeParams p{w, cols, rows * cols, rows, cols, nullptr, experts, nullptr, nullptr, static_cast<uint8_t*>(data), scale, nullptr};
+  QuantizeParams p{w, cols, rows * cols, rows, cols, nullptr, experts, nullptr, nullptr, static_cast<uint8_t*>(data), in_tiles ? nullptr : static_cast<float*>(scale),
+                   in_tiles ? static_cast<uint32_t*>(scale) : nullptr, nullptr};
   return launch_kernel(w_bf16 ? mxb200_block_quantize_weight_bf16 : mxb200_block_quantize_weight_f32, static_cast<unsigned>(tiles),
                        kThreads, 0, static_cast<cudaStream_t>(stream), p);
 }

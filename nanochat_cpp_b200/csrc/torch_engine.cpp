@@ -1041,10 +1041,15 @@ Block new_token_blocks(int64_t rows, int64_t cols, const Experts& e, at::Device 
   return new_block(token_bytes(rows, cols, e), mxb200_block_token_blocks(rows, e.count) * blocks_of(cols) * 128, device);
 }
 
+// Rows as the scaled products take them: in token blocks, with scale tiles. As many bytes as blocks along tokens have.
+Block new_rows_in_blocks(int64_t rows, int64_t cols, const Experts& e, at::Device device) {
+  return new_token_blocks(rows, cols, e, device);
+}
+
 // x (rows, cols) bf16 with contiguous columns into either layout or both.
-void quantize_blocks(const Tensor& x, const Experts& e, const Block& rows, const Block& tokens) {
+void quantize_blocks(const Tensor& x, const Experts& e, const Block& rows, const Block& tokens, bool rows_in_blocks = false) {
   const int64_t ld = x.size(0) > 1 ? x.stride(0) : x.size(1);
-  check(mxb200_block_quantize(x.data_ptr(), x.size(0), x.size(1), ld, e.ends, e.count, rows.data, static_cast<float*>(rows.scale), tokens.data,
+  check(mxb200_block_quantize(x.data_ptr(), x.size(0), x.size(1), ld, e.ends, e.count, rows.data, rows.scale, rows_in_blocks, tokens.data,
                               static_cast<uint32_t*>(tokens.scale), stream()),
         "quantize_block");
 }
@@ -1070,10 +1075,10 @@ void block_product_of(const Tensor& x, const Block& w, const Tensor& y, const Ex
   check(mxb200_block_gemm(&g, stream()), "block_gemm");
 }
 
-void quantize_weight(const Tensor& w_in, const Block& to) {
+void quantize_weight(const Tensor& w_in, const Block& to, bool scale_tiles = false) {
   const Tensor w = dense(w_in.detach());
   check(mxb200_block_quantize_weight(w.data_ptr(), w.scalar_type() == at::kBFloat16, static_cast<int>(w.dim() == 3 ? w.size(0) : 1),
-                                     w.size(-2), w.size(-1), to.data, static_cast<float*>(to.scale), stream()),
+                                     w.size(-2), w.size(-1), to.data, to.scale, scale_tiles, stream()),
         "quantize_block_weight");
 }
 
@@ -1117,28 +1122,30 @@ struct BlockLinear : torch::autograd::Function<BlockLinear> {
     const Experts e = c.experts();
     Block tokens;
     const bool by_product = !grad_w && !c.ends.defined() && !c.x_rows && c.tokens <= MXB200_BLOCK_FEW_TOKENS;
+    // a training pass that quantizes both operands itself, to powers of two: for many tokens the tensor core scales
+    const bool scaled = grad_w && !c.x_rows && !c.w_blocks && mxb200_block_scaled(c.tokens, c.in, c.out, e.count);
     if (!c.x_rows && !by_product) {
-      c.x_rows = new_row_blocks(c.tokens, c.in, c.device);
+      c.x_rows = scaled ? new_rows_in_blocks(c.tokens, c.in, e, c.device) : new_row_blocks(c.tokens, c.in, c.device);
       if (grad_w)
         tokens = new_token_blocks(c.tokens, c.in, e, c.device);
-      quantize_blocks(readable_rows(c.x), grad_w ? e : Experts{}, c.x_rows, tokens);
+      quantize_blocks(readable_rows(c.x), grad_w ? e : Experts{}, c.x_rows, tokens, scaled);
     }
     if (!c.w_blocks) {
       const int64_t matrices = c.w.dim() == 3 ? c.w.size(0) : 1;
-      c.w_blocks = new_block(matrices * c.out * c.in, matrices * blocks_of(c.out) * blocks_of(c.in), c.device);
-      quantize_weight(c.w, c.w_blocks);
+      c.w_blocks = new_block(matrices * c.out * c.in, matrices * blocks_of(c.out) * blocks_of(c.in) * (scaled ? 128 : 1), c.device);
+      quantize_weight(c.w, c.w_blocks, scaled);
     }
     const Tensor y = empty({c.tokens, c.out}, at::kBFloat16, c.device);
     if (by_product)
       block_product_of(readable_rows(c.x), c.w_blocks, y, e, c.tokens, c.in, c.out);
     else
-      block_product(MXB200_BLOCK_FORWARD, c.w_blocks, c.x_rows, y, e, c.tokens, c.in, c.out);
+      block_product(scaled ? MXB200_BLOCK_FORWARD_SCALED : MXB200_BLOCK_FORWARD, c.w_blocks, c.x_rows, y, e, c.tokens, c.in, c.out);
     if (ctx != nullptr) {
       const Tensor none;
       ctx->save_for_backward({grad_x ? c.w_blocks.hold : none, grad_x ? c.w_blocks.hold_scale : none, tokens.hold,
                               grad_w && !tokens ? c.x : none, c.ends});
       const bool bf16 = grad_w && c.w.scalar_type() == at::kBFloat16;
-      ctx->saved_data["sizes"] = std::vector<int64_t>{c.tokens, c.in, c.out, c.ends.defined() ? c.ends.numel() : 0, bf16};
+      ctx->saved_data["sizes"] = std::vector<int64_t>{c.tokens, c.in, c.out, c.ends.defined() ? c.ends.numel() : 0, bf16, scaled};
     }
     return y;
   }
@@ -1157,13 +1164,14 @@ struct BlockLinear : torch::autograd::Function<BlockLinear> {
     const auto device = go.device();
     const Experts e = matrices > 0 ? Experts{static_cast<const int32_t*>(saved[4].data_ptr()), static_cast<int>(matrices)} : Experts{};
     const bool grad_x = saved[0].defined(), grad_w = saved[2].defined() || saved[3].defined();
+    const bool scaled = sizes[5] != 0;  // then the weight gets a gradient too
     Block g_rows, g_tokens;
     if (grad_x)
-      g_rows = new_row_blocks(tokens, out, device);
+      g_rows = scaled ? new_rows_in_blocks(tokens, out, e, device) : new_row_blocks(tokens, out, device);
     if (grad_w)
       g_tokens = new_token_blocks(tokens, out, e, device);
     if (grad_x || grad_w)
-      quantize_blocks(go, grad_w ? e : Experts{}, g_rows, g_tokens);
+      quantize_blocks(go, grad_w ? e : Experts{}, g_rows, g_tokens, scaled && grad_x);
     Tensor dx, dw;
     if (grad_w) {
       Block x_tokens;
@@ -1181,7 +1189,7 @@ struct BlockLinear : torch::autograd::Function<BlockLinear> {
     if (grad_x) {
       dx = empty({tokens, in}, at::kBFloat16, device);
       const Block w = saved[1].defined() ? of_tensors(saved[0], saved[1]) : in_buffer(saved[0], (matrices > 0 ? matrices : 1) * out * in);
-      block_product(MXB200_BLOCK_INPUT_GRAD, w, g_rows, dx, e, tokens, in, out);
+      block_product(scaled ? MXB200_BLOCK_INPUT_GRAD_SCALED : MXB200_BLOCK_INPUT_GRAD, w, g_rows, dx, e, tokens, in, out);
     }
     return {dx, dw, Tensor()};
   }

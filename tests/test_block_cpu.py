@@ -19,13 +19,14 @@ def gemm(**change):
 
 
 @pytest.mark.parametrize("change,status", [
-    (dict(kind=3), capi.ERR_ARGUMENT), (dict(kind=-1), capi.ERR_ARGUMENT), (dict(out_kind=2), capi.ERR_ARGUMENT),
+    (dict(kind=5), capi.ERR_ARGUMENT), (dict(kind=-1), capi.ERR_ARGUMENT), (dict(out_kind=2), capi.ERR_ARGUMENT),
     (dict(out_kind=capi.OUT_F32), capi.ERR_ARGUMENT),
     (dict(tokens=-1), capi.ERR_SHAPE), (dict(tokens=1 << 31), capi.ERR_SHAPE), (dict(in_features=0), capi.ERR_SHAPE),
     (dict(in_features=24), capi.ERR_SHAPE), (dict(out_features=8), capi.ERR_SHAPE), (dict(experts=0), capi.ERR_SHAPE),
     (dict(experts=1025, ends=PTR), capi.ERR_SHAPE), (dict(experts=2), capi.ERR_NULL),
     (dict(b_ld=128, kind=capi.BLOCK_INPUT_GRAD), capi.ERR_ARGUMENT), (dict(b_ld=112), capi.ERR_SHAPE), (dict(b_ld=132), capi.ERR_SHAPE),
-    (dict(b_ld=128, tokens=33), capi.ERR_SHAPE),
+    (dict(b_ld=128, tokens=33), capi.ERR_SHAPE), (dict(b_ld=128, kind=capi.BLOCK_FORWARD_SCALED), capi.ERR_ARGUMENT),
+    (dict(kind=capi.BLOCK_FORWARD_SCALED, out_kind=capi.OUT_F32), capi.ERR_ARGUMENT),
 ])
 def test_gemm_refusals(change, status):
     assert gemm(**change) == status
@@ -37,16 +38,17 @@ def test_gemm_refusals(change, status):
     (4, 128, 128, None, 2, capi.ERR_NULL), (0, 128, 128, None, 1, capi.OK),
 ])
 def test_quantizer_refusals(rows, cols, ld, ends, experts, status):
-    assert lib.mxb200_block_quantize(PTR, rows, cols, ld, ends, experts, PTR, PTR, None, None, None) == status
+    assert lib.mxb200_block_quantize(PTR, rows, cols, ld, ends, experts, PTR, PTR, 0, None, None, None) == status
 
 
 def test_quantizer_needs_an_output():
-    assert lib.mxb200_block_quantize(PTR, 4, 128, 128, None, 1, None, None, None, None, None) == capi.ERR_NULL
+    assert lib.mxb200_block_quantize(PTR, 4, 128, 128, None, 1, None, None, 0, None, None, None) == capi.ERR_NULL
+    assert lib.mxb200_block_quantize(PTR, 4, 128, 128, None, 1, PTR, PTR, 1, None, None, None) == capi.ERR_ARGUMENT
 
 
 @pytest.mark.parametrize("experts,rows,cols", [(0, 128, 128), (1025, 128, 128), (1, 120, 128), (1, 128, 8), (1, 0, 128)])
 def test_weight_quantizer_refusals(experts, rows, cols):
-    assert lib.mxb200_block_quantize_weight(PTR, 1, experts, rows, cols, PTR, PTR, None) == capi.ERR_SHAPE
+    assert lib.mxb200_block_quantize_weight(PTR, 1, experts, rows, cols, PTR, PTR, 0, None) == capi.ERR_SHAPE
 
 
 @pytest.mark.parametrize("rows,cols,status", [(4, 24, capi.ERR_SHAPE), (4, 16400, capi.ERR_SHAPE), (-1, 128, capi.ERR_SHAPE),

@@ -137,6 +137,27 @@ def test_gradients(nc, tokens, cin, cout, dtype):
     assert_product(dw, ref.tokens(dy)[0].t(), ref.tokens(x.detach())[0].t(), "dw")
 
 
+@pytest.mark.parametrize("cin,cout", [(640, 1552), (1040, 2000)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_gradients_scaled_by_the_tensor_core(nc, cin, cout, dtype):
+    tokens, g = 5001, generator(17)
+    assert nc.capi.lib.mxb200_block_scaled(tokens, cin, cout, 1)
+    x = activation(g, tokens, cin).requires_grad_()
+    w = torch.randn(cout, cin, device="cuda", generator=g).to(dtype).requires_grad_()
+    dy = (0.01 * torch.randn(tokens, cout, device="cuda", generator=g)).bfloat16()
+    y = nc.fp8_block_matmul(x, w)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    wv = ref.weight_values(*ref.weight(w.detach()))
+    assert_product(y.detach(), ref.row_values(x.detach()), wv, "y")
+    assert_product(dx, ref.row_values(dy), wv.t(), "dx")
+    assert_product(dw, ref.tokens(dy)[0].t(), ref.tokens(x.detach())[0].t(), "dw")
+    # only one of the gradients wanted
+    one = w.detach().requires_grad_()
+    assert torch.equal(torch.autograd.grad(nc.fp8_block_matmul(x.detach(), one), one, dy)[0], dw)
+    one = x.detach().requires_grad_()
+    assert_product(torch.autograd.grad(nc.fp8_block_matmul(one, w.detach()), one, dy)[0], ref.row_values(dy), wv.t(), "dx")
+
+
 def test_only_the_wanted_gradients(nc):
     g = generator(6)
     x, w = activation(g, 70, 256), torch.randn(128, 256, device="cuda", generator=g)
@@ -270,6 +291,28 @@ def test_experts(nc, counts, tail, cin, cout):
             assert not dw[e].any()
     last = sum(counts)
     assert not y[last:].any() and not dx[last:].any() and not served[last:].any()
+
+
+@pytest.mark.parametrize("tail", [0, 77])
+def test_experts_scaled_by_the_tensor_core(nc, tail):
+    counts, cin, cout, g = [700, 0, 1, 129, 2000, 300, 256, 900, 1200, 0], 1040, 2000, generator(18)
+    rows, ends = sum(counts) + tail, ends_of(counts)
+    assert nc.capi.lib.mxb200_block_scaled(rows, cin, cout, len(counts))
+    x = activation(g, rows, cin).requires_grad_()
+    w = torch.randn(len(counts), cout, cin, device="cuda", generator=g).requires_grad_()
+    dy = (0.01 * torch.randn(rows, cout, device="cuda", generator=g)).bfloat16()
+    y = nc.fp8_block_experts(x, w, ends)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    xr, gr = ref.row_values(x.detach()), ref.row_values(dy)
+    for e, (a, b) in enumerate(ref.spans(ends.tolist(), rows)):
+        wv = ref.weight_values(*ref.weight(w[e].detach()))
+        if b > a:
+            assert_product(y[a:b].detach(), xr[a:b], wv, f"y of expert {e}")
+            assert_product(dx[a:b], gr[a:b], wv.t(), f"dx of expert {e}")
+            assert_product(dw[e], ref.tokens(dy[a:b])[0].t(), ref.tokens(x[a:b].detach())[0].t(), f"dw of expert {e}")
+        else:
+            assert not dw[e].any()
+    assert not y[sum(counts):].any() and not dx[sum(counts):].any()
 
 
 def test_one_expert_is_the_dense_linear(nc):
