@@ -912,6 +912,11 @@ constexpr uint32_t kScaleTile = 512, kScaleBytes = 3 * kScaleTile;
 constexpr uint32_t kAcc1 = 224;  // the second accumulator buffer; the first is at 0
 constexpr uint32_t kScaleA = 480, kScaleB = 484;
 
+// Blocks that a weight gradient sums up in tensor memory at a time; longer sums go on in registers. The tensor core cuts its sums
+// off instead of rounding them, which shortens them by a part of each step's last bit: with all 16384 tokens in one sum dw was
+// 1.1e-6 off (2-norm), with 4096 2.1e-7. The other two products are rounded to bf16.
+constexpr int kSegment = 32;
+
 struct Shared : Common<5> {
   int first_block[kMaxExperts + 2];  // blocks of 128 tokens before an expert's
   LineStage out[kEpilogueWarps];
@@ -1005,34 +1010,36 @@ __device__ __forceinline__ void issue_mmas(const Params& p, Shared* s, uint32_t 
   uint32_t stage = 0, phase = 0, local = 0;
   for (int u = first; u < units; u += step) {
     const int blocks = unit_at<kMode>(p, s, u).blocks;
-    if (blocks == 0)
-      continue;
-    const uint32_t buf = local & 1u;
-    if (!wait_bounded(smem_u32(&s->acc_empty[buf]), ((local >> 1) & 1u) ^ 1u, &s->abort_flag, kSiteAccEmpty) ||
-        (local > 0 && !wait_bounded(smem_u32(&s->overlap_free), (local - 1) & 1u, &s->abort_flag, kSiteOverlap)))
-      return;
-    ++local;
-    for (int b = 0; b < blocks; ++b) {
-      if (!wait_bounded(full0 + stage * 8, phase, &s->abort_flag, kSiteStageFull))
+    for (int b = 0; b < blocks;) {
+      const uint32_t buf = local & 1u;
+      if (!wait_bounded(smem_u32(&s->acc_empty[buf]), ((local >> 1) & 1u) ^ 1u, &s->abort_flag, kSiteAccEmpty) ||
+          (local > 0 && !wait_bounded(smem_u32(&s->overlap_free), (local - 1) & 1u, &s->abort_flag, kSiteOverlap)))
         return;
-      tcgen05_fence_after_sync();
-      const uint64_t sf = sf_desc0 + stage * (kScaleBytes >> 4);
-      tcgen05_cp_32x128b_warpx4_pair(el, sfa, sf);
-      tcgen05_cp_32x128b_warpx4_pair(el, sfb, sf + (kScaleTile >> 4));
-      tcgen05_cp_32x128b_warpx4_pair(el, sfb + 4, sf + 2 * (kScaleTile >> 4));
-      const uint64_t a = a_desc0 + stage * (kABytes >> 4), bd = b_desc0 + stage * (kBBytes >> 4);
+      ++local;
+      const int begin = b, end = kMode == kWeightGrad ? min(b + kSegment, blocks) : blocks;
+      for (; b < end; ++b) {
+        if (!wait_bounded(full0 + stage * 8, phase, &s->abort_flag, kSiteStageFull))
+          return;
+        tcgen05_fence_after_sync();
+        const uint64_t sf = sf_desc0 + stage * (kScaleBytes >> 4);
+        tcgen05_cp_32x128b_warpx4_pair(el, sfa, sf);
+        tcgen05_cp_32x128b_warpx4_pair(el, sfb, sf + (kScaleTile >> 4));
+        tcgen05_cp_32x128b_warpx4_pair(el, sfb + 4, sf + 2 * (kScaleTile >> 4));
+        const uint64_t a = a_desc0 + stage * (kABytes >> 4), bd = b_desc0 + stage * (kBBytes >> 4);
 #pragma unroll
-      for (uint32_t k = 0; k < 4; ++k)
-        tcgen05_mma_mxf8_pair(el, tmem_base + buf * kAcc1, a + k * kAStep, bd + k * kBStep, idesc, sfa, sfb, b > 0 || k > 0);
-      tcgen05_commit_pair(el, empty0 + stage * 8, 3);
-      if (++stage == Shared::kStages)
-        stage = 0, phase ^= 1u;
+        for (uint32_t k = 0; k < 4; ++k)
+          tcgen05_mma_mxf8_pair(el, tmem_base + buf * kAcc1, a + k * kAStep, bd + k * kBStep, idesc, sfa, sfb, b > begin || k > 0);
+        tcgen05_commit_pair(el, empty0 + stage * 8, 3);
+        if (++stage == Shared::kStages)
+          stage = 0, phase ^= 1u;
+      }
+      tcgen05_commit_pair(el, &s->acc_full[buf], 3);
     }
-    tcgen05_commit_pair(el, &s->acc_full[buf], 3);
   }
 }
 
-template <int kMode>
+// kLong: weight gradients whose sums may take more than a segment.
+template <int kMode, bool kLong>
 __device__ __forceinline__ void store(const Params& p, Shared* s, uint32_t tmem_base, int rank, int first, int step, int units, int warp, int lane) {
   const int quarter = warp & 3, part = (warp - kFirstEpilogueWarp) >> 2;
   const uint32_t t0 = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
@@ -1043,6 +1050,57 @@ __device__ __forceinline__ void store(const Params& p, Shared* s, uint32_t tmem_
   uint32_t local = 0;
   for (int u = first; u < units; u += step) {
     const Unit x = unit_at<kMode>(p, s, u);
+    const int row = rank * 128 + quarter * 32, rows = x.rows - row;
+    const int64_t line = static_cast<int64_t>(columns) * (bf16 ? 2 : 4);
+    unsigned char* d = static_cast<unsigned char*>(p.d) + ((kMode == kWeightGrad ? static_cast<int64_t>(x.expert) * p.features : 0) + x.m0 + row) * line +
+                       static_cast<int64_t>(x.n0) * (bf16 ? 2 : 4);
+    if constexpr (kLong) {
+      float sum[4][32];
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int k = 0; k < 32; ++k)
+          sum[c][k] = 0.f;
+      for (int b = 0; b < x.blocks; b += kSegment, ++local) {
+        const uint32_t buf = local & 1u;
+        if (!wait_bounded(smem_u32(&s->acc_full[buf]), (local >> 1) & 1u, &s->abort_flag, kSiteAccFull))
+          return;
+        tcgen05_fence_after_sync();
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t v[32];
+          tmem_ld_32x32b_x32(t0 + buf * kAcc1 + 128 * part + 32 * c, v);
+          tmem_ld_wait(v);
+          if (c == 0 || c == 3) {
+            tcgen05_fence_before_sync();
+            __syncwarp();
+            if (lane == 0 && c == (buf == 0 ? 3 : 0) && part == static_cast<int>(1 - buf))
+              mbar_arrive_cluster(overlap_free);
+            if (lane == 0 && c == 3)
+              mbar_arrive_cluster(acc_empty0 + buf * 8);
+          }
+#pragma unroll
+          for (int k = 0; k < 32; ++k)
+            sum[c][k] += __uint_as_float(v[k]);
+        }
+      }
+      if (!bf16) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          store_lines(stage, lane, d + 128 * (c + 4 * part), line, rows, (columns - x.n0 - 32 * (c + 4 * part)) * 4, [&](int q) {
+            return make_uint4(__float_as_uint(sum[c][4 * q]), __float_as_uint(sum[c][4 * q + 1]), __float_as_uint(sum[c][4 * q + 2]),
+                              __float_as_uint(sum[c][4 * q + 3]));
+          });
+      } else {
+#pragma unroll
+        for (int c = 0; c < 4; c += 2)
+          store_lines(stage, lane, d + 64 * (c + 4 * part), line, rows, (columns - x.n0 - 32 * (c + 4 * part)) * 2, [&](int q) {
+            const float* f = &sum[c + (q >> 2)][8 * (q & 3)];
+            return make_uint4(pack_bf16x2_rn(f[0], f[1]), pack_bf16x2_rn(f[2], f[3]), pack_bf16x2_rn(f[4], f[5]), pack_bf16x2_rn(f[6], f[7]));
+          });
+      }
+      continue;
+    }
     const uint32_t buf = local & 1u;
     if (x.blocks > 0) {
       if (!wait_bounded(smem_u32(&s->acc_full[buf]), (local >> 1) & 1u, &s->abort_flag, kSiteAccFull))
@@ -1050,10 +1108,6 @@ __device__ __forceinline__ void store(const Params& p, Shared* s, uint32_t tmem_
       tcgen05_fence_after_sync();
       ++local;
     }
-    const int row = rank * 128 + quarter * 32, rows = x.rows - row;
-    const int64_t line = static_cast<int64_t>(columns) * (bf16 ? 2 : 4);
-    unsigned char* d = static_cast<unsigned char*>(p.d) + ((kMode == kWeightGrad ? static_cast<int64_t>(x.expert) * p.features : 0) + x.m0 + row) * line +
-                       static_cast<int64_t>(x.n0) * (bf16 ? 2 : 4);
     uint32_t half[16];  // bf16: the first 32 columns of a line
 #pragma unroll 1
     for (int i = 0; i < 4; ++i) {
@@ -1108,7 +1162,7 @@ __device__ __forceinline__ void store(const Params& p, Shared* s, uint32_t tmem_
   }
 }
 
-template <int kMode>
+template <int kMode, bool kLong>
 __device__ __forceinline__ void body(const Params& p, const Maps& maps) {
   extern __shared__ unsigned char smem_raw[];
   unsigned char* base = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
@@ -1120,12 +1174,18 @@ __device__ __forceinline__ void body(const Params& p, const Maps& maps) {
   const uint32_t tmem_base = set_up<2>(p, &maps.a, &maps.b, s, base, warp, set, true, s->first_block);
   const int units = kMode == kWeightGrad ? p.experts * ((p.features + kTile - 1) / kTile) * ((p.n + kTile - 1) / kTile) : units_of(p, s, kTile);
   const int first = blockIdx.x / 2, step = gridDim.x / 2;
-  if (warp == 0)
-    load_operands<kMode>(p, maps, s, a0, rank, first, step, units);
-  else if (warp == 1 && rank == 0)
-    issue_mmas<kMode>(p, s, a0, tmem_base, first, step, units);
-  else if (warp >= kFirstEpilogueWarp)
-    store<kMode>(p, s, tmem_base, rank, first, step, units, warp, lane);
+  if (warp < kFirstEpilogueWarp) {
+    if constexpr (kLong)
+      set_max_registers_down<kFewRegisters>();
+    if (warp == 0)
+      load_operands<kMode>(p, maps, s, a0, rank, first, step, units);
+    else if (warp == 1 && rank == 0)
+      issue_mmas<kMode>(p, s, a0, tmem_base, first, step, units);
+  } else {
+    if constexpr (kLong)
+      set_max_registers_up<kManyRegisters>();
+    store<kMode, kLong>(p, s, tmem_base, rank, first, step, units, warp, lane);
+  }
   tear_down<2>(s, tmem_base, warp, true);
 }
 
@@ -1161,15 +1221,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(mxb200::kThreads, 1)
 }
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(mxb200::kThreads, 1)
       mxb200_block_gemm_weight_grad(const __grid_constant__ mxb200::Launch args) {
-  mxb200::scaled::body<mxb200::kWeightGrad>(args.p, args.maps);
+  mxb200::scaled::body<mxb200::kWeightGrad, false>(args.p, args.maps);
+}
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(mxb200::kThreads, 1)
+      mxb200_block_gemm_weight_grad_long(const __grid_constant__ mxb200::Launch args) {
+  mxb200::scaled::body<mxb200::kWeightGrad, true>(args.p, args.maps);
 }
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(mxb200::kThreads, 1)
       mxb200_block_gemm_forward_scaled(const __grid_constant__ mxb200::Launch args) {
-  mxb200::scaled::body<mxb200::kForward>(args.p, args.maps);
+  mxb200::scaled::body<mxb200::kForward, false>(args.p, args.maps);
 }
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(mxb200::kThreads, 1)
       mxb200_block_gemm_input_grad_scaled(const __grid_constant__ mxb200::Launch args) {
-  mxb200::scaled::body<mxb200::kInputGrad>(args.p, args.maps);
+  mxb200::scaled::body<mxb200::kInputGrad, false>(args.p, args.maps);
 }
 
 namespace mxb200 {
@@ -1218,7 +1282,7 @@ struct Variant {
   int tokens, features; // of a unit
 };
 
-enum VariantId : int { kForwardFew, kForward32, kForwardMany, kForwardQuantizing, kInputGradFew, kInputGradMany, kWeightGradPair, kForwardScaled, kInputGradScaled, kVariants };
+enum VariantId : int { kForwardFew, kForward32, kForwardMany, kForwardQuantizing, kInputGradFew, kInputGradMany, kWeightGradPair, kWeightGradLong, kForwardScaled, kInputGradScaled, kVariants };
 
 const Variant& variant(VariantId id) {
   static const Variant variants[kVariants] = {
@@ -1229,6 +1293,7 @@ const Variant& variant(VariantId id) {
         {mxb200_block_gemm_input_grad_few, few::Tile128::kSmemBytes, 1, few::Tile128::kTileT, few::kTileF},
         {mxb200_block_gemm_input_grad_many, many::kSmemBytes, 2, many::kTileT, many::kTileF},
         {mxb200_block_gemm_weight_grad, scaled::kSmemBytes, 2, scaled::kTile, scaled::kTile},
+        {mxb200_block_gemm_weight_grad_long, scaled::kSmemBytes, 2, scaled::kTile, scaled::kTile},
         {mxb200_block_gemm_forward_scaled, scaled::kSmemBytes, 2, scaled::kTile, scaled::kTile},
         {mxb200_block_gemm_input_grad_scaled, scaled::kSmemBytes, 2, scaled::kTile, scaled::kTile}};
   return variants[id];
@@ -1351,7 +1416,7 @@ int block_gemm(const mxb200_block_gemm_args& g, cudaStream_t stream) {
   const auto most_tiles = [&](int64_t tile) {
     return g.ends == nullptr ? up(g.tokens, tile) : (g.tokens + (tile - 1) * std::min<int64_t>(g.experts + 1, g.tokens)) / tile;
   };
-  VariantId id = kWeightGradPair;
+  VariantId id = g.tokens <= mxb200::scaled::kSegment * kBlock ? kWeightGradPair : kWeightGradLong;
   Configured configured;
   int64_t units;
   int st;

@@ -158,6 +158,21 @@ def test_gradients_scaled_by_the_tensor_core(nc, cin, cout, dtype):
     assert_product(torch.autograd.grad(nc.fp8_block_matmul(one, w.detach()), one, dy)[0], ref.row_values(dy), wv.t(), "dx")
 
 
+def test_long_sums_do_not_lose_precision(nc):
+    """The tensor core cuts its running sums off, an error that grows with their length; beyond 4096 tokens they go on in
+    registers, so that 16384 tokens' gradient is as good as 4096's (and 4500's last segment is short)."""
+    def error(tokens):
+        g = generator(tokens)
+        x = torch.randn(tokens, 256, device="cuda", generator=g).bfloat16()
+        w = torch.randn(256, 256, device="cuda", generator=g).requires_grad_()
+        dy = torch.randn(tokens, 256, device="cuda", generator=g).bfloat16()
+        dw, = torch.autograd.grad(nc.fp8_block_matmul(x, w), w, dy)
+        want = ref.tokens(dy)[0].t() @ ref.tokens(x)[0]
+        return float((dw.double() - want).norm() / want.norm())
+    short = error(4096)
+    assert error(4500) <= 1.5 * short and error(16384) <= 1.5 * short
+
+
 def test_only_the_wanted_gradients(nc):
     g = generator(6)
     x, w = activation(g, 70, 256), torch.randn(128, 256, device="cuda", generator=g)
