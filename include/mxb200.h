@@ -301,7 +301,7 @@ typedef enum mxb200_block_kind {
 /* Whether the scaled kinds are the faster ones for a Linear's forward and input gradient of this size on the current device. */
 MXB200_API int mxb200_block_scaled(int64_t tokens, int64_t in_features, int64_t out_features, int experts);
 
-#define MXB200_BLOCK_FEW_TOKENS 32
+#define MXB200_BLOCK_FEW_TOKENS 16
 
 /* One product per expert over its rows, fp32 accumulation, rounded once. Rows of no expert: zeros; the weight gradient of an
  * expert without rows: zeros. Needs no workspace. tokens may be 0. */

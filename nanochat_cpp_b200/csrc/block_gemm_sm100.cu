@@ -315,8 +315,8 @@ __device__ __forceinline__ void store_lines(LineStage* stage, int lane, unsigned
 // memory, and adds up every n-th token of all of them, always in the cluster's order.
 //
 // kQuantize: the input comes in bf16 and is quantized on its way into shared memory, by the four warps that would accumulate
-// the second half of the columns: up to 32 tokens per tile. That spares a launch, and for a token or two the work is nothing
-// although every CTA repeats it.
+// the second half of the columns: up to 16 tokens. That spares a launch, about 2 us on the device and as much on the host; every
+// CTA's repeating it costs 0.5 us for one token and 2 for 16 (1536 -> 1536).
 
 namespace few {
 
@@ -412,53 +412,51 @@ __device__ __forceinline__ void load_scales(const Params& p, typename C::Shared*
   }
 }
 
-// The input's blocks from bf16 into shared memory as a TMA load would leave them (128-byte swizzle), and their scales: 16 lanes
-// per token, 8 tokens at a time, a block ahead in registers. The values are block_quantize_sm100.cu's.
+// The input's blocks from bf16 into shared memory as a TMA load would leave them (128-byte swizzle), and their scales. Each of
+// the four warps has every fourth block to itself, 16 lanes per token, so that the way of one block (maxima, scale, proxy fence)
+// is covered by the others'; with all four at one block a block took 0.47 us instead of 0.33. The values are
+// block_quantize_sm100.cu's.
 template <typename C>
 __device__ __forceinline__ void quantize(const Params& p, typename C::Shared* s, unsigned char* b_stages, const Place& at, int units, int warp,
                                          int lane) {
-  static_assert(C::kTileT == 32, "four tokens per thread");
+  static_assert(MXB200_BLOCK_FEW_TOKENS <= C::kTileT && C::Shared::kStages % 4 == 0 && kScaleSlots % 4 == 0, "whole turns of the rings");
+  constexpr int kPasses = MXB200_BLOCK_FEW_TOKENS / 2;
   const uint32_t full0 = smem_u32(&s->full[0]), empty0 = smem_u32(&s->empty[0]);
   const uint32_t scale_full0 = smem_u32(&s->scale_full[0]), scale_empty0 = smem_u32(&s->scale_empty[0]);
-  const int lane16 = lane & 15, token0 = 2 * (warp & 3) + (lane >> 4);
+  const int lane16 = lane & 15, token0 = lane >> 4;
   const int in = p.input_cols;
   const uint16_t* input = static_cast<const uint16_t*>(p.input);
-  uint4 ahead[4];
+  uint4 ahead[kPasses];
   float weight_ahead = 0.f;
   const auto fetch = [&](const Unit& x, int b) {
     const int col = b * kBlock + 8 * lane16;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int t = token0 + 8 * i;
+    for (int i = 0; i < kPasses; ++i) {
+      const int t = token0 + 2 * i;
       ahead[i] = t < x.rows && col < in ? *reinterpret_cast<const uint4*>(input + (x.row0 + t) * p.token_ld + col) : make_uint4(0, 0, 0, 0);
     }
     weight_ahead = *weight_scale(p, x, b);
   };
-  uint32_t stage = 0, phase = 0, slot = 0, slot_phase = 0;
+  uint32_t before = 0;  // blocks of the units before this one
   for (int u = at.cluster; u < units; u += at.clusters) {
     const Unit x = unit_at<C::kTileT, kTileF>(p, s, u);
-    const int end = at.end(x.blocks);
-    int b = at.begin(x.blocks);
+    const int begin = at.begin(x.blocks), end = at.end(x.blocks);
+    int b = begin + static_cast<int>(((warp & 3) - before) & 3u);
+    uint32_t n = before + (b - begin);
     if (b < end)
       fetch(x, b);
-    for (; b < end; ++b) {
-      uint4 now[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        now[i] = ahead[i];
-      const float weight = weight_ahead;
-      if (b + 1 < end)
-        fetch(x, b + 1);
-      if (!wait_bounded(empty0 + stage * 8, phase ^ 1u, &s->abort_flag, kSiteStageEmpty) ||
-          !wait_bounded(scale_empty0 + slot * 8, slot_phase ^ 1u, &s->abort_flag, kSiteScaleEmpty))
+    for (; b < end; b += 4, n += 4) {
+      const uint32_t stage = n % C::Shared::kStages, slot = n % kScaleSlots;
+      if (!wait_bounded(empty0 + stage * 8, (n / C::Shared::kStages & 1u) ^ 1u, &s->abort_flag, kSiteStageEmpty) ||
+          !wait_bounded(scale_empty0 + slot * 8, (n / kScaleSlots & 1u) ^ 1u, &s->abort_flag, kSiteScaleEmpty))
         return;
       unsigned char* to = b_stages + stage * C::kStageBBytes;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (8 * i >= x.rows)
+      for (int i = 0; i < kPasses; ++i) {
+        if (2 * i >= x.rows)
           break;
-        const int t = token0 + 8 * i;
-        const uint32_t w[4] = {now[i].x, now[i].y, now[i].z, now[i].w};
+        const int t = token0 + 2 * i;
+        const uint32_t w[4] = {ahead[i].x, ahead[i].y, ahead[i].z, ahead[i].w};
         uint32_t m = max_abs_skip_nan_bf16x2(max_abs_skip_nan_bf16x2(max_abs_skip_nan_bf16x2(max_abs_skip_nan_bf16x2(0u, w[0]), w[1]), w[2]), w[3]);
         m &= 0x7fff7fffu;
         m = max(m & 0xffffu, m >> 16);
@@ -472,19 +470,18 @@ __device__ __forceinline__ void quantize(const Params& p, typename C::Shared* s,
         if (lane16 == 0)
           s->scales[slot].token[t] = __uint_as_float(static_cast<uint32_t>(e) << 23);
       }
-      if (threadIdx.x == 32 * (kFirstEpilogueWarp + C::kWarps))
-        s->scales[slot].weight = weight;
+      if (lane == 0)
+        s->scales[slot].weight = weight_ahead;
+      if (b + 4 < end)
+        fetch(x, b + 4);
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
         mbar_arrive_addr(full0 + stage * 8);
         mbar_arrive_addr(scale_full0 + slot * 8);
       }
-      if (++stage == C::Shared::kStages)
-        stage = 0, phase ^= 1u;
-      if (++slot == kScaleSlots)
-        slot = 0, slot_phase ^= 1u;
     }
+    before += static_cast<uint32_t>(end - begin);
   }
 }
 
@@ -676,9 +673,9 @@ __device__ __forceinline__ void body(const Params& p, const CUtensorMap* map_w, 
     mbar_init(&s->partial_full, C::kWarps * p.splits);
     mbar_init(&s->partial_empty, C::kWarps * p.splits);
   }
-  SetUp set{1, 1, C::kWarps, C::kAccBuffers, C::kQuantize ? 4u : 32u, C::kTileT, true};
+  SetUp set{1, 1, C::kWarps, C::kAccBuffers, C::kQuantize ? 1u : 32u, C::kTileT, true};
   if (C::kQuantize)
-    set.full_arrivals = 5;  // the weight's load and four warps
+    set.full_arrivals = 2;  // the weight's load and the block's warp
   const uint32_t tmem_base = set_up<1>(p, map_w, map_t, s, base, warp, set, p.splits > 1);
   const int units = units_of(p, s, kTileF);
   if (warp == 0)
@@ -698,7 +695,7 @@ __device__ __forceinline__ void body(const Params& p, const CUtensorMap* map_w, 
 
 using Tile128 = Config<128, false>;
 using Tile32 = Config<32, false>;
-using Quantizing = Config<MXB200_BLOCK_FEW_TOKENS, true>;
+using Quantizing = Config<32, true>;
 
 }  // namespace few
 

@@ -381,7 +381,7 @@ Backward backward_of(int cols) {
   const int vecs = cols / 8;
   const auto threads = [&](int per_thread) { return ((vecs + per_thread - 1) / per_thread + 31) / 32 * 32; };
   if (vecs <= kThreads)
-    return {mxb200_block_norm_bwd_1x2, threads(1), 2, std::min(8, 768 / threads(1))};
+    return {mxb200_block_norm_bwd_1x2, threads(1), 2, std::min(8, 512 / threads(1))};
   if (vecs <= 2 * kThreads)
     return {mxb200_block_norm_bwd_2x1, threads(2), 1, 2};
   if (vecs <= 4 * kThreads)

@@ -99,7 +99,7 @@ def test_forward(nc, tokens, cin, cout):
     assert torch.equal(y, again)
 
 
-@pytest.mark.parametrize("tokens", [1, 5, 8, 17, 31, 32])
+@pytest.mark.parametrize("tokens", [1, 2, 5, 8, 15, 16])
 @pytest.mark.parametrize("cin,cout", [(16, 16), (144, 272), (1536, 1536), (2064, 400), (6144, 128)])
 def test_quantized_by_the_product(nc, tokens, cin, cout):
     """The C entry that takes bf16 rows: the bits of quantizing first, dense and by expert."""
