@@ -9,8 +9,13 @@
 
 namespace mxb200 {
 
-constexpr int kBlock = 128;         // values per scale along the quantized axis
+constexpr int kBlock = 128;  // values per scale along the quantized axis
 constexpr int kMaxExperts = 1024;
+constexpr int64_t kMostSize = int64_t{1} << 30;  // of a dimension, and of a launch's tiles
+
+constexpr int64_t blocks_up(int64_t n, int64_t d) {
+  return (n + d - 1) / d;
+}
 
 // Biased exponent of the scale of a block: the smallest power of two with max|block| <= 448 scale, as for MX, but not below
 // 2^-126, so that the scale is a normal fp32 number (the reciprocal is one up to 2^126).

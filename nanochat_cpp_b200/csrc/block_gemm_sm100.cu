@@ -104,7 +104,8 @@ struct Params {
 
 struct Maps {
   CUtensorMap a, b;
-  CUtensorMap a_scale, b_scale;  // weight gradient
+  CUtensorMap a_scale, b_scale;  // scales in the tensor core
+  CUtensorMap d;                 // many tokens: the output, 32 tokens x 64 features
 };
 
 // A warp's wait for a barrier phase, given up after kWaitLimitNs; its lanes agree on the outcome. kCluster: what other CTAs of
@@ -715,12 +716,15 @@ struct __align__(16) ScaleSlot {
   float weight[2];
 };
 
+// A warp's output on its way: 32 tokens x 64 features in the 128-byte swizzle of a TMA store.
+constexpr uint32_t kOutStageBytes = 32 * 128;
+
 struct Shared : Common<5> {
   ScaleSlot scales[kScaleSlots];
-  LineStage out[kEpilogueWarps];
 };
 
-constexpr size_t kSmemBytes = 1024 + Shared::kStages * static_cast<size_t>(kABytes + kBBytes) + sizeof(Shared);
+constexpr size_t kOperandBytes = Shared::kStages * static_cast<size_t>(kABytes + kBBytes);
+constexpr size_t kSmemBytes = 1024 + kOperandBytes + kEpilogueWarps * kOutStageBytes + sizeof(Shared);
 static_assert(kSmemBytes <= 232448, "shared memory of one CTA");
 
 template <int kMode>
@@ -804,8 +808,8 @@ __device__ __forceinline__ void issue_mmas(const Params& p, Shared* s, uint32_t 
   }
 }
 
-__device__ __forceinline__ void accumulate(const Params& p, Shared* s, uint32_t tmem_base, int rank, int first, int step, int units, int warp,
-                                           int lane) {
+__device__ __forceinline__ void accumulate(const Params& p, const CUtensorMap* map_d, Shared* s, unsigned char* out, uint32_t tmem_base, int rank,
+                                           int first, int step, int units, int warp, int lane) {
   const int quarter = warp & 3, part = (warp - kFirstEpilogueWarp) >> 2;
   const uint32_t t0 = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + part * 128;
   const uint32_t acc_empty0 = map_to_cta(smem_u32(&s->acc_empty[0]), 0);
@@ -850,28 +854,54 @@ __device__ __forceinline__ void accumulate(const Params& p, Shared* s, uint32_t 
         slot = 0, slot_phase ^= 1u;
     }
     const int row = rank * 128 + quarter * 32, feature = x.f0 + part * 128;
-    unsigned char* d = static_cast<unsigned char*>(p.d) + (static_cast<int64_t>(x.row0 + row) * p.features + feature) * 2;
+    unsigned char* stage = out + (warp - kFirstEpilogueWarp) * kOutStageBytes;
 #pragma unroll
-    for (int c = 0; c < kChunks; c += 2)
-      store_lines(&s->out[warp - kFirstEpilogueWarp], lane, d + 64 * c, static_cast<int64_t>(p.features) * 2, x.rows - row,
-                  (p.features - feature - 32 * c) * 2, [&](int q) {
-                    uint32_t h[4];
+    for (int c = 0; c < kChunks; c += 2) {
+      if (lane == 0)
+        tma_store_wait_read<0>();  // the stage has been read out
+      __syncwarp();
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                      const float2 o = both(acc[c + (q >> 2)][4 * (q & 3) + j]);
-                      h[j] = pack_bf16x2_rn(o.x, o.y);
-                    }
-                    return make_uint4(h[0], h[1], h[2], h[3]);
-                  });
+      for (int q = 0; q < 8; ++q) {
+        uint32_t h[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 o = both(acc[c + (q >> 2)][4 * (q & 3) + j]);
+          h[j] = pack_bf16x2_rn(o.x, o.y);
+        }
+        *reinterpret_cast<uint4*>(stage + lane * 128 + ((q ^ (lane & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      const int left = p.features - feature - 32 * c;  // columns that exist
+      if (row + 32 <= x.rows) {
+        // all tokens there: handed to the copy engine, and the next unit's blocks are taken up meanwhile
+        if (lane == 0 && left > 0) {
+          tma_store_2d(map_d, stage, feature + 32 * c, x.row0 + row);
+          tma_store_commit();
+        }
+      } else {
+        // the tile ends within the warp's tokens, behind which lie another expert's
+#pragma unroll 1
+        for (int r = lane >> 3; r < x.rows - row; r += 4) {
+          const int q = lane & 7;
+          const uint4 w = *reinterpret_cast<const uint4*>(stage + r * 128 + ((q ^ (r & 7)) << 4));
+          if (8 * q < left)
+            *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.d) + static_cast<int64_t>(x.row0 + row + r) * p.features + feature + 32 * c + 8 * q) = w;
+        }
+      }
+    }
   }
+  if (lane == 0)
+    tma_store_wait_all<0>();
 }
 
 template <int kMode>
-__device__ __forceinline__ void body(const Params& p, const CUtensorMap* map_t, const CUtensorMap* map_w) {
+__device__ __forceinline__ void body(const Params& p, const CUtensorMap* map_t, const CUtensorMap* map_w, const CUtensorMap* map_d) {
   extern __shared__ unsigned char smem_raw[];
   unsigned char* base = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   const uint32_t a0 = smem_u32(base), b0 = a0 + Shared::kStages * kABytes;
-  Shared* s = reinterpret_cast<Shared*>(base + Shared::kStages * (kABytes + kBBytes));
+  unsigned char* out = base + kOperandBytes;
+  Shared* s = reinterpret_cast<Shared*>(out + kEpilogueWarps * kOutStageBytes);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = static_cast<int>(cluster_ctarank());
   const SetUp set{1, 1, 2 * kEpilogueWarps, kAccBuffers, 32, kTileT, true};
@@ -887,7 +917,7 @@ __device__ __forceinline__ void body(const Params& p, const CUtensorMap* map_t, 
       load_scales(p, s, rank, first, step, units, lane);
   } else {
     set_max_registers_up<kManyRegisters>();
-    accumulate(p, s, tmem_base, rank, first, step, units, warp, lane);
+    accumulate(p, map_d, s, out, tmem_base, rank, first, step, units, warp, lane);
   }
   tear_down<2>(s, tmem_base, warp, true);
 }
@@ -1210,11 +1240,11 @@ __global__ void __launch_bounds__(mxb200::kThreads, 1) mxb200_block_gemm_input_g
 }
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(mxb200::kThreads, 1)
       mxb200_block_gemm_forward_many(const __grid_constant__ mxb200::Launch args) {
-  mxb200::many::body<mxb200::kForward>(args.p, &args.maps.a, &args.maps.b);
+  mxb200::many::body<mxb200::kForward>(args.p, &args.maps.a, &args.maps.b, &args.maps.d);
 }
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(mxb200::kThreads, 1)
       mxb200_block_gemm_input_grad_many(const __grid_constant__ mxb200::Launch args) {
-  mxb200::many::body<mxb200::kInputGrad>(args.p, &args.maps.a, &args.maps.b);
+  mxb200::many::body<mxb200::kInputGrad>(args.p, &args.maps.a, &args.maps.b, &args.maps.d);
 }
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(mxb200::kThreads, 1)
       mxb200_block_gemm_weight_grad(const __grid_constant__ mxb200::Launch args) {
@@ -1251,8 +1281,18 @@ int make_map(CUtensorMap* map, const void* base, int64_t x, int64_t y, int64_t z
   return r == CUDA_SUCCESS ? MXB200_OK : MXB200_ERR_DRIVER;
 }
 
-int64_t up(int64_t n, int64_t d) {
-  return (n + d - 1) / d;
+// The (tokens, features) bf16 output, 32 tokens x 64 features at a time, 128-byte swizzle.
+int make_output_map(CUtensorMap* map, void* base, int64_t features, int64_t tokens) {
+  EncodeTiledFn fn = encode_fn();
+  if (fn == nullptr)
+    return MXB200_ERR_DRIVER;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(features), static_cast<cuuint64_t>(tokens)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(features) * 2};
+  const cuuint32_t box[2] = {64, 32};
+  const cuuint32_t estr[2] = {1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? MXB200_OK : MXB200_ERR_DRIVER;
 }
 
 // (z, y) scale tiles of 128 words, `box_z` x `box_y` at a time.
@@ -1300,7 +1340,7 @@ const Variant& variant(VariantId id) {
 // half a tile left over.
 int64_t expected_tiles(int64_t tokens, int experts, int tile) {
   const int64_t used = std::min<int64_t>(experts, tokens);
-  return experts == 1 ? up(tokens, tile) : std::max(used, tokens / tile + used / 2);
+  return experts == 1 ? blocks_up(tokens, tile) : std::max(used, tokens / tile + used / 2);
 }
 
 // Which of the two kernels a product of `blocks` contraction blocks to `features` features takes: the one that is expected to be
@@ -1310,7 +1350,7 @@ int64_t expected_tiles(int64_t tokens, int experts, int tile) {
 // 64: 39 and 54.
 bool many_tokens(int64_t tokens, int experts, int features, int blocks, int sms) {
   const auto time = [&](const Variant& v, double out_blocks, double start) {
-    return start + static_cast<double>(up(expected_tiles(tokens, experts, v.tokens) * up(features, v.features), sms / v.ctas)) * (blocks + out_blocks) * 0.45;
+    return start + static_cast<double>(blocks_up(expected_tiles(tokens, experts, v.tokens) * blocks_up(features, v.features), sms / v.ctas)) * (blocks + out_blocks) * 0.45;
   };
   return time(variant(kForwardMany), 4, 4.5) < time(variant(kForwardFew), 3, 4);
 }
@@ -1361,7 +1401,7 @@ int share_blocks(int64_t units, int blocks, int tile_tokens, const Configured& c
   int best = 1;
   double least = 0.3 * blocks;
   for (int n = 2; n <= std::min(kMostSplits, blocks) && units <= c.clusters[n]; ++n)
-    if (const double t = 0.3 * static_cast<double>(up(blocks, n)) + 2 + 0.02 * tile_tokens; t < least)
+    if (const double t = 0.3 * static_cast<double>(blocks_up(blocks, n)) + 2 + 0.02 * tile_tokens; t < least)
       best = n, least = t;
   return best;
 }
@@ -1370,9 +1410,8 @@ int block_gemm(const mxb200_block_gemm_args& g, cudaStream_t stream) {
   if (g.kind < MXB200_BLOCK_FORWARD || g.kind > MXB200_BLOCK_INPUT_GRAD_SCALED ||
       (g.out_kind != MXB200_OUT_BF16 && (g.out_kind != MXB200_OUT_F32 || g.kind != MXB200_BLOCK_WEIGHT_GRAD)))
     return MXB200_ERR_ARGUMENT;
-  constexpr int64_t kMost = int64_t{1} << 30;
-  if (g.tokens < 0 || g.tokens > kMost || g.in_features <= 0 || g.in_features > kMost || g.out_features <= 0 ||
-      g.out_features > kMost || g.in_features % 16 || g.out_features % 16 || g.experts < 1 || g.experts > kMaxExperts)
+  if (g.tokens < 0 || g.tokens > kMostSize || g.in_features <= 0 || g.in_features > kMostSize || g.out_features <= 0 ||
+      g.out_features > kMostSize || g.in_features % 16 || g.out_features % 16 || g.experts < 1 || g.experts > kMaxExperts)
     return MXB200_ERR_SHAPE;
   if (g.b_ld != 0 && g.kind != MXB200_BLOCK_FORWARD)
     return MXB200_ERR_ARGUMENT;
@@ -1403,7 +1442,7 @@ int block_gemm(const mxb200_block_gemm_args& g, cudaStream_t stream) {
   const int64_t in = g.in_features, out = g.out_features;
   const bool forward = g.kind == MXB200_BLOCK_FORWARD || g.kind == MXB200_BLOCK_FORWARD_SCALED;
   const int from = static_cast<int>(forward ? in : out), to = static_cast<int>(forward ? out : in);
-  const int blocks = static_cast<int>(up(from, kBlock));
+  const int blocks = static_cast<int>(blocks_up(from, kBlock));
   Launch l{};
   Params& p = l.p;
   p.d = g.d, p.ends = g.ends, p.experts = g.experts, p.rows = static_cast<int>(g.tokens);
@@ -1411,7 +1450,7 @@ int block_gemm(const mxb200_block_gemm_args& g, cudaStream_t stream) {
   p.splits = 1;
   // token tiles are known on the device only; this many at most
   const auto most_tiles = [&](int64_t tile) {
-    return g.ends == nullptr ? up(g.tokens, tile) : (g.tokens + (tile - 1) * std::min<int64_t>(g.experts + 1, g.tokens)) / tile;
+    return g.ends == nullptr ? blocks_up(g.tokens, tile) : (g.tokens + (tile - 1) * std::min<int64_t>(g.experts + 1, g.tokens)) / tile;
   };
   VariantId id = g.tokens <= mxb200::scaled::kSegment * kBlock ? kWeightGradPair : kWeightGradLong;
   Configured configured;
@@ -1422,22 +1461,22 @@ int block_gemm(const mxb200_block_gemm_args& g, cudaStream_t stream) {
       return st;
     const int64_t capacity = mxb200_block_token_blocks(g.tokens, g.experts) * kBlock;
     p.features = static_cast<int>(out), p.n = static_cast<int>(in);
-    units = g.experts * up(out, mxb200::scaled::kTile) * up(in, mxb200::scaled::kTile);
+    units = g.experts * blocks_up(out, mxb200::scaled::kTile) * blocks_up(in, mxb200::scaled::kTile);
     st = make_map(&l.maps.a, g.a, out, capacity, 1, 128);
     st = st != MXB200_OK ? st : make_map(&l.maps.b, g.b, in, capacity, 1, 128);
-    st = st != MXB200_OK ? st : make_scale_map(&l.maps.a_scale, g.a_scale, up(out, kBlock), capacity / kBlock, 1, 1);
-    st = st != MXB200_OK ? st : make_scale_map(&l.maps.b_scale, g.b_scale, up(in, kBlock), capacity / kBlock, 2, 1);
+    st = st != MXB200_OK ? st : make_scale_map(&l.maps.a_scale, g.a_scale, blocks_up(out, kBlock), capacity / kBlock, 1, 1);
+    st = st != MXB200_OK ? st : make_scale_map(&l.maps.b_scale, g.b_scale, blocks_up(in, kBlock), capacity / kBlock, 2, 1);
   } else if (scaled) {
     id = forward ? kForwardScaled : kInputGradScaled;
     if (st = configure(id, dev, &configured); st != MXB200_OK)
       return st;
     const int64_t capacity = mxb200_block_token_blocks(g.tokens, g.experts) * kBlock;
-    p.features = to, p.blocks = blocks, p.w_scale_rows = static_cast<int>(up(out, kBlock));
-    units = most_tiles(mxb200::scaled::kTile) * up(to, mxb200::scaled::kTile);
+    p.features = to, p.blocks = blocks, p.w_scale_rows = static_cast<int>(blocks_up(out, kBlock));
+    units = most_tiles(mxb200::scaled::kTile) * blocks_up(to, mxb200::scaled::kTile);
     st = make_map(&l.maps.a, g.b, from, capacity, 1, 128);
     st = st != MXB200_OK ? st : make_map(&l.maps.b, g.a, in, out, g.experts, 128);
     st = st != MXB200_OK ? st : make_scale_map(&l.maps.a_scale, g.b_scale, blocks, capacity / kBlock, 1, 1);
-    st = st != MXB200_OK ? st : make_scale_map(&l.maps.b_scale, g.a_scale, up(in, kBlock), up(out, kBlock) * g.experts, forward ? 1 : 2, forward ? 2 : 1);
+    st = st != MXB200_OK ? st : make_scale_map(&l.maps.b_scale, g.a_scale, blocks_up(in, kBlock), blocks_up(out, kBlock) * g.experts, forward ? 1 : 2, forward ? 2 : 1);
   } else {
     const bool many = !quantize && many_tokens(g.tokens, g.experts, to, blocks, dev.sms);
     // at most half a small tile per expert expected, so that few experts need a second one
@@ -1447,21 +1486,22 @@ int block_gemm(const mxb200_block_gemm_args& g, cudaStream_t stream) {
     p.weight_scale = static_cast<const float*>(g.a_scale), p.token_scale = static_cast<const float*>(g.b_scale);
     p.token_ld = quantize ? g.b_ld : g.tokens, p.features = to, p.blocks = blocks;
     p.input = g.b, p.input_cols = from;
-    p.w_scale_expert = up(out, kBlock) * up(in, kBlock);
-    p.w_scale_f = forward ? static_cast<int>(up(in, kBlock)) : 1, p.w_scale_b = forward ? 1 : static_cast<int>(up(in, kBlock));
-    units = most_tiles(v.tokens) * up(to, v.features);
+    p.w_scale_expert = blocks_up(out, kBlock) * blocks_up(in, kBlock);
+    p.w_scale_f = forward ? static_cast<int>(blocks_up(in, kBlock)) : 1, p.w_scale_b = forward ? 1 : static_cast<int>(blocks_up(in, kBlock));
+    units = most_tiles(v.tokens) * blocks_up(to, v.features);
     if (st = configure(id, dev, &configured); st != MXB200_OK)
       return st;
     if (!many)
-      p.splits = share_blocks(expected_tiles(g.tokens, g.experts, v.tokens) * up(to, v.features), blocks,
-                              static_cast<int>(std::min<int64_t>(v.tokens, up(g.tokens, g.experts))), configured);
+      p.splits = share_blocks(expected_tiles(g.tokens, g.experts, v.tokens) * blocks_up(to, v.features), blocks,
+                              static_cast<int>(std::min<int64_t>(v.tokens, blocks_up(g.tokens, g.experts))), configured);
     CUtensorMap *weight = many ? &l.maps.b : &l.maps.a, *token = many ? &l.maps.a : &l.maps.b;
     st = make_map(weight, g.a, in, out, g.experts, 128);
     st = st != MXB200_OK || quantize ? st : make_map(token, g.b, from, g.tokens, 1, many ? 128 : 32);
+    st = st != MXB200_OK || !many ? st : make_output_map(&l.maps.d, g.d, to, g.tokens);
   }
   if (st != MXB200_OK)
     return st;
-  if (units > kMost)
+  if (units > kMostSize)
     return MXB200_ERR_SHAPE;
   const Variant& v = variant(id);
   const unsigned grid = static_cast<unsigned>(std::min<int64_t>(units, configured.clusters[p.splits])) * std::max(v.ctas, p.splits);
@@ -1494,8 +1534,8 @@ extern "C" int mxb200_block_scaled(int64_t tokens, int64_t in_features, int64_t 
   DeviceInfo dev;
   if (tokens <= 0 || in_features <= 0 || out_features <= 0 || experts <= 0 || current_device(&dev) != MXB200_OK)
     return 0;
-  return many_tokens(tokens, experts, static_cast<int>(out_features), static_cast<int>(up(in_features, kBlock)), dev.sms) &&
-         many_tokens(tokens, experts, static_cast<int>(in_features), static_cast<int>(up(out_features, kBlock)), dev.sms);
+  return many_tokens(tokens, experts, static_cast<int>(out_features), static_cast<int>(blocks_up(in_features, kBlock)), dev.sms) &&
+         many_tokens(tokens, experts, static_cast<int>(in_features), static_cast<int>(blocks_up(out_features, kBlock)), dev.sms);
 }
 
 extern "C" int mxb200_block_gemm(const mxb200_block_gemm_args* args, void* stream) {

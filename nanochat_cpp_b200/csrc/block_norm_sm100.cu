@@ -345,8 +345,6 @@ __global__ void __launch_bounds__(1024) mxb200_block_norm_sum_gain(const float* 
 namespace mxb200 {
 namespace {
 
-constexpr int64_t kMost = int64_t{1} << 30;
-
 struct Forward {
   void (*kernel)(ForwardParams);
   int rows_per_block;
@@ -390,7 +388,7 @@ Backward backward_of(int cols) {
 }
 
 int check_shape(int64_t rows, int32_t cols) {
-  return rows < 0 || rows > kMost || cols <= 0 || cols > kMaxCols || cols % 16 ? MXB200_ERR_SHAPE : MXB200_OK;
+  return rows < 0 || rows > kMostSize || cols <= 0 || cols > kMaxCols || cols % 16 ? MXB200_ERR_SHAPE : MXB200_OK;
 }
 
 // needed pointers first, then optional ones

@@ -300,12 +300,6 @@ __global__ void __launch_bounds__(mxb200::kThreads) mxb200_block_quantize_weight
 namespace mxb200 {
 namespace {
 
-constexpr int64_t kMost = int64_t{1} << 30;
-
-int64_t up(int64_t n, int64_t d) {
-  return (n + d - 1) / d;
-}
-
 // Null or misaligned pointers among those that are needed.
 int check_pointers(std::initializer_list<const void*> pointers) {
   for (const void* q : pointers) {
@@ -323,7 +317,7 @@ int check_pointers(std::initializer_list<const void*> pointers) {
 extern "C" int mxb200_block_quantize(const void* x, int64_t rows, int64_t cols, int64_t ld, const int32_t* ends, int experts,
                                      void* row_data, void* row_scale, int rows_in_blocks, void* token_data, uint32_t* token_scale, void* stream) {
   using namespace mxb200;
-  if (rows < 0 || rows > kMost || cols <= 0 || cols > kMost || cols % 16 || ld < cols || ld % 8 || experts < 1 || experts > kMaxExperts)
+  if (rows < 0 || rows > kMostSize || cols <= 0 || cols > kMostSize || cols % 16 || ld < cols || ld % 8 || experts < 1 || experts > kMaxExperts)
     return MXB200_ERR_SHAPE;
   if (ends == nullptr && experts != 1)
     return MXB200_ERR_NULL;
@@ -352,8 +346,8 @@ extern "C" int mxb200_block_quantize(const void* x, int64_t rows, int64_t cols, 
     p.row_scale = static_cast<float*>(row_scale);
   p.col_data = static_cast<uint8_t*>(token_data), p.col_scale_words = token_scale;
   // enough blocks to fill the machine; beyond that a block goes on to its rows' next columns, with its experts looked up once
-  const int64_t blocks = want_tokens ? mxb200_block_token_blocks(rows, experts) : up(rows, kBlock);
-  const int64_t parts = std::min<int64_t>(up(cols, kBlock), std::max<int64_t>(1, up(8 * dev.sms, blocks)));
+  const int64_t blocks = want_tokens ? mxb200_block_token_blocks(rows, experts) : blocks_up(rows, kBlock);
+  const int64_t parts = std::min<int64_t>(blocks_up(cols, kBlock), std::max<int64_t>(1, blocks_up(8 * dev.sms, blocks)));
   const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(std::min<int64_t>(parts, 65535)));
   const auto kernel = !want_tokens     ? mxb200_block_quantize_rows
                       : rows_in_blocks ? mxb200_block_quantize_both_in_blocks
@@ -365,10 +359,10 @@ extern "C" int mxb200_block_quantize(const void* x, int64_t rows, int64_t cols, 
 extern "C" int mxb200_block_quantize_weight(const void* w, int w_bf16, int experts, int64_t rows, int64_t cols, void* data,
                                             void* scale, int in_tiles, void* stream) {
   using namespace mxb200;
-  if (rows <= 0 || rows > kMost || cols <= 0 || cols > kMost || rows % 16 || cols % 16 || experts < 1 || experts > kMaxExperts)
+  if (rows <= 0 || rows > kMostSize || cols <= 0 || cols > kMostSize || rows % 16 || cols % 16 || experts < 1 || experts > kMaxExperts)
     return MXB200_ERR_SHAPE;
-  const int64_t tiles = experts * up(rows, kBlock) * up(cols, kBlock);
-  if (tiles > kMost)
+  const int64_t tiles = experts * blocks_up(rows, kBlock) * blocks_up(cols, kBlock);
+  if (tiles > kMostSize)
     return MXB200_ERR_SHAPE;
   DeviceInfo dev;
   if (int st = current_device(&dev); st != MXB200_OK)

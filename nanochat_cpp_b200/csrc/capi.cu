@@ -72,7 +72,7 @@ extern "C" const char* mxb200_strerror(int status) {
     case MXB200_OK:
       return "ok";
     case MXB200_ERR_SHAPE:
-      return "mxb200: dimensions must be positive multiples of 128 (and fit the views given)";
+      return "mxb200: a dimension is out of range or not a multiple of 128 (of 16 in blocks of 128), or does not fit the view given";
     case MXB200_ERR_ALIGNMENT:
       return "mxb200: pointers and leading dimensions must be 16-byte aligned (workspace: 256)";
     case MXB200_ERR_NULL:
