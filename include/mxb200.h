@@ -316,9 +316,10 @@ typedef struct mxb200_block_gemm_args {
   int32_t experts;
   int32_t kind;     /* mxb200_block_kind */
   int32_t out_kind; /* mxb200_out_kind; F32 for the weight gradient only */
-  int64_t b_ld;     /* 0: b is quantized. Else (FORWARD of up to MXB200_BLOCK_FEW_TOKENS tokens) b is bf16, b_ld values between
-                       rows (b_ld % 8 == 0), and quantized on its way, with the bits that mxb200_block_quantize and this
-                       product of its output give; b_scale is not read. A launch costs more than every CTA's repeating that. */
+  int64_t b_ld;     /* 0: b is quantized. Else (FORWARD only) b is bf16, b_ld values between rows (b_ld % 8 == 0), and quantized on
+                       its way, to the values that mxb200_block_quantize gives; b_scale is not read. For few tokens, or few per
+                       expert: every CTA repeats it. Up to MXB200_BLOCK_FEW_TOKENS tokens the result has the bits of the
+                       product of the quantized b. */
 } mxb200_block_gemm_args;
 MXB200_API int mxb200_block_gemm(const mxb200_block_gemm_args* args, void* stream);
 

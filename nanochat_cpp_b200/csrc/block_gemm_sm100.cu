@@ -316,8 +316,8 @@ __device__ __forceinline__ void store_lines(LineStage* stage, int lane, unsigned
 // memory, and adds up every n-th token of all of them, always in the cluster's order.
 //
 // kQuantize: the input comes in bf16 and is quantized on its way into shared memory, by the four warps that would accumulate
-// the second half of the columns: up to 16 tokens. That spares a launch, about 2 us on the device and as much on the host; every
-// CTA's repeating it costs 0.5 us for one token and 2 for 16 (1536 -> 1536).
+// the second half of the columns. That spares a launch, about 2 us on the device and as much on the host; every CTA's repeating
+// it costs 0.5 us for one token and 2 for 16 (1536 -> 1536), 1.2 for 32 rows over 64 experts and 3.7 for 64.
 
 namespace few {
 
@@ -420,8 +420,8 @@ __device__ __forceinline__ void load_scales(const Params& p, typename C::Shared*
 template <typename C>
 __device__ __forceinline__ void quantize(const Params& p, typename C::Shared* s, unsigned char* b_stages, const Place& at, int units, int warp,
                                          int lane) {
-  static_assert(MXB200_BLOCK_FEW_TOKENS <= C::kTileT && C::Shared::kStages % 4 == 0 && kScaleSlots % 4 == 0, "whole turns of the rings");
-  constexpr int kPasses = MXB200_BLOCK_FEW_TOKENS / 2;
+  static_assert(C::Shared::kStages % 4 == 0 && kScaleSlots % 4 == 0, "whole turns of the rings");
+  constexpr int kPasses = C::kTileT / 2;
   const uint32_t full0 = smem_u32(&s->full[0]), empty0 = smem_u32(&s->empty[0]);
   const uint32_t scale_full0 = smem_u32(&s->scale_full[0]), scale_empty0 = smem_u32(&s->scale_empty[0]);
   const int lane16 = lane & 15, token0 = lane >> 4;
@@ -1415,7 +1415,7 @@ int block_gemm(const mxb200_block_gemm_args& g, cudaStream_t stream) {
     return MXB200_ERR_SHAPE;
   if (g.b_ld != 0 && g.kind != MXB200_BLOCK_FORWARD)
     return MXB200_ERR_ARGUMENT;
-  if (g.b_ld != 0 && (g.b_ld < g.in_features || g.b_ld % 8 || g.tokens > MXB200_BLOCK_FEW_TOKENS))
+  if (g.b_ld != 0 && (g.b_ld < g.in_features || g.b_ld % 8))
     return MXB200_ERR_SHAPE;
   if (g.ends == nullptr && g.experts != 1)
     return MXB200_ERR_NULL;
@@ -1479,8 +1479,9 @@ int block_gemm(const mxb200_block_gemm_args& g, cudaStream_t stream) {
     st = st != MXB200_OK ? st : make_scale_map(&l.maps.b_scale, g.a_scale, blocks_up(in, kBlock), blocks_up(out, kBlock) * g.experts, forward ? 1 : 2, forward ? 2 : 1);
   } else {
     const bool many = !quantize && many_tokens(g.tokens, g.experts, to, blocks, dev.sms);
-    // at most half a small tile per expert expected, so that few experts need a second one
-    const bool small = g.tokens <= few::Tile32::kTileT || g.tokens <= int64_t{few::Tile32::kTileT} / 2 * g.experts;
+    // the small tile as long as few experts need a second one: 600 rows over 64 experts (1536 -> 2048) take 36.7 us in small tiles
+    // and 38.8 in large ones, 1000 rows 41.2 and 40.0
+    const bool small = g.tokens <= few::Tile32::kTileT || g.tokens <= int64_t{12} * g.experts;
     id = quantize ? kForwardQuantizing : many ? (forward ? kForwardMany : kInputGradMany) : !forward ? kInputGradFew : small ? kForward32 : kForwardFew;
     const Variant& v = variant(id);
     p.weight_scale = static_cast<const float*>(g.a_scale), p.token_scale = static_cast<const float*>(g.b_scale);

@@ -120,6 +120,26 @@ def test_quantized_by_the_product(nc, tokens, cin, cout):
         assert torch.equal(torch.nan_to_num(got, nan=1e9), torch.nan_to_num(want, nan=1e9))
 
 
+@pytest.mark.parametrize("counts", [[0, 1, 2, 0] * 20, [40, 0, 70, 3], [33] * 3], ids=str)
+def test_experts_quantized_by_the_product(nc, counts):
+    """More rows than the small tile has, in the C entry that quantizes them; and what the experts' call takes by itself."""
+    import ctypes
+    g, capi, cin, cout = generator(19), nc.capi, 272, 400
+    rows, ends = sum(counts) + 5, ends_of(counts)
+    x, w = activation(g, rows, cin), given_weight(nc, g, len(counts), cout, cin)
+    got = torch.full((rows, cout), 7.0, device="cuda", dtype=torch.bfloat16)
+    args = capi.BlockGemmArgs(w.data.data_ptr(), w.scale.data_ptr(), x.data_ptr(), None, got.data_ptr(), ends.data_ptr(), rows, cin, cout,
+                              len(counts), capi.BLOCK_FORWARD, capi.OUT_BF16, cin)
+    capi.check(capi.lib.mxb200_block_gemm(ctypes.byref(args), torch.cuda.current_stream().cuda_stream), "block_gemm")
+    called = nc.fp8_block_experts(x, w, ends)
+    xr = ref.row_values(x)
+    for y in (got, called):
+        for e, (a, b) in enumerate(ref.spans(ends.tolist(), rows)):
+            if b > a:
+                assert_product(y[a:b], xr[a:b], ref.weight_values(w.data[e], w.scale[e]), f"y of expert {e}")
+        assert not y[sum(counts):].any()
+
+
 @pytest.mark.parametrize("tokens", [1, 16, 129, 384, 1000])
 @pytest.mark.parametrize("cin,cout", [(16, 16), (272, 144), (128, 640), (1040, 2000)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
