@@ -301,7 +301,9 @@ typedef enum mxb200_block_kind {
 /* Whether the scaled kinds are the faster ones for a Linear's forward and input gradient of this size on the current device. */
 MXB200_API int mxb200_block_scaled(int64_t tokens, int64_t in_features, int64_t out_features, int experts);
 
-#define MXB200_BLOCK_FEW_TOKENS 16
+/* Whether the forward product of bf16 input (b_ld below) is expected to take less than mxb200_block_quantize and the product of
+ * its output, on the current device. Its result has the latter's bits then. */
+MXB200_API int mxb200_block_quantizes(int64_t tokens, int64_t in_features, int64_t out_features, int experts);
 
 /* One product per expert over its rows, fp32 accumulation, rounded once. Rows of no expert: zeros; the weight gradient of an
  * expert without rows: zeros. Needs no workspace. tokens may be 0. */
@@ -317,9 +319,8 @@ typedef struct mxb200_block_gemm_args {
   int32_t kind;     /* mxb200_block_kind */
   int32_t out_kind; /* mxb200_out_kind; F32 for the weight gradient only */
   int64_t b_ld;     /* 0: b is quantized. Else (FORWARD only) b is bf16, b_ld values between rows (b_ld % 8 == 0), and quantized on
-                       its way, to the values that mxb200_block_quantize gives; b_scale is not read. For few tokens, or few per
-                       expert: every CTA repeats it. Up to MXB200_BLOCK_FEW_TOKENS tokens the result has the bits of the
-                       product of the quantized b. */
+                       its way, to the values that mxb200_block_quantize gives; b_scale is not read. Every CTA repeats it:
+                       for where mxb200_block_quantizes says so. */
 } mxb200_block_gemm_args;
 MXB200_API int mxb200_block_gemm(const mxb200_block_gemm_args* args, void* stream);
 

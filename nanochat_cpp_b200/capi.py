@@ -29,6 +29,7 @@ SYMBOLS = (
     "mxb200_gemm_group_workspace_bytes", "mxb200_gemm_group",
     "mxb200_gemm_splits", "mxb200_gemm_workspace_bytes", "mxb200_gemm_splitk", "mxb200_gemm_splitk_static",
     "mxb200_block_token_blocks", "mxb200_block_quantize", "mxb200_block_quantize_weight", "mxb200_block_gemm", "mxb200_block_scaled",
+    "mxb200_block_quantizes",
     "mxb200_block_norm_fwd", "mxb200_block_norm_workspace_bytes", "mxb200_block_norm_bwd",
     "mxb200_strerror",
     "mxb200_device_status", "mxb200_selftest_bounded_wait", "mxb200_set_gemm_config", "mxb200_launch_count", "mxb200_version",
@@ -129,7 +130,7 @@ def _load() -> ctypes.CDLL:
     lib.mxb200_block_token_blocks.restype = i64
     lib.mxb200_block_quantize.argtypes = [vp, i64, i64, i64, vp, i32, vp, vp, i32, vp, vp, vp]
     lib.mxb200_block_quantize_weight.argtypes = [vp, i32, i32, i64, i64, vp, vp, i32, vp]
-    lib.mxb200_block_scaled.argtypes = [i64, i64, i64, i32]
+    lib.mxb200_block_scaled.argtypes = lib.mxb200_block_quantizes.argtypes = [i64, i64, i64, i32]
     lib.mxb200_block_gemm.argtypes = [ctypes.POINTER(BlockGemmArgs), vp]
     lib.mxb200_block_norm_fwd.argtypes = [ctypes.POINTER(BlockNormArgs), vp]
     lib.mxb200_block_norm_workspace_bytes.argtypes = [i64, ctypes.c_int32]

@@ -317,7 +317,12 @@ __device__ __forceinline__ void store_lines(LineStage* stage, int lane, unsigned
 //
 // kQuantize: the input comes in bf16 and is quantized on its way into shared memory, by the four warps that would accumulate
 // the second half of the columns. That spares a launch, about 2 us on the device and as much on the host; every CTA's repeating
-// it costs 0.5 us for one token and 2 for 16 (1536 -> 1536), 1.2 for 32 rows over 64 experts and 3.7 for 64.
+// it costs 0.6 us for one token and 1.9 for 16 (1536 -> 1536), 2.2 for 32 rows over 64 experts and 5.9 for 64.
+//
+// Blocks go through the barriers in pairs, and of a pair 32 tokens come from tensor memory with one wait: what a warp spends on a
+// block besides its bytes (two barriers, the way to tensor memory and back) is as long as the block's way into shared memory. 64
+// rows over 64 experts (1536 -> 2048) take 20.4 us by pairs, 23.1 one by one and 20.8 by fours; one token of 6144 -> 24576 29.7,
+// 36.3 and 30.9; 128 tokens of 1536 -> 6144 in large tiles 7.9 and 8.9.
 
 namespace few {
 
@@ -325,8 +330,7 @@ constexpr int kTileF = 128;
 constexpr uint32_t kStageRowBytes = 80;  // 32 bf16 and 16 bytes that put 8 rows' 16-byte pieces into different banks
 constexpr int kPartialRow = 132;         // floats of a token's 128 features: fragments' rows fall into different banks
 
-// kTile: tokens of a unit, 128, or 32 where no more are expected: more stages of the weight, which is what such a product reads,
-// fit beside so few tokens.
+// kTile: tokens of a unit, 128 or 32; fewer are done with their columns sooner and leave room for more stages of the weight.
 template <int kTile, bool kQuantize_>
 struct Config {
   static constexpr bool kQuantize = kQuantize_;
@@ -335,25 +339,26 @@ struct Config {
   static constexpr int kParts = kWarps / 4;           // columns are shared by the warps of a tensor memory quarter
   static constexpr int kPartT = kTile / kParts;
   static constexpr int kChunks = kPartT / 32;
-  static constexpr int kAccBuffers = 4;
+  static constexpr int kTurn = 2;                     // blocks that the barriers pass on at a time
+  static constexpr int kAccBuffers = kTmemCols / (kTurn * kTile) < 4 ? kTmemCols / (kTurn * kTile) : 4;
 
   struct __align__(16) ScaleSlot {  // tokens' scales are read in pairs
     float token[kTileT];
     float weight;
   };
 
-  struct Shared : Common<kTile == 32 ? 8 : 5> {
+  struct Shared : Common<(kTile == 32 ? 8 : 4) / kTurn> {
     uint64_t partial_full, partial_empty;
-    ScaleSlot scales[kScaleSlots];
+    ScaleSlot scales[kScaleSlots][kTurn];
     union {
       __align__(16) unsigned char out[kWarps][32 * kStageRowBytes];
       __align__(16) float partial[kPartT][kPartialRow];
     };
   };
-  static constexpr uint32_t kStageBBytes = kTileT * kBlock;
-  static constexpr size_t kSmemBytes = 1024 + Shared::kStages * static_cast<size_t>(kABytes + kStageBBytes) + sizeof(Shared);
+  static constexpr uint32_t kBlockBBytes = kTileT * kBlock, kStageABytes = kTurn * kABytes, kStageBBytes = kTurn * kBlockBBytes;
+  static constexpr size_t kSmemBytes = 1024 + Shared::kStages * static_cast<size_t>(kStageABytes + kStageBBytes) + sizeof(Shared);
   static_assert(kSmemBytes <= 232448, "shared memory of one CTA");
-  static_assert(Shared::kStages * kABytes >= kMaxExperts * 4, "the operand stages hold the scan's copy of ends");
+  static_assert(Shared::kStages * kStageABytes >= kMaxExperts * 4, "the operand stages hold the scan's copy of ends");
 };
 
 // Which CTA of which cluster this is, and its share of a unit's blocks.
@@ -373,14 +378,19 @@ __device__ __forceinline__ void load_operands(const Params& p, const CUtensorMap
   for (int u = at.cluster; u < units; u += at.clusters) {
     const Unit x = unit_at<C::kTileT, kTileF>(p, s, u);
     const int boxes = C::kQuantize ? 0 : (x.rows + 31) / 32;
-    for (int b = at.begin(x.blocks); b < at.end(x.blocks); ++b) {
+    const int end = at.end(x.blocks);
+    for (int b = at.begin(x.blocks); b < end; b += C::kTurn) {
+      const int turn = min(C::kTurn, end - b);
       if (!wait_bounded(empty0 + stage * 8, phase ^ 1u, &s->abort_flag, kSiteStageEmpty))
         return;
       const uint32_t full = full0 + stage * 8;
-      mbar_arrive_expect_tx(el, full, kABytes + boxes * kBBoxBytes);
-      tma_load_3d(el, a0 + stage * kABytes, map_w, full, kMode == kForward ? b * kBlock : x.f0, kMode == kForward ? x.f0 : b * kBlock, x.expert);
-      for (int i = 0; i < boxes; ++i)
-        tma_load_3d(el, b0 + stage * C::kStageBBytes + i * kBBoxBytes, map_t, full, b * kBlock, x.row0 + 32 * i, 0);
+      mbar_arrive_expect_tx(el, full, turn * (kABytes + boxes * kBBoxBytes));
+      for (int n = 0; n < turn; ++n) {
+        const int k = (b + n) * kBlock;
+        tma_load_3d(el, a0 + stage * C::kStageABytes + n * kABytes, map_w, full, kMode == kForward ? k : x.f0, kMode == kForward ? x.f0 : k, x.expert);
+        for (int i = 0; i < boxes; ++i)
+          tma_load_3d(el, b0 + stage * C::kStageBBytes + n * C::kBlockBBytes + i * kBBoxBytes, map_t, full, k, x.row0 + 32 * i, 0);
+      }
       if (++stage == C::Shared::kStages)
         stage = 0, phase ^= 1u;
     }
@@ -398,14 +408,18 @@ __device__ __forceinline__ void load_scales(const Params& p, typename C::Shared*
   uint32_t slot = 0, slot_phase = 0;
   for (int u = at.cluster; u < units; u += at.clusters) {
     const Unit x = unit_at<C::kTileT, kTileF>(p, s, u);
-    for (int b = at.begin(x.blocks); b < at.end(x.blocks); ++b) {
+    const int end = at.end(x.blocks);
+    for (int b = at.begin(x.blocks); b < end; b += C::kTurn) {
       if (!wait_bounded(scale_empty0 + slot * 8, slot_phase ^ 1u, &s->abort_flag, kSiteScaleEmpty))
         return;
-      const float* token = p.token_scale + b * p.token_ld + x.row0;
-      for (int i = lane; i < x.rows; i += 32)
-        cp_async_4(smem_u32(&s->scales[slot].token[i]), token + i);
-      if (lane == 0)
-        cp_async_4(smem_u32(&s->scales[slot].weight), weight_scale(p, x, b));
+      for (int n = 0; n < min(C::kTurn, end - b); ++n) {
+        auto& to = s->scales[slot][n];
+        const float* token = p.token_scale + (b + n) * p.token_ld + x.row0;
+        for (int i = lane; i < x.rows; i += 32)
+          cp_async_4(smem_u32(&to.token[i]), token + i);
+        if (lane == 0)
+          cp_async_4(smem_u32(&to.weight), weight_scale(p, x, b + n));
+      }
       cp_async_arrive(scale_full0 + slot * 8);
       if (++slot == kScaleSlots)
         slot = 0, slot_phase ^= 1u;
@@ -420,7 +434,7 @@ __device__ __forceinline__ void load_scales(const Params& p, typename C::Shared*
 template <typename C>
 __device__ __forceinline__ void quantize(const Params& p, typename C::Shared* s, unsigned char* b_stages, const Place& at, int units, int warp,
                                          int lane) {
-  static_assert(C::Shared::kStages % 4 == 0 && kScaleSlots % 4 == 0, "whole turns of the rings");
+  static_assert(C::kTurn == 2, "pairs of blocks");
   constexpr int kPasses = C::kTileT / 2;
   const uint32_t full0 = smem_u32(&s->full[0]), empty0 = smem_u32(&s->empty[0]);
   const uint32_t scale_full0 = smem_u32(&s->scale_full[0]), scale_empty0 = smem_u32(&s->scale_empty[0]);
@@ -438,7 +452,7 @@ __device__ __forceinline__ void quantize(const Params& p, typename C::Shared* s,
     }
     weight_ahead = *weight_scale(p, x, b);
   };
-  uint32_t before = 0;  // blocks of the units before this one
+  uint32_t before = 0;  // blocks of the units before this one, in whole pairs
   for (int u = at.cluster; u < units; u += at.clusters) {
     const Unit x = unit_at<C::kTileT, kTileF>(p, s, u);
     const int begin = at.begin(x.blocks), end = at.end(x.blocks);
@@ -447,11 +461,11 @@ __device__ __forceinline__ void quantize(const Params& p, typename C::Shared* s,
     if (b < end)
       fetch(x, b);
     for (; b < end; b += 4, n += 4) {
-      const uint32_t stage = n % C::Shared::kStages, slot = n % kScaleSlots;
-      if (!wait_bounded(empty0 + stage * 8, (n / C::Shared::kStages & 1u) ^ 1u, &s->abort_flag, kSiteStageEmpty) ||
-          !wait_bounded(scale_empty0 + slot * 8, (n / kScaleSlots & 1u) ^ 1u, &s->abort_flag, kSiteScaleEmpty))
+      const uint32_t pair = n >> 1, of_pair = n & 1, stage = pair % C::Shared::kStages, slot = pair % kScaleSlots;
+      if (!wait_bounded(empty0 + stage * 8, (pair / C::Shared::kStages & 1u) ^ 1u, &s->abort_flag, kSiteStageEmpty) ||
+          !wait_bounded(scale_empty0 + slot * 8, (pair / kScaleSlots & 1u) ^ 1u, &s->abort_flag, kSiteScaleEmpty))
         return;
-      unsigned char* to = b_stages + stage * C::kStageBBytes;
+      unsigned char* to = b_stages + stage * C::kStageBBytes + of_pair * C::kBlockBBytes;
 #pragma unroll
       for (int i = 0; i < kPasses; ++i) {
         if (2 * i >= x.rows)
@@ -469,20 +483,21 @@ __device__ __forceinline__ void quantize(const Params& p, typename C::Shared* s,
         *reinterpret_cast<uint2*>(to + t * kBlock + (((lane16 >> 1) ^ (t & 7)) << 4) + (lane16 & 1) * 8) =
               make_uint2(e4m3x4_scaled_fma(w[0], w[1], by, by), e4m3x4_scaled_fma(w[2], w[3], by, by));
         if (lane16 == 0)
-          s->scales[slot].token[t] = __uint_as_float(static_cast<uint32_t>(e) << 23);
+          s->scales[slot][of_pair].token[t] = __uint_as_float(static_cast<uint32_t>(e) << 23);
       }
       if (lane == 0)
-        s->scales[slot].weight = weight_ahead;
+        s->scales[slot][of_pair].weight = weight_ahead;
       if (b + 4 < end)
         fetch(x, b + 4);
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) {
+      // a last block without a second one arrives for both
+      if (lane < (of_pair == 0 && b + 1 == end ? 2 : 1)) {
         mbar_arrive_addr(full0 + stage * 8);
         mbar_arrive_addr(scale_full0 + slot * 8);
       }
     }
-    before += static_cast<uint32_t>(end - begin);
+    before += static_cast<uint32_t>((end - begin + 1) & ~1);
   }
 }
 
@@ -499,15 +514,22 @@ __device__ __forceinline__ void issue_mmas(const Params& p, typename C::Shared* 
   for (int u = at.cluster; u < units; u += at.clusters) {
     const Unit x = unit_at<C::kTileT, kTileF>(p, s, u);
     const uint32_t idesc = make_idesc_f8(kTileF, (x.rows + 15) / 16 * 16, kAMn, false);
-    for (int b = at.begin(x.blocks); b < at.end(x.blocks); ++b) {
+    const int end = at.end(x.blocks);
+    for (int b = at.begin(x.blocks); b < end; b += C::kTurn) {
       if (!wait_bounded(smem_u32(&s->acc_empty[buf]), buf_phase ^ 1u, &s->abort_flag, kSiteAccEmpty) ||
           !wait_bounded(full0 + stage * 8, phase, &s->abort_flag, kSiteStageFull))
         return;
       tcgen05_fence_after_sync();
-      const uint64_t a = a_desc0 + stage * (kABytes >> 4), bd = b_desc0 + stage * (C::kStageBBytes >> 4);
+      const uint64_t a = a_desc0 + stage * (C::kStageABytes >> 4), bd = b_desc0 + stage * (C::kStageBBytes >> 4);
+      const uint32_t d = tmem_base + buf * (C::kTurn * C::kTileT);
 #pragma unroll
-      for (uint32_t k = 0; k < 4; ++k)
-        tcgen05_mma_f8(el, tmem_base + buf * C::kTileT, a + k * kAStep, bd + k * kBStep, idesc, k > 0);
+      for (int n = 0; n < C::kTurn; ++n) {
+        if (b + n >= end)
+          break;
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k)
+          tcgen05_mma_f8(el, d + n * C::kTileT, a + n * (kABytes >> 4) + k * kAStep, bd + n * (C::kBlockBBytes >> 4) + k * kBStep, idesc, k > 0);
+      }
       tcgen05_commit(el, &s->empty[stage]);
       tcgen05_commit(el, &s->acc_full[buf]);
       if (++stage == C::Shared::kStages)
@@ -561,39 +583,52 @@ __device__ __forceinline__ void accumulate(const Params& p, typename C::Shared* 
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           acc[c][j][i] = 0;
-    for (int b = at.begin(x.blocks); b < at.end(x.blocks); ++b) {
+    const int end = at.end(x.blocks);
+    for (int b = at.begin(x.blocks); b < end; b += C::kTurn) {
       if (!wait_bounded(smem_u32(&s->scale_full[slot]), slot_phase, &s->abort_flag, kSiteScaleFull) ||
           !wait_bounded(smem_u32(&s->acc_full[buf]), buf_phase, &s->abort_flag, kSiteAccFull))
         return;
       tcgen05_fence_after_sync();
-      const auto& sc = s->scales[slot];
-      const uint64_t weight = pair_f32(sc.weight, sc.weight);
-      const uint32_t t = tmem_base + lane_base + buf * C::kTileT + part0;
 #pragma unroll
       for (int c = 0; c < C::kChunks; ++c) {
         if (part0 + 32 * c >= x.rows)
           break;
-        uint32_t lo[16], hi[16];
-        tmem_ld_16x256b_x4(t + 32 * c, lo);
-        tmem_ld_16x256b_x4(t + 32 * c + (16u << 16), hi);
-        uint64_t scale[4];
+        // a last block without a second one: that one's are read and not used
+        uint32_t lo[C::kTurn][16], hi[C::kTurn][16];
+        uint64_t scale[C::kTurn][4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 f = *reinterpret_cast<const float2*>(&sc.token[part0 + 32 * c + 8 * j + 2 * (lane & 3)]);
-          scale[j] = mul_f32x2(pair_f32(f.x, f.y), weight);
+        for (int n = 0; n < C::kTurn; ++n) {
+          const uint32_t t = tmem_base + lane_base + (buf * C::kTurn + n) * C::kTileT + part0 + 32 * c;
+          tmem_ld_16x256b_x4(t, lo[n]);
+          tmem_ld_16x256b_x4(t + (16u << 16), hi[n]);
+        }
+#pragma unroll
+        for (int n = 0; n < C::kTurn; ++n) {
+          const auto& sc = s->scales[slot][n];
+          const uint64_t weight = pair_f32(sc.weight, sc.weight);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float2 f = *reinterpret_cast<const float2*>(&sc.token[part0 + 32 * c + 8 * j + 2 * (lane & 3)]);
+            scale[n][j] = mul_f32x2(pair_f32(f.x, f.y), weight);
+          }
         }
         tmem_ld_wait();
 #pragma unroll
-        for (int k = 0; k < 16; ++k)
-          asm volatile("" : "+r"(lo[k]), "+r"(hi[k]));
+        for (int n = 0; n < C::kTurn; ++n) {
+          if (b + n >= end)
+            break;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+          for (int k = 0; k < 16; ++k)
+            asm volatile("" : "+r"(lo[n][k]), "+r"(hi[n][k]));
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint64_t v = i < 2 ? pair_u32(lo[4 * j + 2 * i], lo[4 * j + 2 * i + 1])
-                                     : pair_u32(hi[4 * j + 2 * i - 4], hi[4 * j + 2 * i - 3]);
-            acc[c][j][i] = fma_f32x2(v, scale[j], acc[c][j][i]);
-          }
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint64_t v = i < 2 ? pair_u32(lo[n][4 * j + 2 * i], lo[n][4 * j + 2 * i + 1])
+                                       : pair_u32(hi[n][4 * j + 2 * i - 4], hi[n][4 * j + 2 * i - 3]);
+              acc[c][j][i] = fma_f32x2(v, scale[n][j], acc[c][j][i]);
+            }
+        }
       }
       tcgen05_fence_before_sync();
       __syncwarp();
@@ -665,7 +700,7 @@ template <int kMode, typename C>
 __device__ __forceinline__ void body(const Params& p, const CUtensorMap* map_w, const CUtensorMap* map_t) {
   extern __shared__ unsigned char smem_raw[];
   unsigned char* base = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
-  unsigned char* b_stages = base + C::Shared::kStages * kABytes;
+  unsigned char* b_stages = base + C::Shared::kStages * C::kStageABytes;
   const uint32_t a0 = smem_u32(base), b0 = smem_u32(b_stages);
   auto* s = reinterpret_cast<typename C::Shared*>(b_stages + C::Shared::kStages * C::kStageBBytes);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -674,9 +709,9 @@ __device__ __forceinline__ void body(const Params& p, const CUtensorMap* map_w, 
     mbar_init(&s->partial_full, C::kWarps * p.splits);
     mbar_init(&s->partial_empty, C::kWarps * p.splits);
   }
-  SetUp set{1, 1, C::kWarps, C::kAccBuffers, C::kQuantize ? 1u : 32u, C::kTileT, true};
+  SetUp set{1, 1, C::kWarps, C::kAccBuffers, C::kQuantize ? 2u : 32u, C::kTileT, true};
   if (C::kQuantize)
-    set.full_arrivals = 2;  // the weight's load and the block's warp
+    set.full_arrivals = 3;  // the weights' load and the blocks' warps
   const uint32_t tmem_base = set_up<1>(p, map_w, map_t, s, base, warp, set, p.splits > 1);
   const int units = units_of(p, s, kTileF);
   if (warp == 0)
@@ -1238,6 +1273,9 @@ __global__ void __launch_bounds__(mxb200::kThreads, 1) mxb200_block_gemm_quantiz
 __global__ void __launch_bounds__(mxb200::kThreads, 1) mxb200_block_gemm_input_grad_few(const __grid_constant__ mxb200::Launch args) {
   mxb200::few::body<mxb200::kInputGrad, mxb200::few::Tile128>(args.p, &args.maps.a, &args.maps.b);
 }
+__global__ void __launch_bounds__(mxb200::kThreads, 1) mxb200_block_gemm_input_grad_32(const __grid_constant__ mxb200::Launch args) {
+  mxb200::few::body<mxb200::kInputGrad, mxb200::few::Tile32>(args.p, &args.maps.a, &args.maps.b);
+}
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(mxb200::kThreads, 1)
       mxb200_block_gemm_forward_many(const __grid_constant__ mxb200::Launch args) {
   mxb200::many::body<mxb200::kForward>(args.p, &args.maps.a, &args.maps.b, &args.maps.d);
@@ -1319,7 +1357,7 @@ struct Variant {
   int tokens, features; // of a unit
 };
 
-enum VariantId : int { kForwardFew, kForward32, kForwardMany, kForwardQuantizing, kInputGradFew, kInputGradMany, kWeightGradPair, kWeightGradLong, kForwardScaled, kInputGradScaled, kVariants };
+enum VariantId : int { kForwardFew, kForward32, kForwardMany, kForwardQuantizing, kInputGradFew, kInputGrad32, kInputGradMany, kWeightGradPair, kWeightGradLong, kForwardScaled, kInputGradScaled, kVariants };
 
 const Variant& variant(VariantId id) {
   static const Variant variants[kVariants] = {
@@ -1328,6 +1366,7 @@ const Variant& variant(VariantId id) {
         {mxb200_block_gemm_forward_many, many::kSmemBytes, 2, many::kTileT, many::kTileF},
         {mxb200_block_gemm_quantize_few, few::Quantizing::kSmemBytes, 1, few::Quantizing::kTileT, few::kTileF},
         {mxb200_block_gemm_input_grad_few, few::Tile128::kSmemBytes, 1, few::Tile128::kTileT, few::kTileF},
+        {mxb200_block_gemm_input_grad_32, few::Tile32::kSmemBytes, 1, few::Tile32::kTileT, few::kTileF},
         {mxb200_block_gemm_input_grad_many, many::kSmemBytes, 2, many::kTileT, many::kTileF},
         {mxb200_block_gemm_weight_grad, scaled::kSmemBytes, 2, scaled::kTile, scaled::kTile},
         {mxb200_block_gemm_weight_grad_long, scaled::kSmemBytes, 2, scaled::kTile, scaled::kTile},
@@ -1341,18 +1380,6 @@ const Variant& variant(VariantId id) {
 int64_t expected_tiles(int64_t tokens, int experts, int tile) {
   const int64_t used = std::min<int64_t>(experts, tokens);
   return experts == 1 ? blocks_up(tokens, tile) : std::max(used, tokens / tile + used / 2);
-}
-
-// Which of the two kernels a product of `blocks` contraction blocks to `features` features takes: the one that is expected to be
-// done first. Both take about 0.45 us for a block of their tile when all SMs are at work, a unit's output costs as much as 3 or 4
-// blocks, and a pair's tile is twice the work per SM of the other's. 16384 x 6144 -> 1536: few tokens 235 us, many 134; 2500 x
-// 1280 -> 3840: 27 and 20; 1111 x 1040 -> 2000: 7.6 and 8.8; 8192 rows over 32 experts, 1536 -> 2048: 59 and 42; 1000 rows over
-// 64: 39 and 54.
-bool many_tokens(int64_t tokens, int experts, int features, int blocks, int sms) {
-  const auto time = [&](const Variant& v, double out_blocks, double start) {
-    return start + static_cast<double>(blocks_up(expected_tiles(tokens, experts, v.tokens) * blocks_up(features, v.features), sms / v.ctas)) * (blocks + out_blocks) * 0.45;
-  };
-  return time(variant(kForwardMany), 4, 4.5) < time(variant(kForwardFew), 3, 4);
 }
 
 constexpr int kMostSplits = 8;
@@ -1394,16 +1421,66 @@ int configure(VariantId id, const DeviceInfo& dev, Configured* out) {
   return MXB200_OK;
 }
 
-// CTAs that share a unit's blocks: what is expected to take least, among those of which all units' clusters find room at once. A
-// block takes a CTA about 0.3 us, the exchange 2 us and 0.02 for each of the tile's tokens: one token of 6144 -> 1536 takes 16 us
-// in one CTA per unit and 6.9 in eight, 128 tokens of 1536 -> 6144 8.4 in one and 10.8 in two.
-int share_blocks(int64_t units, int blocks, int tile_tokens, const Configured& c) {
+int tile_tokens(int64_t tokens, int experts, int tile) {
+  return static_cast<int>(std::min<int64_t>(tile, blocks_up(tokens, experts)));
+}
+
+// Few tokens: CTAs that share a unit's blocks, what is expected to take least among those of which all units' clusters find room at
+// once. A block takes a CTA 0.17 us of a small tile and 0.3 of a large one or
+// where it is quantized (up to 16 tokens go by that, so that the result does not depend on who quantizes them), the exchange 2.5 us
+// and 0.02 for each of the tile's tokens. One token of 6144 -> 1536: 16.6 us in one CTA per unit and 7.5 in eight; 32 tokens of
+// 1536 -> 1536 5.1 in one and 6.2 in eight.
+int share_blocks(int64_t units, int blocks, int tile, int tokens, const Configured& c) {
+  const double block = tile == few::Tile32::kTileT && tokens > 16 ? 0.17 : 0.3;
   int best = 1;
-  double least = 0.3 * blocks;
+  double least = block * blocks;
   for (int n = 2; n <= std::min(kMostSplits, blocks) && units <= c.clusters[n]; ++n)
-    if (const double t = 0.3 * static_cast<double>(blocks_up(blocks, n)) + 2 + 0.02 * tile_tokens; t < least)
+    if (const double t = block * static_cast<double>(blocks_up(blocks, n)) + 2.5 + 0.02 * tokens; t < least)
       best = n, least = t;
   return best;
+}
+
+struct Plan {
+  VariantId id;
+  int splits;
+  int64_t units;  // expected
+};
+
+// The kernel that a product of `blocks` contraction blocks to `features` features takes: the one that is expected to be done first.
+// With all SMs at work a block of their tile takes about 0.2 us (32 tokens), 0.33 (128) and 0.37 (a pair's 256 x 256), a unit's
+// output costs as much as 2 to 4 blocks. In small, large and pairs' tiles: 256 x 1536 -> 1536 5.4, 7.9 and 9.2 us; 512 x 1536 ->
+// 6144 18.8, 13.5 and 10.2; 1111 x 1040 -> 2000 -, 8.3 and 8.9; 16384 x 1536 -> 1536 -, 59.7 and 41.2; 16 rows for each of 64 experts
+// (1536 -> 2048) 35.5, 38.5 and 54, 48 rows for each 48.4, 46.0 and -; 1024 rows over 8 experts (2048 -> 2048) -, 19.7 and 14.9.
+int plan_product(int64_t tokens, int experts, int features, int blocks, bool forward, const DeviceInfo& dev, Plan* plan) {
+  struct Kind {
+    VariantId id;
+    double start, output_blocks, block;
+  };
+  const Kind kinds[3] = {{forward ? kForward32 : kInputGrad32, 3, 2, 0.2}, {forward ? kForwardFew : kInputGradFew, 4, 3, 0.33}, {forward ? kForwardMany : kInputGradMany, 4.5, 4, 0.37}};
+  double least = 0;
+  for (const Kind& kind : kinds) {
+    const Variant& v = variant(kind.id);
+    Configured c;
+    if (const int st = configure(kind.id, dev, &c); st != MXB200_OK)
+      return st;
+    const int64_t units = expected_tiles(tokens, experts, v.tokens) * blocks_up(features, v.features);
+    const int of_tile = tile_tokens(tokens, experts, v.tokens);
+    const int splits = v.ctas == 1 ? share_blocks(units, blocks, v.tokens, of_tile, c) : 1;
+    const double t = kind.start + (splits > 1 ? 2.5 + 0.02 * of_tile : 0) +
+                     static_cast<double>(blocks_up(units, dev.sms / v.ctas)) * (blocks_up(blocks, splits) + kind.output_blocks) * kind.block;
+    if (least == 0 || t < least)
+      *plan = {kind.id, splits, units}, least = t;
+  }
+  return MXB200_OK;
+}
+
+// Whether a forward product of bf16 input takes less than the quantizer's launch and the product of its output, which is 2 to 3 us
+// and as much on the host: every CTA's repeating it costs about 0.014 us for a token of a block and 0.03 a block. One token of 1536
+// -> 6144: 6.6 us in one launch and 5.0 + 1.9 in two; 16 tokens 9.3 and 5.0 + 1.9; one token of 6144 -> 24576 35.2 and 29.6 + 1.9;
+// 16 rows over 16 experts (1536 -> 2048) 8.5 and 7.0 + 1.9, 64 rows over 64 experts 26.3 and 20.4 + 1.9.
+bool quantizes(int64_t tokens, int experts, int blocks, const DeviceInfo& dev, const Plan& plan) {
+  return plan.id == kForward32 && blocks_up(plan.units, dev.sms) * blocks_up(blocks, plan.splits) *
+                                        (tile_tokens(tokens, experts, few::Quantizing::kTileT) + 2) <= 140;
 }
 
 int block_gemm(const mxb200_block_gemm_args& g, cudaStream_t stream) {
@@ -1478,11 +1555,11 @@ int block_gemm(const mxb200_block_gemm_args& g, cudaStream_t stream) {
     st = st != MXB200_OK ? st : make_scale_map(&l.maps.a_scale, g.b_scale, blocks, capacity / kBlock, 1, 1);
     st = st != MXB200_OK ? st : make_scale_map(&l.maps.b_scale, g.a_scale, blocks_up(in, kBlock), blocks_up(out, kBlock) * g.experts, forward ? 1 : 2, forward ? 2 : 1);
   } else {
-    const bool many = !quantize && many_tokens(g.tokens, g.experts, to, blocks, dev.sms);
-    // the small tile as long as few experts need a second one: 600 rows over 64 experts (1536 -> 2048) take 36.7 us in small tiles
-    // and 38.8 in large ones, 1000 rows 41.2 and 40.0
-    const bool small = g.tokens <= few::Tile32::kTileT || g.tokens <= int64_t{12} * g.experts;
-    id = quantize ? kForwardQuantizing : many ? (forward ? kForwardMany : kInputGradMany) : !forward ? kInputGradFew : small ? kForward32 : kForwardFew;
+    Plan plan;
+    if (st = plan_product(g.tokens, g.experts, to, blocks, forward, dev, &plan); st != MXB200_OK)
+      return st;
+    id = quantize ? kForwardQuantizing : plan.id;
+    const bool many = id == kForwardMany || id == kInputGradMany;
     const Variant& v = variant(id);
     p.weight_scale = static_cast<const float*>(g.a_scale), p.token_scale = static_cast<const float*>(g.b_scale);
     p.token_ld = quantize ? g.b_ld : g.tokens, p.features = to, p.blocks = blocks;
@@ -1493,8 +1570,8 @@ int block_gemm(const mxb200_block_gemm_args& g, cudaStream_t stream) {
     if (st = configure(id, dev, &configured); st != MXB200_OK)
       return st;
     if (!many)
-      p.splits = share_blocks(expected_tiles(g.tokens, g.experts, v.tokens) * blocks_up(to, v.features), blocks,
-                              static_cast<int>(std::min<int64_t>(v.tokens, blocks_up(g.tokens, g.experts))), configured);
+      p.splits = share_blocks(expected_tiles(g.tokens, g.experts, v.tokens) * blocks_up(to, v.features), blocks, v.tokens,
+                              tile_tokens(g.tokens, g.experts, v.tokens), configured);
     CUtensorMap *weight = many ? &l.maps.b : &l.maps.a, *token = many ? &l.maps.a : &l.maps.b;
     st = make_map(weight, g.a, in, out, g.experts, 128);
     st = st != MXB200_OK || quantize ? st : make_map(token, g.b, from, g.tokens, 1, many ? 128 : 32);
@@ -1535,8 +1612,21 @@ extern "C" int mxb200_block_scaled(int64_t tokens, int64_t in_features, int64_t 
   DeviceInfo dev;
   if (tokens <= 0 || in_features <= 0 || out_features <= 0 || experts <= 0 || current_device(&dev) != MXB200_OK)
     return 0;
-  return many_tokens(tokens, experts, static_cast<int>(out_features), static_cast<int>(blocks_up(in_features, kBlock)), dev.sms) &&
-         many_tokens(tokens, experts, static_cast<int>(in_features), static_cast<int>(blocks_up(out_features, kBlock)), dev.sms);
+  const int in_blocks = static_cast<int>(blocks_up(in_features, kBlock)), out_blocks = static_cast<int>(blocks_up(out_features, kBlock));
+  Plan plan;
+  return plan_product(tokens, experts, static_cast<int>(out_features), in_blocks, true, dev, &plan) == MXB200_OK && plan.id == kForwardMany &&
+         plan_product(tokens, experts, static_cast<int>(in_features), out_blocks, false, dev, &plan) == MXB200_OK && plan.id == kInputGradMany;
+}
+
+extern "C" int mxb200_block_quantizes(int64_t tokens, int64_t in_features, int64_t out_features, int experts) {
+  using namespace mxb200;
+  DeviceInfo dev;
+  if (tokens <= 0 || in_features <= 0 || out_features <= 0 || experts <= 0 || current_device(&dev) != MXB200_OK)
+    return 0;
+  const int blocks = static_cast<int>(blocks_up(in_features, kBlock));
+  Plan plan;
+  return plan_product(tokens, experts, static_cast<int>(out_features), blocks, true, dev, &plan) == MXB200_OK &&
+         quantizes(tokens, experts, blocks, dev, plan);
 }
 
 extern "C" int mxb200_block_gemm(const mxb200_block_gemm_args* args, void* stream) {

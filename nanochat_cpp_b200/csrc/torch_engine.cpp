@@ -1068,7 +1068,7 @@ void block_product(int kind, const Block& a, const Block& b, const Tensor& d, co
 }
 
 // The forward product of so few tokens that it quantizes them itself rather than wait for a launch that does: one token of 1536
-// features to 1536 takes 8.5 us in two launches and 6.0 in one.
+// features to 1536 takes 8.5 us in two launches and 6.0 in one (mxb200_block_quantizes).
 void block_product_of(const Tensor& x, const Block& w, const Tensor& y, const Experts& e, int64_t tokens, int64_t in, int64_t out) {
   const mxb200_block_gemm_args g{w.data, w.scale, x.data_ptr(), nullptr, y.data_ptr(), e.ends, tokens, in, out, e.count,
                                  MXB200_BLOCK_FORWARD, MXB200_OUT_BF16, tokens > 1 ? x.stride(0) : in};
@@ -1121,9 +1121,7 @@ struct BlockLinear : torch::autograd::Function<BlockLinear> {
     const bool grad_x = ctx != nullptr && c.x.defined() && c.x.requires_grad();
     const Experts e = c.experts();
     Block tokens;
-    // (32 rows over 64 experts take 15.2 us in one launch and 14.0 + 1.9 in two, 64 rows 26.8 and 23.1 + 1.9)
-    const int64_t few = std::max<int64_t>(MXB200_BLOCK_FEW_TOKENS, e.count / 2);
-    const bool by_product = !grad_w && !c.x_rows && c.tokens <= few;
+    const bool by_product = !grad_w && !c.x_rows && mxb200_block_quantizes(c.tokens, c.in, c.out, e.count);
     // a training pass that quantizes both operands itself, to powers of two: for many tokens the tensor core scales
     const bool scaled = grad_w && !c.x_rows && !c.w_blocks && mxb200_block_scaled(c.tokens, c.in, c.out, e.count);
     if (!c.x_rows && !by_product) {

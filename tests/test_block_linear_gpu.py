@@ -140,6 +140,20 @@ def test_experts_quantized_by_the_product(nc, counts):
         assert not y[sum(counts):].any()
 
 
+@pytest.mark.parametrize("tokens,cin,cout,experts", [
+    (1, 1536, 1536, 1), (16, 1536, 400, 1), (100, 128, 144, 1), (40, 272, 640, 1), (32, 1536, 272, 16), (24, 272, 400, 80), (200, 128, 128, 40)])
+def test_bits_do_not_depend_on_who_quantizes(nc, tokens, cin, cout, experts):
+    g = generator(23)
+    assert nc.capi.lib.mxb200_block_quantizes(tokens, cin, cout, experts)
+    x, w = activation(g, tokens, cin), given_weight(nc, g, experts, cout, cin)
+    if experts == 1:
+        w = nc.BlockTensor(w.data[0], w.scale[0])
+        assert torch.equal(nc.fp8_block_matmul(x, w), nc.fp8_block_matmul(None, w, x_block=nc.quantize_block(x)))
+    else:
+        ends = torch.sort(torch.randint(0, tokens + 1, (experts,), generator=g, device="cuda")).values.int()
+        assert torch.equal(nc.fp8_block_experts(x, w, ends), nc.fp8_block_experts(None, w, ends, x_block=nc.quantize_block(x)))
+
+
 @pytest.mark.parametrize("tokens", [1, 16, 129, 384, 1000])
 @pytest.mark.parametrize("cin,cout", [(16, 16), (272, 144), (128, 640), (1040, 2000)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
