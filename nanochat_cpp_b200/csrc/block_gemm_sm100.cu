@@ -31,6 +31,7 @@
 #include "block_common.cuh"
 #include "internal.h"
 #include "ptx_sm100.cuh"
+#include "register_split.h"
 
 namespace mxb200 {
 
@@ -42,13 +43,15 @@ namespace {
 constexpr uint64_t kWaitLimitNs = 2000000000ull;
 constexpr uint32_t kTmemCols = 512;
 constexpr int kEpilogueWarps = 8;
-// Warps 0 to 2 load operands, issue MMAs and load scales, warp 3 idles; 4 to 11 are the epilogue. The epilogue warps of the
-// pair kernel need more registers than an even share (168 of 384 threads): they draw on the first four warps' (setmaxnreg; the
-// sum, 128 x 72 + 256 x 216, is what the block was launched with).
+// Warps 0 to 2 load operands, issue MMAs and load scales, warp 3 idles; 4 to 11 are the epilogue. The epilogue warps of `many`
+// and of the long weight gradient need more registers than an even share (168 of 384 threads): they draw on the first four
+// warps'. The sum, 128 x 72 + 256 x 216, is what a block of 168 a thread is launched with; configure() refuses a build in which
+// the compiler gave those kernels fewer.
 constexpr int kFirstEpilogueWarp = 4;
 constexpr int kThreads = 32 * (kFirstEpilogueWarp + kEpilogueWarps);
-constexpr int kLaunchRegisters = 168, kFewRegisters = 72, kManyRegisters = 216;
-static_assert(4 * kFewRegisters + kEpilogueWarps * kManyRegisters <= (4 + kEpilogueWarps) * kLaunchRegisters, "registers of the block");
+constexpr int kFewRegisters = 72, kManyRegisters = 216;
+constexpr RegisterSplit kTraded{kFirstEpilogueWarp, kFewRegisters, kEpilogueWarps, kManyRegisters}, kNotTraded{};
+static_assert(kTraded.needed() * kThreads <= 65536, "registers of an SM");
 constexpr int kScaleSlots = 8;
 constexpr uint32_t kABytes = 128 * 128, kBBytes = 128 * 128;
 constexpr uint32_t kBBoxBytes = 32 * 128;  // few tokens' rows come 32 at a time, as many as the tile has
@@ -1355,6 +1358,7 @@ struct Variant {
   size_t smem;
   int ctas;             // per unit
   int tokens, features; // of a unit
+  RegisterSplit registers = kNotTraded;
 };
 
 enum VariantId : int { kForwardFew, kForward32, kForwardMany, kForwardQuantizing, kInputGradFew, kInputGrad32, kInputGradMany, kWeightGradPair, kWeightGradLong, kForwardScaled, kInputGradScaled, kVariants };
@@ -1363,13 +1367,13 @@ const Variant& variant(VariantId id) {
   static const Variant variants[kVariants] = {
         {mxb200_block_gemm_forward_few, few::Tile128::kSmemBytes, 1, few::Tile128::kTileT, few::kTileF},
         {mxb200_block_gemm_forward_32, few::Tile32::kSmemBytes, 1, few::Tile32::kTileT, few::kTileF},
-        {mxb200_block_gemm_forward_many, many::kSmemBytes, 2, many::kTileT, many::kTileF},
+        {mxb200_block_gemm_forward_many, many::kSmemBytes, 2, many::kTileT, many::kTileF, kTraded},
         {mxb200_block_gemm_quantize_few, few::Quantizing::kSmemBytes, 1, few::Quantizing::kTileT, few::kTileF},
         {mxb200_block_gemm_input_grad_few, few::Tile128::kSmemBytes, 1, few::Tile128::kTileT, few::kTileF},
         {mxb200_block_gemm_input_grad_32, few::Tile32::kSmemBytes, 1, few::Tile32::kTileT, few::kTileF},
-        {mxb200_block_gemm_input_grad_many, many::kSmemBytes, 2, many::kTileT, many::kTileF},
+        {mxb200_block_gemm_input_grad_many, many::kSmemBytes, 2, many::kTileT, many::kTileF, kTraded},
         {mxb200_block_gemm_weight_grad, scaled::kSmemBytes, 2, scaled::kTile, scaled::kTile},
-        {mxb200_block_gemm_weight_grad_long, scaled::kSmemBytes, 2, scaled::kTile, scaled::kTile},
+        {mxb200_block_gemm_weight_grad_long, scaled::kSmemBytes, 2, scaled::kTile, scaled::kTile, kTraded},
         {mxb200_block_gemm_forward_scaled, scaled::kSmemBytes, 2, scaled::kTile, scaled::kTile},
         {mxb200_block_gemm_input_grad_scaled, scaled::kSmemBytes, 2, scaled::kTile, scaled::kTile}};
   return variants[id];
@@ -1384,7 +1388,7 @@ int64_t expected_tiles(int64_t tokens, int experts, int tile) {
 
 constexpr int kMostSplits = 8;
 
-// What the current device does with a kernel, looked up once: its shared memory, and how many clusters of 1 to 8 of its CTAs
+// What the current device does with a kernel, looked up once: its registers, its shared memory, and how many clusters of 1 to 8 of its CTAs
 // find room at a time (a cluster stays within one of the GPU's groups of SMs: 15 clusters of 8, 33 of 4, 45 of 3).
 struct Configured {
   bool done = false;
@@ -1400,7 +1404,9 @@ int configure(VariantId id, const DeviceInfo& dev, Configured* out) {
   if (!c.done) {
     const Variant& v = variant(id);
     const void* const kernel = reinterpret_cast<const void*>(v.kernel);
-    bool ok = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(v.smem)) == cudaSuccess;
+    cudaFuncAttributes built{};
+    bool ok = cudaFuncGetAttributes(&built, kernel) == cudaSuccess && v.registers.served_by(built.numRegs) &&
+              cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(v.smem)) == cudaSuccess;
     for (int n = 2; ok && v.ctas == 1 && n <= kMostSplits; ++n) {
       cudaLaunchAttribute attribute{};
       attribute.id = cudaLaunchAttributeClusterDimension;
