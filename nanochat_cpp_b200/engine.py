@@ -577,8 +577,8 @@ def _block_operands(w, x_block, cache):
     x_data, x_scale = (None, None) if x_block is None else (x_block.data, x_block.scale)
     if isinstance(w, BlockTensor):
         return None, x_data, x_scale, w.data, w.scale
-    if cache is None:
-        return w, x_data, x_scale, None, None
+    if cache is None or (getattr(type(cache), "get", None) is native.WeightCache.get and not cache.enabled):
+        return w, x_data, x_scale, None, None  # a cache that is switched off is none
     w_data, w_scale = cache.get(2, [w], lambda: list(native.quantize_block_weight(w)))
     return w, x_data, x_scale, w_data, w_scale
 
