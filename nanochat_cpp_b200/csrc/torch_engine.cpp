@@ -1163,15 +1163,18 @@ struct BlockLinear : torch::autograd::Function<BlockLinear> {
     const Tensor go = readable_rows(grads[0]);
     const auto device = go.device();
     const Experts e = matrices > 0 ? Experts{static_cast<const int32_t*>(saved[4].data_ptr()), static_cast<int>(matrices)} : Experts{};
-    const bool grad_x = saved[0].defined(), grad_w = saved[2].defined() || saved[3].defined();
-    const bool scaled = sizes[5] != 0;  // then the weight gets a gradient too
+    // what forward kept something for and this pass asks for; the input is the node's first edge, a weight its second
+    const bool grad_x = saved[0].defined() && ctx->needs_input_grad(0);
+    const bool grad_w = (saved[2].defined() || saved[3].defined()) && ctx->needs_input_grad(1);
+    const bool scaled = sizes[5] != 0;
+    const bool rows_in_blocks = scaled && grad_x, by_token = grad_w || rows_in_blocks;  // rows in blocks come with the other layout
     Block g_rows, g_tokens;
     if (grad_x)
       g_rows = scaled ? new_rows_in_blocks(tokens, out, e, device) : new_row_blocks(tokens, out, device);
-    if (grad_w)
+    if (by_token)
       g_tokens = new_token_blocks(tokens, out, e, device);
     if (grad_x || grad_w)
-      quantize_blocks(go, grad_w ? e : Experts{}, g_rows, g_tokens, scaled && grad_x);
+      quantize_blocks(go, by_token ? e : Experts{}, g_rows, g_tokens, rows_in_blocks);
     Tensor dx, dw;
     if (grad_w) {
       Block x_tokens;
