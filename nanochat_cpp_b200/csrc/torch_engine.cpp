@@ -1310,7 +1310,9 @@ struct ResidualNormBlock : torch::autograd::Function<ResidualNormBlock> {
     require(!at::GradMode::is_enabled(), "residual_norm_block: its backward has no derivative (create_graph)");
     const auto saved = ctx->get_saved_variables();
     const Tensor &res = saved[0], &rstd = saved[1], &gain = saved[2];
-    const bool has_r = ctx->saved_data["r"].toBool(), want_gain = ctx->saved_data["want_gain"].toBool();
+    const bool has_r = ctx->saved_data["r"].toBool();
+    // the node's edges are those of the tensors that were given: x, r, gain
+    const bool want_gain = ctx->saved_data["want_gain"].toBool() && ctx->needs_input_grad(has_r ? 2 : 1);
     const Tensor dres = grads[0].defined() ? dense(grads[0]) : Tensor();
     Tensor dx, dgain;
     if (!grads[1].defined()) {

@@ -44,7 +44,7 @@ def test_linears(nc, tokens, scaled, experts):  # noqa: F811
     # a weight without a gradient of its own
     frozen = given_weight(nc, g, *w.shape)
     (dx,), for_x = launches_of(nc, lambda: torch.autograd.grad(forward(x, frozen), x, dy))
-    assert dx.shape == x.shape and for_x <= 2 + 2  # the forward's two among them
+    assert dx.shape == x.shape and for_x <= 4  # the forward's one or two among them
 
 
 def test_a_gradient_that_is_not_asked_for_takes_no_memory(nc):  # noqa: F811
@@ -69,3 +69,25 @@ def test_accumulated_into_the_leaves_that_want_it(nc):  # noqa: F811
     assert x.grad is None and torch.equal(w.grad, dw)
     y.backward(dy, inputs=[x])
     assert torch.equal(x.grad, dx) and torch.equal(w.grad, dw)
+
+
+@pytest.mark.parametrize("add", [True, False])
+@pytest.mark.parametrize("gain_type", [torch.float32, torch.bfloat16])
+def test_norm(nc, add, gain_type):  # noqa: F811
+    g = generator(4)
+    x = activation(g, 300, 528).requires_grad_()
+    r = torch.randn(300, 528, device="cuda", generator=g).bfloat16().requires_grad_() if add else None
+    gain = (1 + 0.2 * torch.randn(528, device="cuda", generator=g)).to(gain_type).requires_grad_()
+    dn = torch.randn(300, 528, device="cuda", generator=g).bfloat16()
+    res, n, _, _ = nc.residual_norm_block(x, r, gain)
+    (dx, dgain), both = launches_of(nc, lambda: torch.autograd.grad(n, (x, gain), dn, retain_graph=True))
+    (only_x,), for_x = launches_of(nc, lambda: torch.autograd.grad(n, x, dn, retain_graph=True))
+    (only_gain,), for_gain = launches_of(nc, lambda: torch.autograd.grad(n, gain, dn, retain_graph=True))
+    assert (both, for_x, for_gain) == (2, 1, 2)
+    assert torch.equal(only_x, dx) and torch.equal(only_gain, dgain)
+    if add:
+        (only_r,), for_r = launches_of(nc, lambda: torch.autograd.grad(n, r, dn, retain_graph=True))
+        assert for_r == 1 and torch.equal(only_r, dx)
+    # through the residual alone: the norm's gain has no part in it
+    (through,), none = launches_of(nc, lambda: torch.autograd.grad(res, x, dn))
+    assert none == 0 and torch.equal(through, dn)
