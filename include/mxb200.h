@@ -324,6 +324,11 @@ typedef struct mxb200_block_gemm_args {
 } mxb200_block_gemm_args;
 MXB200_API int mxb200_block_gemm(const mxb200_block_gemm_args* args, void* stream);
 
+/* Which kernel a call with these sizes takes on the current device, by the end of its name after mxb200_block_gemm_, and in
+ * *splits (optional) how many CTAs share a tile's contraction. Pointers are not looked at. Null where there is none: sizes that are
+ * refused, no tokens, no device. */
+MXB200_API const char* mxb200_block_gemm_kernel(const mxb200_block_gemm_args* args, int* splits);
+
 /* RMS norm behind a residual add, its result also in blocks of 128 along rows. All matrices (rows, cols) contiguous bf16,
  * cols % 16 == 0 and <= 16384, any number of rows.
  *   res = bf16(x + r); rstd = 1 / sqrt(mean(res^2) + eps); n = bf16(res * rstd * gain); q, scale as mxb200_block_quantize of n.

@@ -28,7 +28,7 @@ SYMBOLS = (
     "mxb200_count_valid", "mxb200_reduce_losses", "mxb200_scale_bf16",
     "mxb200_gemm_group_workspace_bytes", "mxb200_gemm_group",
     "mxb200_gemm_splits", "mxb200_gemm_workspace_bytes", "mxb200_gemm_splitk", "mxb200_gemm_splitk_static",
-    "mxb200_block_token_blocks", "mxb200_block_quantize", "mxb200_block_quantize_weight", "mxb200_block_gemm", "mxb200_block_scaled",
+    "mxb200_block_token_blocks", "mxb200_block_quantize", "mxb200_block_quantize_weight", "mxb200_block_gemm", "mxb200_block_gemm_kernel", "mxb200_block_scaled",
     "mxb200_block_quantizes",
     "mxb200_block_norm_fwd", "mxb200_block_norm_workspace_bytes", "mxb200_block_norm_bwd",
     "mxb200_strerror",
@@ -132,6 +132,8 @@ def _load() -> ctypes.CDLL:
     lib.mxb200_block_quantize_weight.argtypes = [vp, i32, i32, i64, i64, vp, vp, i32, vp]
     lib.mxb200_block_scaled.argtypes = lib.mxb200_block_quantizes.argtypes = [i64, i64, i64, i32]
     lib.mxb200_block_gemm.argtypes = [ctypes.POINTER(BlockGemmArgs), vp]
+    lib.mxb200_block_gemm_kernel.argtypes = [ctypes.POINTER(BlockGemmArgs), ctypes.POINTER(ctypes.c_int)]
+    lib.mxb200_block_gemm_kernel.restype = ctypes.c_char_p
     lib.mxb200_block_norm_fwd.argtypes = [ctypes.POINTER(BlockNormArgs), vp]
     lib.mxb200_block_norm_workspace_bytes.argtypes = [i64, ctypes.c_int32]
     lib.mxb200_block_norm_workspace_bytes.restype = ctypes.c_size_t

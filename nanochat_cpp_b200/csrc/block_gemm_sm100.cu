@@ -1354,6 +1354,7 @@ int make_scale_map(CUtensorMap* map, const void* base, int64_t y, int64_t z, int
 using Kernel = void (*)(Launch);
 
 struct Variant {
+  const char* name;
   Kernel kernel;
   size_t smem;
   int ctas;             // per unit
@@ -1365,17 +1366,17 @@ enum VariantId : int { kForwardFew, kForward32, kForwardMany, kForwardQuantizing
 
 const Variant& variant(VariantId id) {
   static const Variant variants[kVariants] = {
-        {mxb200_block_gemm_forward_few, few::Tile128::kSmemBytes, 1, few::Tile128::kTileT, few::kTileF},
-        {mxb200_block_gemm_forward_32, few::Tile32::kSmemBytes, 1, few::Tile32::kTileT, few::kTileF},
-        {mxb200_block_gemm_forward_many, many::kSmemBytes, 2, many::kTileT, many::kTileF, kTraded},
-        {mxb200_block_gemm_quantize_few, few::Quantizing::kSmemBytes, 1, few::Quantizing::kTileT, few::kTileF},
-        {mxb200_block_gemm_input_grad_few, few::Tile128::kSmemBytes, 1, few::Tile128::kTileT, few::kTileF},
-        {mxb200_block_gemm_input_grad_32, few::Tile32::kSmemBytes, 1, few::Tile32::kTileT, few::kTileF},
-        {mxb200_block_gemm_input_grad_many, many::kSmemBytes, 2, many::kTileT, many::kTileF, kTraded},
-        {mxb200_block_gemm_weight_grad, scaled::kSmemBytes, 2, scaled::kTile, scaled::kTile},
-        {mxb200_block_gemm_weight_grad_long, scaled::kSmemBytes, 2, scaled::kTile, scaled::kTile, kTraded},
-        {mxb200_block_gemm_forward_scaled, scaled::kSmemBytes, 2, scaled::kTile, scaled::kTile},
-        {mxb200_block_gemm_input_grad_scaled, scaled::kSmemBytes, 2, scaled::kTile, scaled::kTile}};
+        {"forward_few", mxb200_block_gemm_forward_few, few::Tile128::kSmemBytes, 1, few::Tile128::kTileT, few::kTileF},
+        {"forward_32", mxb200_block_gemm_forward_32, few::Tile32::kSmemBytes, 1, few::Tile32::kTileT, few::kTileF},
+        {"forward_many", mxb200_block_gemm_forward_many, many::kSmemBytes, 2, many::kTileT, many::kTileF, kTraded},
+        {"quantize_few", mxb200_block_gemm_quantize_few, few::Quantizing::kSmemBytes, 1, few::Quantizing::kTileT, few::kTileF},
+        {"input_grad_few", mxb200_block_gemm_input_grad_few, few::Tile128::kSmemBytes, 1, few::Tile128::kTileT, few::kTileF},
+        {"input_grad_32", mxb200_block_gemm_input_grad_32, few::Tile32::kSmemBytes, 1, few::Tile32::kTileT, few::kTileF},
+        {"input_grad_many", mxb200_block_gemm_input_grad_many, many::kSmemBytes, 2, many::kTileT, many::kTileF, kTraded},
+        {"weight_grad", mxb200_block_gemm_weight_grad, scaled::kSmemBytes, 2, scaled::kTile, scaled::kTile},
+        {"weight_grad_long", mxb200_block_gemm_weight_grad_long, scaled::kSmemBytes, 2, scaled::kTile, scaled::kTile, kTraded},
+        {"forward_scaled", mxb200_block_gemm_forward_scaled, scaled::kSmemBytes, 2, scaled::kTile, scaled::kTile},
+        {"input_grad_scaled", mxb200_block_gemm_input_grad_scaled, scaled::kSmemBytes, 2, scaled::kTile, scaled::kTile}};
   return variants[id];
 }
 
@@ -1489,7 +1490,7 @@ bool quantizes(int64_t tokens, int experts, int blocks, const DeviceInfo& dev, c
                                         (tile_tokens(tokens, experts, few::Quantizing::kTileT) + 2) <= 140;
 }
 
-int block_gemm(const mxb200_block_gemm_args& g, cudaStream_t stream) {
+int check_sizes(const mxb200_block_gemm_args& g) {
   if (g.kind < MXB200_BLOCK_FORWARD || g.kind > MXB200_BLOCK_INPUT_GRAD_SCALED ||
       (g.out_kind != MXB200_OUT_BF16 && (g.out_kind != MXB200_OUT_F32 || g.kind != MXB200_BLOCK_WEIGHT_GRAD)))
     return MXB200_ERR_ARGUMENT;
@@ -1500,6 +1501,45 @@ int block_gemm(const mxb200_block_gemm_args& g, cudaStream_t stream) {
     return MXB200_ERR_ARGUMENT;
   if (g.b_ld != 0 && (g.b_ld < g.in_features || g.b_ld % 8))
     return MXB200_ERR_SHAPE;
+  return MXB200_OK;
+}
+
+struct Choice {
+  VariantId id;
+  int splits;  // few tokens: CTAs that share a unit's blocks
+  Configured configured;
+};
+
+// The kernel of a call with checked sizes and at least one token.
+int choose(const mxb200_block_gemm_args& g, const DeviceInfo& dev, Choice* out) {
+  const bool forward = g.kind == MXB200_BLOCK_FORWARD || g.kind == MXB200_BLOCK_FORWARD_SCALED;
+  out->splits = 1;
+  if (g.kind == MXB200_BLOCK_WEIGHT_GRAD) {
+    out->id = g.tokens <= scaled::kSegment * kBlock ? kWeightGradPair : kWeightGradLong;
+    return configure(out->id, dev, &out->configured);
+  }
+  if (g.kind == MXB200_BLOCK_FORWARD_SCALED || g.kind == MXB200_BLOCK_INPUT_GRAD_SCALED) {
+    out->id = forward ? kForwardScaled : kInputGradScaled;
+    return configure(out->id, dev, &out->configured);
+  }
+  const int blocks = static_cast<int>(blocks_up(forward ? g.in_features : g.out_features, kBlock));
+  const int features = static_cast<int>(forward ? g.out_features : g.in_features);
+  Plan plan;
+  if (const int st = plan_product(g.tokens, g.experts, features, blocks, forward, dev, &plan); st != MXB200_OK)
+    return st;
+  out->id = g.b_ld != 0 ? kForwardQuantizing : plan.id;
+  const Variant& v = variant(out->id);
+  if (const int st = configure(out->id, dev, &out->configured); st != MXB200_OK)
+    return st;
+  if (v.ctas == 1)
+    out->splits = share_blocks(expected_tiles(g.tokens, g.experts, v.tokens) * blocks_up(features, v.features), blocks, v.tokens,
+                               tile_tokens(g.tokens, g.experts, v.tokens), out->configured);
+  return MXB200_OK;
+}
+
+int block_gemm(const mxb200_block_gemm_args& g, cudaStream_t stream) {
+  if (const int st = check_sizes(g); st != MXB200_OK)
+    return st;
   if (g.ends == nullptr && g.experts != 1)
     return MXB200_ERR_NULL;
   DeviceInfo dev;
@@ -1530,18 +1570,18 @@ int block_gemm(const mxb200_block_gemm_args& g, cudaStream_t stream) {
   Params& p = l.p;
   p.d = g.d, p.ends = g.ends, p.experts = g.experts, p.rows = static_cast<int>(g.tokens);
   p.out_bf16 = g.out_kind == MXB200_OUT_BF16;
-  p.splits = 1;
   // token tiles are known on the device only; this many at most
   const auto most_tiles = [&](int64_t tile) {
     return g.ends == nullptr ? blocks_up(g.tokens, tile) : (g.tokens + (tile - 1) * std::min<int64_t>(g.experts + 1, g.tokens)) / tile;
   };
-  VariantId id = g.tokens <= mxb200::scaled::kSegment * kBlock ? kWeightGradPair : kWeightGradLong;
-  Configured configured;
+  Choice choice;
+  int st = choose(g, dev, &choice);
+  if (st != MXB200_OK)
+    return st;
+  const Variant& v = variant(choice.id);
+  p.splits = choice.splits;
   int64_t units;
-  int st;
   if (wgrad) {
-    if (st = configure(id, dev, &configured); st != MXB200_OK)
-      return st;
     const int64_t capacity = mxb200_block_token_blocks(g.tokens, g.experts) * kBlock;
     p.features = static_cast<int>(out), p.n = static_cast<int>(in);
     units = g.experts * blocks_up(out, mxb200::scaled::kTile) * blocks_up(in, mxb200::scaled::kTile);
@@ -1550,9 +1590,6 @@ int block_gemm(const mxb200_block_gemm_args& g, cudaStream_t stream) {
     st = st != MXB200_OK ? st : make_scale_map(&l.maps.a_scale, g.a_scale, blocks_up(out, kBlock), capacity / kBlock, 1, 1);
     st = st != MXB200_OK ? st : make_scale_map(&l.maps.b_scale, g.b_scale, blocks_up(in, kBlock), capacity / kBlock, 2, 1);
   } else if (scaled) {
-    id = forward ? kForwardScaled : kInputGradScaled;
-    if (st = configure(id, dev, &configured); st != MXB200_OK)
-      return st;
     const int64_t capacity = mxb200_block_token_blocks(g.tokens, g.experts) * kBlock;
     p.features = to, p.blocks = blocks, p.w_scale_rows = static_cast<int>(blocks_up(out, kBlock));
     units = most_tiles(mxb200::scaled::kTile) * blocks_up(to, mxb200::scaled::kTile);
@@ -1561,23 +1598,13 @@ int block_gemm(const mxb200_block_gemm_args& g, cudaStream_t stream) {
     st = st != MXB200_OK ? st : make_scale_map(&l.maps.a_scale, g.b_scale, blocks, capacity / kBlock, 1, 1);
     st = st != MXB200_OK ? st : make_scale_map(&l.maps.b_scale, g.a_scale, blocks_up(in, kBlock), blocks_up(out, kBlock) * g.experts, forward ? 1 : 2, forward ? 2 : 1);
   } else {
-    Plan plan;
-    if (st = plan_product(g.tokens, g.experts, to, blocks, forward, dev, &plan); st != MXB200_OK)
-      return st;
-    id = quantize ? kForwardQuantizing : plan.id;
-    const bool many = id == kForwardMany || id == kInputGradMany;
-    const Variant& v = variant(id);
+    const bool many = v.ctas == 2;
     p.weight_scale = static_cast<const float*>(g.a_scale), p.token_scale = static_cast<const float*>(g.b_scale);
     p.token_ld = quantize ? g.b_ld : g.tokens, p.features = to, p.blocks = blocks;
     p.input = g.b, p.input_cols = from;
     p.w_scale_expert = blocks_up(out, kBlock) * blocks_up(in, kBlock);
     p.w_scale_f = forward ? static_cast<int>(blocks_up(in, kBlock)) : 1, p.w_scale_b = forward ? 1 : static_cast<int>(blocks_up(in, kBlock));
     units = most_tiles(v.tokens) * blocks_up(to, v.features);
-    if (st = configure(id, dev, &configured); st != MXB200_OK)
-      return st;
-    if (!many)
-      p.splits = share_blocks(expected_tiles(g.tokens, g.experts, v.tokens) * blocks_up(to, v.features), blocks, v.tokens,
-                              tile_tokens(g.tokens, g.experts, v.tokens), configured);
     CUtensorMap *weight = many ? &l.maps.b : &l.maps.a, *token = many ? &l.maps.a : &l.maps.b;
     st = make_map(weight, g.a, in, out, g.experts, 128);
     st = st != MXB200_OK || quantize ? st : make_map(token, g.b, from, g.tokens, 1, many ? 128 : 32);
@@ -1587,8 +1614,7 @@ int block_gemm(const mxb200_block_gemm_args& g, cudaStream_t stream) {
     return st;
   if (units > kMostSize)
     return MXB200_ERR_SHAPE;
-  const Variant& v = variant(id);
-  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(units, configured.clusters[p.splits])) * std::max(v.ctas, p.splits);
+  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(units, choice.configured.clusters[p.splits])) * std::max(v.ctas, p.splits);
   return launch_kernel_clusters(p.splits > 1 ? p.splits : 0, v.kernel, grid, kThreads, v.smem, stream, l);
 }
 
@@ -1633,6 +1659,18 @@ extern "C" int mxb200_block_quantizes(int64_t tokens, int64_t in_features, int64
   Plan plan;
   return plan_product(tokens, experts, static_cast<int>(out_features), blocks, true, dev, &plan) == MXB200_OK &&
          quantizes(tokens, experts, blocks, dev, plan);
+}
+
+extern "C" const char* mxb200_block_gemm_kernel(const mxb200_block_gemm_args* args, int* splits) {
+  using namespace mxb200;
+  DeviceInfo dev;
+  Choice choice;
+  if (args == nullptr || check_sizes(*args) != MXB200_OK || args->tokens == 0 || current_device(&dev) != MXB200_OK ||
+      choose(*args, dev, &choice) != MXB200_OK)
+    return nullptr;
+  if (splits != nullptr)
+    *splits = choice.splits;
+  return variant(choice.id).name;
 }
 
 extern "C" int mxb200_block_gemm(const mxb200_block_gemm_args* args, void* stream) {
