@@ -514,13 +514,8 @@ __device__ __forceinline__ void tcgen05_mma_f8_pair(uint32_t pred, uint32_t d_tm
 
 // ---------------------------------------------------------------------------------------------- fragments
 
-// Four 8 x 8 matrices of 16-bit values, one fragment register each, into shared memory: lane l gives the address of row
-// l % 8 of matrix l / 8 (16 bytes, 16-byte aligned). The transposed form stores the matrices' columns as those rows.
-__device__ __forceinline__ void stmatrix_x4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-  asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d)
-               : "memory");
-}
-
+// Four 8 x 8 matrices of 16-bit values, one fragment register each, their columns as rows in shared memory: lane l gives the
+// address of row l % 8 of matrix l / 8 (16 bytes, 16-byte aligned).
 __device__ __forceinline__ void stmatrix_x4_trans(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d)
                : "memory");
