@@ -1542,6 +1542,8 @@ int block_gemm(const mxb200_block_gemm_args& g, cudaStream_t stream) {
     return st;
   if (g.ends == nullptr && g.experts != 1)
     return MXB200_ERR_NULL;
+  if ((reinterpret_cast<uintptr_t>(g.ends) & 3) != 0)
+    return MXB200_ERR_ALIGNMENT;
   DeviceInfo dev;
   if (int st = current_device(&dev); st != MXB200_OK)
     return st;
@@ -1559,7 +1561,7 @@ int block_gemm(const mxb200_block_gemm_args& g, cudaStream_t stream) {
   if (g.a == nullptr || g.a_scale == nullptr || g.b == nullptr || (g.b_scale == nullptr && !quantize) || g.d == nullptr)
     return MXB200_ERR_NULL;
   const auto bits = [](const void* q) { return reinterpret_cast<uintptr_t>(q); };
-  if (!aligned16(g.a) || !aligned16(g.b) || !aligned16(g.d) || (bits(g.ends) & 3) != 0 ||
+  if (!aligned16(g.a) || !aligned16(g.b) || !aligned16(g.d) ||
       ((bits(g.a_scale) | bits(g.b_scale)) & (wgrad || scaled ? 15 : 3)) != 0)
     return MXB200_ERR_ALIGNMENT;
   const int64_t in = g.in_features, out = g.out_features;

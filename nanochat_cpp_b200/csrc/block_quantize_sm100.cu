@@ -321,6 +321,8 @@ extern "C" int mxb200_block_quantize(const void* x, int64_t rows, int64_t cols, 
     return MXB200_ERR_SHAPE;
   if (ends == nullptr && experts != 1)
     return MXB200_ERR_NULL;
+  if ((reinterpret_cast<uintptr_t>(ends) & 3) != 0)
+    return MXB200_ERR_ALIGNMENT;
   if (rows == 0)
     return MXB200_OK;
   const bool want_rows = row_data != nullptr, want_tokens = token_data != nullptr;
