@@ -591,7 +591,13 @@ def fp8_block_matmul(x: Optional[torch.Tensor], w, x_block: Optional[BlockTensor
     no gradient.
 
     Gradients come through autograd, the weight's in its own type. They use the incoming gradient in blocks along its rows for
-    dx, and gradient and input in blocks of 128 tokens for dw."""
+    dx, and gradient and input in blocks of 128 tokens for dw.
+
+    A pass that makes both operands' blocks itself for a weight with a gradient lets the tensor core apply the scales where the
+    tokens are many (mxb200_block_scaled). That is faster, and y and dx may differ in a last bit from the same call under no_grad,
+    with x_block, or with a cache that is on, which all go by the products for any scales. So leave x_block out in training of many
+    tokens: norm and Linear of 16384 x 1536 -> 6144, forward and backward, take 564 us without it and 574 with it, 2048 tokens 107
+    and 115; 1111 x 1040 -> 2000, which is not scaled, 57 and 54."""
     return native.fp8_block_matmul(x, *_block_operands(w, x_block, cache))
 
 
@@ -609,7 +615,7 @@ def residual_norm_block(x: torch.Tensor, r: Optional[torch.Tensor] = None, gain:
                         eps: float = torch.finfo(torch.float32).eps, with_n: bool = True):
     """res = x + r (bf16), n = rms_norm(res) * gain, and n in blocks of 128: (res, n, n_block, rstd). x, r: bf16 (..., C), C a
     multiple of 16 up to 16384; gain: (C) bf16 or fp32. n_block is quantize_block(n.view(-1, C)), bit for bit: hand it to
-    fp8_block_matmul or fp8_block_experts as x_block, with n as x. Without r, res is x. Gradients reach x, r and gain through res
+    fp8_block_matmul or fp8_block_experts as x_block, with n.view(-1, C) as x (but see fp8_block_matmul for training). Without r, res is x. Gradients reach x, r and gain through res
     and n. with_n=False (no gradients then): n is not written and None."""
     res, n, data, scale, rstd = native.residual_norm_block(x, r, gain, eps, with_n)
     return res, n, BlockTensor(data, scale), rstd
