@@ -337,7 +337,8 @@ MXB200_API const char* mxb200_block_gemm_kernel(const mxb200_block_gemm_args* ar
 /* RMS norm behind a residual add, its result also in blocks of 128 along rows. All matrices (rows, cols) contiguous bf16,
  * cols % 16 == 0 and <= 16384, any number of rows.
  *   res = bf16(x + r); rstd = 1 / sqrt(mean(res^2) + eps); n = bf16(res * rstd * gain); q, scale as mxb200_block_quantize of n.
- * Without r, res is x itself and not written (both null). */
+ * Without r, res is x itself and not written (both null). The squares are summed in fp32: a row whose sum of them passes 3.4e38
+ * (values of about 1e18) gets rstd = 0, and with eps = 0 one whose squares vanish (1e-23) rstd = infinity. */
 typedef struct mxb200_block_norm_args {
   const void* x;
   const void* r;    /* optional, with res */
