@@ -10,7 +10,7 @@ using mxb200::RegisterSplit;
 constexpr RegisterSplit split{4, 72, 8, 216};
 static_assert(split.needed() == 168);
 static_assert(split.served_by(168) && split.served_by(255));
-// 128 x 72 + 256 x 216 registers from a block of 384 x 160: the last warps would wait for 3072 that nobody has
+// 128 x 72 + 256 x 216 registers from a block of 384 x 160: the last warps would wait for some that nobody has
 static_assert(!split.served_by(160) && !split.served_by(167) && !split.served_by(128));
 static_assert(RegisterSplit{4, 40, 8, 121}.needed() == 94);  // rounded up
 static_assert(RegisterSplit{}.needed() == 0 && RegisterSplit{}.served_by(32));
